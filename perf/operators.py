@@ -220,7 +220,8 @@ def _own_state(s, seed, rounds, pages):
     history = _history(case, seed, rounds)
     torch.cuda.synchronize()         # calls without a stream run on the handle's own
     for h, a, x in history:
-        kv.plan(_int(h).data_ptr(), _int(a).data_ptr(), int(a.sum()))
+        before, more = _int(h), _int(a)
+        kv.plan(before.data_ptr(), more.data_ptr(), int(a.sum()))
         if x is not None and x.shape[0]:
             k, v = _parts(case, x)
             kv.append(0, k.data_ptr(), v.data_ptr(), s["type"], x.shape[1], x.shape[1])
