@@ -10,11 +10,13 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "lib")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+SOURCES = ["q4hip.hip", "kv8.hip"]
 NODE_INCLUDE = os.environ.get("NODE_INCLUDE", "/usr/include/node")
 
 # -ffp-contract=off: no multiply-add fusion, so every binary32 operation rounds once as on the CPU.
@@ -39,7 +41,12 @@ def build_hip() -> str:
     os.makedirs(LIB, exist_ok=True)
     out = os.path.join(LIB, "libq4hip.so")
     tmp = out + ".tmp"
-    _run([HIPCC, *HIP_FLAGS, "-shared", "-o", tmp, os.path.join(PKG, "csrc", "q4hip.hip")])
+    objects = [os.path.join(LIB, n + ".o") for n in SOURCES]
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        list(pool.map(lambda n, o: _run([HIPCC, *HIP_FLAGS, "-c", "-o", o, os.path.join(PKG, "csrc", n)]), SOURCES, objects))
+    _run([HIPCC, *HIP_FLAGS, "-shared", "-o", tmp, *objects])
+    for o in objects:
+        os.remove(o)
     os.replace(tmp, out)
     return out
 

@@ -1,0 +1,61 @@
+// kv8.h -- the paged K/V cache in 8 bits: its layout, and what the other translation units launch of it.
+//
+// A page holds kKv8Block = 32 positions of one sequence in one layer.  Per (layer, page, kv head) there
+// are 32 x HD codes of K, then as many of V, and one fp32 scale for each: a value is scale * code, the
+// code in -127..127 held as code + 128 in a byte.  Which 16 bytes a lane loads at once is laid out as the
+// matrix cores take them (v_mfma_f32_16x16x32_f16: lane l holds row l % 16 and the 8 values of quarter
+// l / 16 of the contraction):
+//   K  byte of (position t, column d): the rows of the operand are 16 positions, the contraction 32
+//      columns; one 16-byte load holds a lane's 8 columns of two contractions, 64 columns apart by halves
+//   V  the rows are 16 columns, the contraction the 32 positions of the page in the order in which the
+//      scores of 16 x 16 tiles lie in the lanes (quarter g: 4g..4g+3, then 16+4g..16+4g+3); one load holds a
+//      lane's 8 positions of two neighbouring tiles of columns
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace q4 {
+
+constexpr int kKv8Block = 32;
+constexpr float kKv8MinScale = 0x1p-100f;     // a smaller scale is 0, and so are the values
+
+__host__ __device__ constexpr int kv8_k_byte(int HD, int t, int d) {
+  const int lane = ((d >> 3) & 3) * 16 + (t & 15);
+  return (((t >> 4) * (HD / 64) + (d >> 6)) * 64 + lane) * 16 + ((d >> 5) & 1) * 8 + (d & 7);
+}
+__host__ __device__ constexpr int kv8_v_byte(int t, int d) {
+  const int lane = ((t >> 2) & 3) * 16 + (d & 15);
+  return ((d >> 5) * 64 + lane) * 16 + ((d >> 4) & 1) * 8 + (t >> 4) * 4 + (t & 3);
+}
+
+// What a plan says of itself.
+struct Kv8Head {
+  int status;      // KV8_*
+  int rows;        // rows of the plan, 0 when it failed
+  int free_pages;
+};
+enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES };
+
+// The device side of a cache.
+struct Kv8View {
+  uint8_t* codes;      // [layers][pages][kv_heads][K, V][32 * HD]
+  float2* scales;      // [layers][pages][kv_heads] of K, V
+  int* table;          // [seqs][blocks] pages, -1 past those a sequence holds
+  int* held;           // [seqs] pages of a sequence
+  int* stack;          // [pages] free pages, the next one to take last
+  Kv8Head* head;
+  int *base, *lens;    // [seqs] positions before and after the step
+  int* starts;         // [seqs + 1] first row of a sequence in the step
+  int *seq, *pos, *slot;   // [max_rows] of a row: sequence, position, 32 * page + position % 32
+  int layers, H, KVH, HD, B, W, pages, max_len;
+};
+
+}  // namespace q4
+
+struct q4hip_kv8 {
+  q4::Kv8View v{};
+  int device = 0, max_rows = 0;
+  int rows = 0;                // rows the last plan was called for
+  hipStream_t stream = nullptr;
+  q4::Kv8Head* pin = nullptr;  // pinned copy of v.head
+};

@@ -1,0 +1,516 @@
+// kv8.hip -- the paged 8-bit K/V cache: plan, append, read and attention (include/q4hip.h, q4hip_kv8_*).
+#include "kv8.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "host.h"
+
+namespace q4 {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// Inclusive sum over the workgroup's threads; *total receives the sum of all.  `part`: one int per wave.
+__device__ int wg_scan(int v, int* part, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  __syncthreads();                       // `part` of the scan before has been read
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < waves; w++) {
+    if (w < wave) before += part[w];
+    all += part[w];
+  }
+  *total = all;
+  return v + before;
+}
+
+// Pages and starts of a step from have[b] and add[b]: one workgroup.  Pages beyond a sequence's need
+// go back to the stack in the order of the sequences, then they are taken from its top in that order.
+__global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int* __restrict__ have,
+                                                           const int* __restrict__ add, int rows,
+                                                           int* __restrict__ starts_out) {
+  __shared__ int part[kPlanThreads / 64];
+  __shared__ unsigned long long adds, needs;
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) { adds = 0; needs = 0; bad = KV8_OK; }
+  __syncthreads();
+  unsigned long long a_sum = 0, n_sum = 0;
+  int worst = KV8_OK;
+  for (int b = tid; b < v.B; b += kPlanThreads) {
+    const int h = have[b], a = add[b];
+    if (h < 0 || a < 0) worst = max(worst, (int)KV8_BAD_LENGTH);
+    else if ((long long)h + a > v.max_len) worst = max(worst, (int)KV8_TOO_LONG);
+    else { a_sum += a; n_sum += (h + a + kKv8Block - 1) / kKv8Block; }
+  }
+  atomicAdd(&adds, a_sum);
+  atomicAdd(&needs, n_sum);
+  if (worst) atomicMax(&bad, worst);
+  __syncthreads();
+  const int status = bad ? bad : adds > (unsigned long long)rows ? KV8_ROWS
+                     : needs > (unsigned long long)v.pages ? KV8_PAGES : KV8_OK;
+  const int free0 = v.head->free_pages;
+  if (status) {
+    for (int b = tid; b <= v.B; b += kPlanThreads) {
+      v.starts[b] = 0;
+      if (starts_out) starts_out[b] = 0;
+    }
+    if (tid == 0) { v.head->status = status; v.head->rows = 0; }
+    return;
+  }
+  int back = 0, first = 0, total = 0;
+  for (int b0 = 0; b0 < v.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0, a = 0, need = 0;
+    if (b < v.B) {
+      const int h = have[b];
+      a = add[b];
+      need = (h + a + kKv8Block - 1) / kKv8Block;
+      n = max(v.held[b] - need, 0);
+      v.base[b] = h;
+      v.lens[b] = h + a;
+    }
+    int at = wg_scan(n, part, &total) - n + free0 + back;
+    back += total;
+    for (int i = 0; i < n; i++) {
+      int* e = v.table + (size_t)b * v.W + need + i;
+      v.stack[at + i] = *e;
+      *e = -1;
+    }
+    at = wg_scan(a, part, &total) - a + first;
+    first += total;
+    if (b < v.B) {
+      v.starts[b] = at;
+      if (starts_out) starts_out[b] = at;
+    }
+  }
+  __syncthreads();
+  const int top = free0 + back;
+  int taken = 0;
+  for (int b0 = 0; b0 < v.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0, had = 0;
+    if (b < v.B) {
+      const int need = (have[b] + add[b] + kKv8Block - 1) / kKv8Block;
+      had = v.held[b];
+      n = max(need - had, 0);
+      v.held[b] = need;
+    }
+    const int at = top - 1 - (wg_scan(n, part, &total) - n + taken);
+    taken += total;
+    for (int i = 0; i < n; i++) v.table[(size_t)b * v.W + had + i] = v.stack[at - i];
+  }
+  if (tid == 0) {
+    v.starts[v.B] = first;
+    if (starts_out) starts_out[v.B] = first;
+    v.head->status = KV8_OK;
+    v.head->rows = first;
+    v.head->free_pages = top - taken;
+  }
+}
+
+// Sequence, position and slot of every row; a copy of the tables.
+__global__ __launch_bounds__(256) void k_kv8_rows(Kv8View v, int* __restrict__ pos_out, int* __restrict__ slot_out,
+                                                  int* __restrict__ tables_out) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t < v.head->rows) {
+    int lo = 0, hi = v.B;                  // the last sequence that starts at or before t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (v.starts[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int p = v.base[lo] + t - v.starts[lo];
+    const int s = v.table[(size_t)lo * v.W + p / kKv8Block] * kKv8Block + p % kKv8Block;
+    v.seq[t] = lo;
+    v.pos[t] = p;
+    v.slot[t] = s;
+    if (pos_out) pos_out[t] = p;
+    if (slot_out) slot_out[t] = s;
+  }
+  if (tables_out)
+    for (size_t i = t; i < (size_t)v.B * v.W; i += (size_t)gridDim.x * 256) tables_out[i] = v.table[i];
+}
+
+// Nothing but a value's own bits decides: a NaN counts as 0, an infinity as the block's largest value.
+__device__ float magnitude(float x) {
+  const float a = __builtin_fabsf(x);
+  return a < __builtin_inff() ? a : 0.0f;
+}
+
+__device__ int to_code(float x, float s) {
+  if (!(s > 0.0f) || x != x) return 0;
+  return (int)__builtin_fminf(__builtin_fmaxf(__builtin_rintf(x / s), -127.0f), 127.0f);
+}
+
+// The smallest k >= 0 with s * 2^k >= t (s, t > 0).
+__device__ int doublings(float s, float t) {
+  if (!(t > s)) return 0;
+  const float ms = __builtin_amdgcn_frexp_mantf(s), mt = __builtin_amdgcn_frexp_mantf(t);
+  return __builtin_amdgcn_frexp_expf(t) - __builtin_amdgcn_frexp_expf(s) + (mt > ms ? 1 : 0);
+}
+
+// One run of rows in one block (row t and those behind it), one kv head; K for blockIdx.z = 0, else V.
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
+                                                    int64_t k_stride, int64_t v_stride) {
+  __shared__ float tile[kKv8Block][HD + 1];
+  __shared__ float most[4];
+  const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const bool is_v = blockIdx.z != 0;
+  const int rows = v.head->rows;
+  if (t >= rows) return;
+  const int slot = v.slot[t], f = slot % kKv8Block;
+  if (f != 0 && t > 0 && v.slot[t - 1] == slot - 1) return;      // a row behind the first of its run
+  const bool next = lane < kKv8Block - f && t + lane < rows && v.slot[t + lane] == slot + lane;
+  const int m = __builtin_ctzll(~__builtin_amdgcn_ballot_w64(next));
+  const T* x = (is_v ? val : k) + (int64_t)t * (is_v ? v_stride : k_stride) + g * HD;
+  const int64_t ld = is_v ? v_stride : k_stride;
+  float a = 0.0f;
+  for (int i = tid; i < m * HD; i += 256) {
+    const int r = i / HD, c = i % HD;
+    const float y = (float)x[r * ld + c];
+    tile[f + r][c] = y;
+    a = __builtin_fmaxf(a, magnitude(y));
+  }
+  for (int d = 1; d < 64; d <<= 1) a = __builtin_fmaxf(a, __shfl_xor(a, d));
+  if (lane == 0) most[tid >> 6] = a;
+  __syncthreads();
+  a = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
+  const size_t block = ((size_t)layer * v.pages + slot / kKv8Block) * v.KVH + g;
+  float* const scale = (float*)(v.scales + block) + (is_v ? 1 : 0);
+  const float old = f ? *scale : 0.0f, t127 = a / 127.0f, need = t127 < kKv8MinScale ? 0.0f : t127;
+  const int twice = old > 0.0f ? doublings(old, need) : 0;
+  const float s = old > 0.0f ? __builtin_ldexpf(old, twice) : need;
+  uint4* const codes = (uint4*)(v.codes + (block * 2 + (is_v ? 1 : 0)) * (kKv8Block * HD));
+  for (int u = tid; u < 2 * HD; u += 256) {
+    uint4 w = codes[u];
+    uint8_t* const b = (uint8_t*)&w;
+    const int ln = u & 63, q = u >> 6;
+    bool changed = false;
+    for (int j = 0; j < 16; j++) {
+      int tok, col;
+      if (is_v) {
+        tok = ((j >> 2) & 1) * 16 + (ln >> 4) * 4 + (j & 3);
+        col = (2 * q + (j >> 3)) * 16 + (ln & 15);
+      } else {
+        tok = q / (HD / 64) * 16 + (ln & 15);
+        col = (2 * (q % (HD / 64)) + (j >> 3)) * 32 + (ln >> 4) * 8 + (j & 7);
+      }
+      if (tok >= f && tok < f + m) {
+        b[j] = (uint8_t)(to_code(tile[tok][col], s) + 128);
+        changed = true;
+      } else if (tok < f && twice) {
+        b[j] = (uint8_t)((int)__builtin_rintf(__builtin_ldexpf((float)((int)b[j] - 128), -twice)) + 128);
+        changed = true;
+      }
+    }
+    if (changed) codes[u] = w;
+  }
+  __syncthreads();                        // every thread has read the old scale
+  if (tid == 0) *scale = s;
+}
+
+// The values that the cache stands for at n pairs of a sequence and a position; 0 where it holds none.
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv8_read(Kv8View v, int layer, const int* __restrict__ seq, const int* __restrict__ pos,
+                                                  int n, float* __restrict__ k, float* __restrict__ val) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = (int64_t)v.KVH * HD;
+  if (i >= n * row) return;
+  const int r = (int)(i / row), g = (int)(i % row) / HD, d = (int)(i % HD);
+  const int b = seq[r], p = pos[r];
+  float a = 0.0f, c = 0.0f;
+  if (b >= 0 && b < v.B && p >= 0 && p < v.lens[b]) {
+    const int t = p % kKv8Block;
+    const size_t block = ((size_t)layer * v.pages + v.table[(size_t)b * v.W + p / kKv8Block]) * v.KVH + g;
+    const uint8_t* codes = v.codes + block * 2 * (kKv8Block * HD);
+    const float2 s = v.scales[block];
+    a = s.x * (float)((int)codes[kv8_k_byte(HD, t, d)] - 128);
+    c = s.y * (float)((int)codes[kKv8Block * HD + kv8_v_byte(t, d)] - 128);
+  }
+  k[i] = a;
+  val[i] = c;
+}
+
+// Attention of one row and head by one wave: a page at a time, with the running maximum and sum of the softmax.
+template <int HD, class T>
+__global__ __launch_bounds__(64) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
+                                                   int64_t q_stride, int64_t out_stride, float scale) {
+  __shared__ float qs[HD];
+  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, g = h / (v.H / v.KVH);
+  if (t >= v.head->rows) return;
+  for (int d = lane; d < HD; d += 64) qs[d] = (float)q[t * q_stride + h * HD + d];
+  __syncthreads();
+  const int last = v.pos[t];
+  const int* const table = v.table + (size_t)v.seq[t] * v.W;
+  float m = -__builtin_inff(), l = 0.0f, o[HD / 64] = {};
+  for (int p0 = 0; p0 <= last; p0 += kKv8Block) {
+    const size_t block = ((size_t)layer * v.pages + table[p0 / kKv8Block]) * v.KVH + g;
+    const uint8_t* const kc = v.codes + block * 2 * (kKv8Block * HD);
+    const uint8_t* const vc = kc + kKv8Block * HD;
+    const float2 s = v.scales[block];
+    const int tok = lane & 31;
+    float x = 0.0f;
+    for (int d = (lane >> 5) * (HD / 2), i = 0; i < HD / 2; i++, d++)
+      x = __builtin_fmaf(qs[d], (float)((int)kc[kv8_k_byte(HD, tok, d)] - 128), x);
+    x += __shfl_xor(x, 32);
+    x = p0 + tok <= last ? x * (s.x * scale) : -__builtin_inff();
+    float most = x;
+    for (int d = 1; d < 32; d <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    const float m2 = __builtin_fmaxf(m, most);
+    const float w = expf(x - m2), old = expf(m - m2);
+    float sum = w;
+    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
+    l = l * old + sum;
+    for (int c = 0; c < HD / 64; c++) o[c] *= old;
+    for (int j = 0; j < kKv8Block; j++) {
+      const float wj = __shfl(w, j) * s.y;
+      for (int c = 0; c < HD / 64; c++)
+        o[c] = __builtin_fmaf(wj, (float)((int)vc[kv8_v_byte(j, c * 64 + lane)] - 128), o[c]);
+    }
+    m = m2;
+  }
+  for (int c = 0; c < HD / 64; c++) out[t * out_stride + h * HD + c * 64 + lane] = (T)(o[c] / l);
+}
+
+// The free pages in the order in which they are taken, and a table without pages.
+__global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < (size_t)v.B * v.W) v.table[i] = -1;
+  if (i < (size_t)v.pages) v.stack[i] = v.pages - 1 - (int)i;
+  if (i <= (size_t)v.B) {
+    v.starts[i] = 0;
+    if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
+  }
+  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages};
+}
+
+int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
+
+int check_layer(const q4hip_kv8* kv, int layer, int type) {
+  if (layer < 0 || layer >= kv->v.layers) return fail(Q4HIP_EINVAL, "layer %d of %d", layer, kv->v.layers);
+  if (type != Q4HIP_TYPE_F32 && type != Q4HIP_TYPE_F16 && type != Q4HIP_TYPE_BF16)
+    return fail(Q4HIP_ETYPE, "type %d: expected F32, F16 or BF16", type);
+  return Q4HIP_OK;
+}
+
+// `rows` rows of `width` elements, `stride` elements apart.
+int check_rows(const q4hip_kv8* kv, const void* p, int rows, int width, int64_t stride, int type, const char* what) {
+  const int es = elem_size(type);
+  if ((uintptr_t)p % es) return fail(Q4HIP_EINVAL, "%s: not aligned to its type", what);
+  if (stride < width) return fail(Q4HIP_EINVAL, "%s: rows of %d values, %lld apart", what, width, (long long)stride);
+  if (stride > ((int64_t)1 << 31)) return fail(Q4HIP_EINVAL, "%s: rows %lld values apart", what, (long long)stride);
+  return check_device_span(p, ((size_t)(rows - 1) * stride + width) * es, kv->device, what);
+}
+
+int plan_error(const q4hip_kv8* kv, int status) {
+  switch (status) {
+    case KV8_OK: return Q4HIP_OK;
+    case KV8_BAD_LENGTH: return fail(Q4HIP_EINVAL, "plan: a negative length");
+    case KV8_TOO_LONG: return fail(Q4HIP_ECONTEXT, "plan: a sequence longer than %d positions", kv->v.max_len);
+    case KV8_ROWS: return fail(Q4HIP_EINVAL, "plan: more rows than the %d it was called for", kv->rows);
+    default: return fail(Q4HIP_ECONTEXT, "plan: more than the pool's %d pages", kv->v.pages);
+  }
+}
+
+int read_head(q4hip_kv8* kv, hipStream_t s) {
+  HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
+  HIPCHK(hipStreamSynchronize(s));
+  return Q4HIP_OK;
+}
+
+template <class F>
+void by_type(int type, F f) {
+  if (type == Q4HIP_TYPE_F32) f(float());
+  else if (type == Q4HIP_TYPE_F16) f(_Float16());
+  else f(__bf16());
+}
+
+}  // namespace
+}  // namespace q4
+
+using namespace q4;
+
+extern "C" {
+
+void q4hip_kv8_destroy(q4hip_kv8* kv) {
+  if (!kv) return;
+  (void)hipSetDevice(kv->device);
+  if (kv->stream) (void)hipStreamSynchronize(kv->stream);
+  Kv8View& v = kv->v;
+  void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.seq, v.pos, v.slot};
+  for (void* p : bufs) if (p) (void)hipFree(p);
+  if (kv->pin) (void)hipHostFree(kv->pin);
+  if (kv->stream) (void)hipStreamDestroy(kv->stream);
+  delete kv;
+}
+
+int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages,
+                     int max_rows, int device) {
+  if (!out) return fail(Q4HIP_EINVAL, "null argument");
+  *out = nullptr;
+  if (layers <= 0 || heads <= 0 || kv_heads <= 0 || seqs <= 0 || max_len <= 0 || pages <= 0 || max_rows <= 0)
+    return fail(Q4HIP_EINVAL, "bad configuration");
+  if (heads % kv_heads) return fail(Q4HIP_EINVAL, "heads must be a multiple of kv_heads");
+  if (head_dim != 64 && head_dim != 128) return fail(Q4HIP_EINVAL, "head_dim %d unsupported (64 or 128)", head_dim);
+  if (heads > 65535 || layers > 65535) return fail(Q4HIP_EINVAL, "bad configuration");
+  if (pages > INT32_MAX / kKv8Block) return fail(Q4HIP_EINVAL, "%d pages: at most %d", pages, INT32_MAX / kKv8Block);
+  if (max_len > INT32_MAX - kKv8Block) return fail(Q4HIP_EINVAL, "sequences of %d positions", max_len);
+  int ndev = 0;
+  HIPCHK(hipGetDeviceCount(&ndev));
+  if (device < 0 || device >= ndev) return fail(Q4HIP_EINVAL, "device %d of %d", device, ndev);
+  HIPCHK(hipSetDevice(device));
+  q4hip_kv8* kv = new (std::nothrow) q4hip_kv8();
+  if (!kv) return fail(Q4HIP_EHIP, "out of host memory");
+  kv->device = device;
+  kv->max_rows = max_rows;
+  Kv8View& v = kv->v;
+  v.layers = layers; v.H = heads; v.KVH = kv_heads; v.HD = head_dim;
+  v.B = seqs; v.W = (max_len + kKv8Block - 1) / kKv8Block; v.pages = pages; v.max_len = max_len;
+  const size_t blocks = (size_t)layers * pages * kv_heads, bytes = blocks * 2 * kKv8Block * head_dim;
+  hipError_t e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
+  auto al = [&](auto** p, size_t n) { if (e == hipSuccess) e = hipMalloc((void**)p, n * sizeof(**p)); };
+  al(&v.codes, bytes);
+  al(&v.scales, blocks);
+  al(&v.table, (size_t)seqs * v.W);
+  al(&v.held, seqs);
+  al(&v.stack, pages);
+  al(&v.head, 1);
+  al(&v.base, seqs);
+  al(&v.lens, seqs);
+  al(&v.starts, (size_t)seqs + 1);
+  al(&v.seq, max_rows);
+  al(&v.pos, max_rows);
+  al(&v.slot, max_rows);
+  if (e == hipSuccess) e = hipHostMalloc((void**)&kv->pin, sizeof(Kv8Head), hipHostMallocDefault);
+  if (e == hipSuccess) e = hipMemsetAsync(v.codes, 128, bytes, kv->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(v.scales, 0, blocks * sizeof(float2), kv->stream);
+  if (e == hipSuccess) {
+    const size_t n = std::max({(size_t)seqs * v.W, (size_t)pages, (size_t)seqs + 1});
+    k_kv8_reset<<<(unsigned)((n + 255) / 256), 256, 0, kv->stream>>>(v);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
+  if (e != hipSuccess) {
+    const int rc = fail(Q4HIP_EHIP, "8-bit cache of %d pages: %s", pages, hipGetErrorString(e));
+    q4hip_kv8_destroy(kv);
+    return rc;
+  }
+  *out = kv;
+  return Q4HIP_OK;
+}
+
+int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
+                   int* tables, void* stream) {
+  if (!kv || !have || !add) return fail(Q4HIP_EINVAL, "null argument");
+  if (rows < 0 || rows > kv->max_rows) return fail(Q4HIP_EINVAL, "%d rows: a plan holds up to %d", rows, kv->max_rows);
+  const Kv8View& v = kv->v;
+  HIPCHK(hipSetDevice(kv->device));
+  const struct { const void* p; size_t n; const char* what; } spans[] = {
+      {have, (size_t)v.B, "have"}, {add, (size_t)v.B, "add"}, {starts, (size_t)v.B + 1, "starts"},
+      {positions, (size_t)rows, "positions"}, {slots, (size_t)rows, "slots"}, {tables, (size_t)v.B * v.W, "tables"}};
+  for (const auto& a : spans)
+    if (a.p && a.n) {
+      const int rc = check_device_span(a.p, a.n * 4, kv->device, a.what);
+      if (rc) return rc;
+    }
+  hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  kv->rows = rows;
+  k_kv8_plan<<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts);
+  const int wgs = std::max((rows + 255) / 256, tables ? (int)std::min<size_t>(((size_t)v.B * v.W + 255) / 256, 512) : 0);
+  if (wgs) k_kv8_rows<<<wgs, 256, 0, s>>>(v, positions, slots, tables);
+  HIPCHK(hipGetLastError());
+  if (stream) return Q4HIP_OK;
+  const int rc = read_head(kv, s);
+  return rc ? rc : plan_error(kv, kv->pin->status);
+}
+
+int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages) {
+  if (!kv) return fail(Q4HIP_EINVAL, "null argument");
+  HIPCHK(hipSetDevice(kv->device));
+  const int rc = read_head(kv, stream ? (hipStream_t)stream : kv->stream);
+  if (rc) return rc;
+  if (rows) *rows = kv->pin->rows;
+  if (free_pages) *free_pages = kv->pin->free_pages;
+  return plan_error(kv, kv->pin->status);
+}
+
+int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int type, int64_t k_stride, int64_t v_stride,
+                     void* stream) {
+  if (!kv || !k || !v) return fail(Q4HIP_EINVAL, "null argument");
+  int rc = check_layer(kv, layer, type);
+  if (rc) return rc;
+  if (!kv->rows) return Q4HIP_OK;
+  HIPCHK(hipSetDevice(kv->device));
+  const Kv8View& w = kv->v;
+  rc = check_rows(kv, k, kv->rows, w.KVH * w.HD, k_stride, type, "k");
+  if (!rc) rc = check_rows(kv, v, kv->rows, w.KVH * w.HD, v_stride, type, "v");
+  if (rc) return rc;
+  hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  const dim3 grid((unsigned)kv->rows, (unsigned)w.KVH, 2);
+  by_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    if (w.HD == 64) k_kv8_append<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride);
+    else k_kv8_append<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride);
+  });
+  HIPCHK(hipGetLastError());
+  if (!stream) HIPCHK(hipStreamSynchronize(s));
+  return Q4HIP_OK;
+}
+
+int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int n, float* k, float* v, void* stream) {
+  if (!kv || !seq || !pos || !k || !v) return fail(Q4HIP_EINVAL, "null argument");
+  int rc = check_layer(kv, layer, Q4HIP_TYPE_F32);
+  if (rc) return rc;
+  if (n < 0) return fail(Q4HIP_EINVAL, "%d positions", n);
+  if (!n) return Q4HIP_OK;
+  HIPCHK(hipSetDevice(kv->device));
+  const Kv8View& w = kv->v;
+  const size_t row = (size_t)w.KVH * w.HD;
+  rc = check_device_span(seq, (size_t)n * 4, kv->device, "seq");
+  if (!rc) rc = check_device_span(pos, (size_t)n * 4, kv->device, "pos");
+  if (!rc) rc = check_rows(kv, k, n, (int)row, row, Q4HIP_TYPE_F32, "k");
+  if (!rc) rc = check_rows(kv, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
+  if (rc) return rc;
+  const size_t wgs = (n * row + 255) / 256;
+  if (wgs > INT32_MAX) return fail(Q4HIP_EINVAL, "%d positions at once", n);
+  hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  if (w.HD == 64) k_kv8_read<64><<<(unsigned)wgs, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  else k_kv8_read<128><<<(unsigned)wgs, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  HIPCHK(hipGetLastError());
+  if (!stream) HIPCHK(hipStreamSynchronize(s));
+  return Q4HIP_OK;
+}
+
+int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
+                     float scale, void* stream) {
+  if (!kv || !q || !out) return fail(Q4HIP_EINVAL, "null argument");
+  int rc = check_layer(kv, layer, type);
+  if (rc) return rc;
+  if (!std::isfinite(scale) || scale < 0.0f) return fail(Q4HIP_EINVAL, "scale %g", (double)scale);
+  if (!kv->rows) return Q4HIP_OK;
+  HIPCHK(hipSetDevice(kv->device));
+  const Kv8View& w = kv->v;
+  rc = check_rows(kv, q, kv->rows, w.H * w.HD, q_stride, type, "q");
+  if (!rc) rc = check_rows(kv, out, kv->rows, w.H * w.HD, out_stride, type, "out");
+  if (rc) return rc;
+  if (scale == 0.0f) scale = 1.0f / std::sqrt((float)w.HD);
+  hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  const dim3 grid((unsigned)kv->rows, (unsigned)w.H);
+  by_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    if (w.HD == 64) k_kv8_attend<64, T><<<grid, 64, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, scale);
+    else k_kv8_attend<128, T><<<grid, 64, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, scale);
+  });
+  HIPCHK(hipGetLastError());
+  if (!stream) HIPCHK(hipStreamSynchronize(s));
+  return Q4HIP_OK;
+}
+
+}  // extern "C"

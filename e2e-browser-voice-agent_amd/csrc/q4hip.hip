@@ -21,6 +21,7 @@
 #include "attn_head.h"
 #include "gemm_sk.h"
 #include "gemm_tile.h"
+#include "host.h"
 #include "kernels.h"
 #include "persistent.h"
 #include "q4hip.h"
@@ -1604,11 +1605,9 @@ __global__ __launch_bounds__(256) void k_argmax_rows2(const float* __restrict__ 
 
 // ================================================================ host side
 
-namespace {
+static thread_local std::string g_err;
 
-thread_local std::string g_err;
-
-int fail(int code, const char* fmt, ...) {
+int q4::fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -1618,11 +1617,10 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define HIPCHK(call)                                                                   \
-  do {                                                                                 \
-    hipError_t e_ = (call);                                                            \
-    if (e_ != hipSuccess) return fail(Q4HIP_EHIP, "%s: %s", #call, hipGetErrorString(e_)); \
-  } while (0)
+namespace {
+
+using q4::check_device_span;
+using q4::fail;
 
 constexpr size_t kWeightPadQ = 32768, kWeightPadD = 8192;
 
@@ -3773,9 +3771,9 @@ int scratch_on(int device, uint4** out) {
   return Q4HIP_OK;
 }
 
-// `bytes` of device memory of `device` start at p (checked before any launch, so a host pointer or
-// a short buffer is an error, not a memory fault).
-int check_device_span(const void* p, size_t bytes, int device, const char* what) {
+}  // namespace
+
+int q4::check_device_span(const void* p, size_t bytes, int device, const char* what) {
   hipPointerAttribute_t a;
   if (hipPointerGetAttributes(&a, p) != hipSuccess) {
     (void)hipGetLastError();
@@ -3794,8 +3792,6 @@ int check_device_span(const void* p, size_t bytes, int device, const char* what)
                 (size_t)((const char*)base + size - (const char*)p));
   return Q4HIP_OK;
 }
-
-}  // namespace
 
 extern "C" {
 

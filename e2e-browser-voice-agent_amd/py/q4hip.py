@@ -20,6 +20,8 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libq4hip.so")
 OK, EINVAL, ECONTEXT, ETYPE, EHIP, ESTATE = 0, 1, 2, 3, 4, 5
 DECODE_AUTO, DECODE_GRAPH, DECODE_PERSISTENT = 0, 1, 2
 KV_F32, KV_F16 = 0, 1
+F32, F16, BF16 = 0, 1, 30      # element types of an 8-bit cache's rows (GGML numbers)
+KV8_BLOCK = 32                 # positions of its pages
 NOALLOC_MAX_K = 65536          # include/q4hip.h Q4HIP_NOALLOC_MAX_K
 PROF_NAMES = ["embed", "norm+quantize", "matvec qkv", "rope+kv", "attention", "quantize", "matvec o",
               "matvec gate+up", "swiglu+quantize", "matvec down", "matvec output", "sample"]
@@ -32,7 +34,8 @@ EXPORTS = [
     "q4hip_set_kv", "q4hip_profile_pass", "q4hip_batch_create", "q4hip_batch_destroy",
     "q4hip_batch_prefill", "q4hip_batch_set_kv", "q4hip_batch_generate", "q4hip_batch_time_generate",
     "q4hip_batch_read_logits", "q4hip_mv_time_cold", "q4hip_check_division", "q4hip_mv_run_noalloc",
-    "q4hip_attn_ring_rows", "q4hip_check_ordered_sum",
+    "q4hip_attn_ring_rows", "q4hip_check_ordered_sum", "q4hip_kv8_create", "q4hip_kv8_destroy", "q4hip_kv8_plan",
+    "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend",
 ]
 
 _lib = None
@@ -85,6 +88,13 @@ def lib() -> ctypes.CDLL:
         "q4hip_batch_read_logits": (I, [P, P, I64]),
         "q4hip_mv_time_cold": (I, [P, I64, I, ctypes.POINTER(F), ctypes.POINTER(I)]),
         "q4hip_mv_run_noalloc": (I, [P, P, P, P]),
+        "q4hip_kv8_create": (I, [ctypes.POINTER(P), I, I, I, I, I, I, I, I, I]),
+        "q4hip_kv8_destroy": (None, [P]),
+        "q4hip_kv8_plan": (I, [P, P, P, I, P, P, P, P, P]),
+        "q4hip_kv8_status": (I, [P, P, ctypes.POINTER(I), ctypes.POINTER(I)]),
+        "q4hip_kv8_append": (I, [P, I, P, P, I, I64, I64, P]),
+        "q4hip_kv8_read": (I, [P, I, P, P, I, P, P, P]),
+        "q4hip_kv8_attend": (I, [P, I, P, P, I, I64, I64, F, P]),
         "q4hip_attn_ring_rows": (I, [I, I, I, I, I, I, ctypes.POINTER(I), ctypes.POINTER(I), ctypes.POINTER(I)]),
     }
     for name, (res, args) in sig.items():
@@ -375,6 +385,55 @@ class Matvec:
     def close(self) -> None:
         if self.h:
             lib().q4hip_mv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Kv8:
+    """A paged K/V cache in 8 bits, on device buffers given by address: plan, append and attend of a step
+    (include/q4hip.h, q4hip_kv8_*).  A call waits for its end unless a stream is given."""
+
+    def __init__(self, layers: int, heads: int, kv_heads: int, head_dim: int, seqs: int, max_len: int, pages: int,
+                 max_rows: int, device: int = 0):
+        self.seqs, self.blocks = seqs, -(-max_len // KV8_BLOCK)
+        h = ctypes.c_void_p()
+        _check(lib().q4hip_kv8_create(ctypes.byref(h), layers, heads, kv_heads, head_dim, seqs, max_len, pages, max_rows,
+                                      device))
+        self.h = h
+
+    def plan(self, have: int, add: int, rows: int, starts: int = 0, positions: int = 0, slots: int = 0, tables: int = 0,
+             stream: int = 0) -> None:
+        """Pages and rows of the step that adds add[b] rows to the have[b] of sequence b."""
+        _check(lib().q4hip_kv8_plan(self.h, have or None, add or None, rows, starts or None, positions or None, slots or None,
+                                    tables or None, stream or None))
+
+    def status(self, stream: int = 0) -> tuple:
+        """(rows of the last plan, free pages); raises the plan's error."""
+        rows, free = ctypes.c_int(0), ctypes.c_int(0)
+        _check(lib().q4hip_kv8_status(self.h, stream or None, ctypes.byref(rows), ctypes.byref(free)))
+        return rows.value, free.value
+
+    def append(self, layer: int, k: int, v: int, dtype: int, k_stride: int, v_stride: int, stream: int = 0) -> None:
+        """K and V of the step's rows into the cache."""
+        _check(lib().q4hip_kv8_append(self.h, layer, k or None, v or None, dtype, k_stride, v_stride, stream or None))
+
+    def read(self, layer: int, seq: int, pos: int, n: int, k: int, v: int, stream: int = 0) -> None:
+        """The fp32 K and V that the cache stands for at n (sequence, position) pairs."""
+        _check(lib().q4hip_kv8_read(self.h, layer, seq or None, pos or None, n, k or None, v or None, stream or None))
+
+    def attend(self, layer: int, q: int, out: int, dtype: int, q_stride: int, out_stride: int, stream: int = 0,
+               scale: float = 0.0) -> None:
+        """Attention of the step's rows; scale 0 is head_dim ** -0.5."""
+        _check(lib().q4hip_kv8_attend(self.h, layer, q or None, out or None, dtype, q_stride, out_stride, scale, stream or None))
+
+    def close(self) -> None:
+        if self.h:
+            lib().q4hip_kv8_destroy(self.h)
             self.h = None
 
     def __del__(self):

@@ -30,6 +30,9 @@ extern "C" {
 #define Q4HIP_TYPE_F32 0
 #define Q4HIP_TYPE_Q4_0 2
 #define Q4HIP_TYPE_Q8_0 8
+/* and, with F32, the element types of the 8-bit cache's rows (q4hip_kv8_append, q4hip_kv8_attend) */
+#define Q4HIP_TYPE_F16 1
+#define Q4HIP_TYPE_BF16 30
 
 /* Tensor kinds, numbered as the reference's set_tensor (engine/kernels.c:422):
  * 0 qkv, 1 o, 2 gate+up, 3 down (Q4_0); 4 attn_norm, 5 ffn_norm, 6 qkv bias (F32);
@@ -227,6 +230,65 @@ void q4hip_mv_destroy(q4hip_mv* m);
  * that overlap on one GPU (other streams, other threads, other handles) race. */
 #define Q4HIP_NOALLOC_MAX_K 65536
 int q4hip_mv_run_noalloc(q4hip_mv* m, const float* x, float* y, void* stream);
+
+/* ---- paged K/V cache in 8 bits -----------------------------------------------------------------
+ * A pool of pages shared by up to `seqs` sequences, for callers that bring their own device buffers and
+ * streams (no counterpart in the reference, whose cache is fp32 and of fixed size).  A page holds
+ * Q4HIP_KV8_BLOCK positions of one sequence in every layer; K and V are int8 codes with one fp32 scale for
+ * each (page, layer, kv head).  A step is
+ *
+ *   q4hip_kv8_plan    once: which pages the sequences hold, where the step's rows lie
+ *   q4hip_kv8_append  per layer: the rows' K and V into the cache
+ *   q4hip_kv8_attend  per layer: attention of the rows over it
+ *
+ * Nothing is allocated after q4hip_kv8_create, and all of a step's work is enqueued on the caller's
+ * stream, so that it can be captured into a HIP graph.  `stream` (a hipStream_t) NULL: the handle's own
+ * stream, and the call waits for its end.  Pointers are device memory of the handle's device and are
+ * checked, with the bytes behind them, before anything is launched.  Calls on one handle are serialized by the caller, also on the GPU: calls on
+ * several streams, or graphs that hold them, are ordered by events or waits.  Handles are independent. */
+typedef struct q4hip_kv8 q4hip_kv8;
+#define Q4HIP_KV8_BLOCK 32
+/* A cache of `pages` pages for `seqs` sequences of up to max_len positions; plans hold up to max_rows
+ * rows.  head_dim is 64 or 128, heads a multiple of kv_heads. */
+int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages,
+                     int max_rows, int device);
+void q4hip_kv8_destroy(q4hip_kv8* kv);
+/* The step in which sequence b holds have[b] positions and adds add[b] (int32 device arrays of `seqs`).
+ * Afterwards every sequence has exactly the ceil((have + add) / 32) pages that it needs: one that needs
+ * fewer than it had gives the rest back (0 and 0: all of them), then those that lack some take them from
+ * the pool.  Positions from have[b] on are written by the step; have[b] may be less than the sequence held
+ * (a chat cut back).  The same plan again changes nothing.  `rows` is at least the sum of add; the
+ * rows of the step lie one sequence after the other.  Device arrays that are not NULL receive
+ *   starts[seqs + 1]   the first row of each sequence, and the number of rows
+ *   positions[rows]    a row's position in its sequence
+ *   slots[rows]        32 * page + position % 32
+ *   tables[seqs][ceil(max_len / 32)]   the pages of each sequence, -1 behind them
+ * (of positions and slots, entries behind the step's rows are left as they were).  Lengths that do not
+ * fit (negative, beyond max_len, more rows than `rows`, more pages than the pool has) make the plan fail as a whole:
+ * no page changes hands, the step has no rows, and append and attend do nothing.  With `stream` NULL the call
+ * returns that error; otherwise q4hip_kv8_status does. */
+int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
+                   int* tables, void* stream);
+/* Waits for `stream` (NULL: the handle's) and returns the last plan's error, its rows and the pages left. */
+int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages);
+/* K and V of the step's rows, `type` F32, F16 or BF16: row t, kv head g, column d at
+ * k[t * k_stride + g * head_dim + d] (strides in elements; the buffers hold the `rows` of the plan).  Of the rows that fall
+ * into one page, with the first at offset f of it, and one head: t = max|x| / 127 in fp32, or 0 where that is below 2^-100; f = 0 sets the scale to t; f > 0
+ * doubles it until it reaches t, and halves the codes of the f positions before as often, to the nearest even
+ * integer.  A code is x / scale in fp32 rounded to the nearest even integer.  A value read back is off by at most
+ * half of its page's scale, or by less than the whole of it if the scale has grown since.  NaN counts as 0, an infinity
+ * as the largest code of its sign; neither counts for the maximum. */
+int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int type, int64_t k_stride, int64_t v_stride,
+                     void* stream);
+/* What the cache stands for: K and V [n][kv_heads][head_dim] in fp32 of n pairs (seq[i], pos[i]) (int32 device
+ * arrays); 0 for a sequence or position that the last plan does not have. */
+int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int n, float* k, float* v, void* stream);
+/* out = softmax(scale * q . K) V of the step's rows, each over the positions of its sequence up to its own: row t, head h,
+ * column d at q[t * q_stride + h * head_dim + d], `out` alike; head h reads kv head h / (heads / kv_heads).
+ * Scores, the softmax and the sums are fp32; `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
+ * the step's are left as they were. */
+int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
+                     float scale, void* stream);
 
 /* ---- self-check of the quotient forms ------------------------------------------------------
  * The kernels compute the reference's IEEE binary32 divisions (engine/kernels.c:84, 98-99, 395)
