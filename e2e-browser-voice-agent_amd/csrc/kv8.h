@@ -17,6 +17,7 @@
 namespace q4 {
 
 constexpr int kKv8Block = 32;
+constexpr int kKv8MinPart = 16;               // pages of the smallest part of a unit
 constexpr float kKv8MinScale = 0x1p-100f;     // a smaller scale is 0, and so are the values
 
 __host__ __device__ constexpr int kv8_k_byte(int HD, int t, int d) {
@@ -33,8 +34,25 @@ struct Kv8Head {
   int status;      // KV8_*
   int rows;        // rows of the plan, 0 when it failed
   int free_pages;
+  int runs, items;
+  int parts_of;    // pages from which on a unit's pages are shared among several items, and in parts of how many
 };
-enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES };
+enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE };
+
+// A run: rows t.. that lie in one page from `slot` on, m of them.
+struct Kv8Run {
+  int t, slot, m, unused;
+};
+
+// Attention's work.  A unit is up to 16 / G neighbouring rows of a sequence (G query heads to a kv head; one row
+// where G > 16), so that they fill 16 rows of a matrix core; an item is one of the `parts` that share a unit's pages.
+struct Kv8Item {
+  int seq, t, n;         // sequence, first row, rows
+  int pos;               // position of the first row
+  int page0, pages;      // of the sequence's table
+  int part, slot;        // slot: of the unit's first part in the workspace, -1 for a unit in one part
+  int parts, unused[3];
+};
 
 // The device side of a cache.
 struct Kv8View {
@@ -46,8 +64,17 @@ struct Kv8View {
   Kv8Head* head;
   int *base, *lens;    // [seqs] positions before and after the step
   int* starts;         // [seqs + 1] first row of a sequence in the step
-  int *seq, *pos, *slot;   // [max_rows] of a row: sequence, position, 32 * page + position % 32
+  int *free_at, *take_at, *run_at, *item_at, *part_at;   // [seqs + 1] sums over the sequences before: pages given back
+                       // and taken, runs, items, slots in the workspace
+  Kv8Run* runs;
+  Kv8Item* items;
+  float* part_o;       // [slots][kv_heads * row tiles][16][HD] sums of a part, relative to 2^part_ml.x
+  float2* part_ml;     // [slots][kv_heads * row tiles][16] reference exponent, sum of the probabilities
+  int* arrived;        // [slots][kv_heads * row tiles] parts of a unit that are done (at its first slot)
   int layers, H, KVH, HD, B, W, pages, max_len;
+  int unit_rows;       // rows of a unit
+  int row_tiles;       // 16-row tiles of a unit
+  int items_aim;       // items that fill the GPU
 };
 
 }  // namespace q4

@@ -6,137 +6,14 @@
 #include <new>
 
 #include "host.h"
+#include "kv8_attend.h"
+#include "kv8_plan.h"
 
 namespace q4 {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-
-// Inclusive sum over the workgroup's threads; *total receives the sum of all.  `part`: one int per wave.
-__device__ int wg_scan(int v, int* part, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  __syncthreads();                       // `part` of the scan before has been read
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < waves; w++) {
-    if (w < wave) before += part[w];
-    all += part[w];
-  }
-  *total = all;
-  return v + before;
-}
-
-// Pages and starts of a step from have[b] and add[b]: one workgroup.  Pages beyond a sequence's need
-// go back to the stack in the order of the sequences, then they are taken from its top in that order.
-__global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int* __restrict__ have,
-                                                           const int* __restrict__ add, int rows,
-                                                           int* __restrict__ starts_out) {
-  __shared__ int part[kPlanThreads / 64];
-  __shared__ unsigned long long adds, needs;
-  __shared__ int bad;
-  const int tid = threadIdx.x;
-  if (tid == 0) { adds = 0; needs = 0; bad = KV8_OK; }
-  __syncthreads();
-  unsigned long long a_sum = 0, n_sum = 0;
-  int worst = KV8_OK;
-  for (int b = tid; b < v.B; b += kPlanThreads) {
-    const int h = have[b], a = add[b];
-    if (h < 0 || a < 0) worst = max(worst, (int)KV8_BAD_LENGTH);
-    else if ((long long)h + a > v.max_len) worst = max(worst, (int)KV8_TOO_LONG);
-    else { a_sum += a; n_sum += (h + a + kKv8Block - 1) / kKv8Block; }
-  }
-  atomicAdd(&adds, a_sum);
-  atomicAdd(&needs, n_sum);
-  if (worst) atomicMax(&bad, worst);
-  __syncthreads();
-  const int status = bad ? bad : adds > (unsigned long long)rows ? KV8_ROWS
-                     : needs > (unsigned long long)v.pages ? KV8_PAGES : KV8_OK;
-  const int free0 = v.head->free_pages;
-  if (status) {
-    for (int b = tid; b <= v.B; b += kPlanThreads) {
-      v.starts[b] = 0;
-      if (starts_out) starts_out[b] = 0;
-    }
-    if (tid == 0) { v.head->status = status; v.head->rows = 0; }
-    return;
-  }
-  int back = 0, first = 0, total = 0;
-  for (int b0 = 0; b0 < v.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    int n = 0, a = 0, need = 0;
-    if (b < v.B) {
-      const int h = have[b];
-      a = add[b];
-      need = (h + a + kKv8Block - 1) / kKv8Block;
-      n = max(v.held[b] - need, 0);
-      v.base[b] = h;
-      v.lens[b] = h + a;
-    }
-    int at = wg_scan(n, part, &total) - n + free0 + back;
-    back += total;
-    for (int i = 0; i < n; i++) {
-      int* e = v.table + (size_t)b * v.W + need + i;
-      v.stack[at + i] = *e;
-      *e = -1;
-    }
-    at = wg_scan(a, part, &total) - a + first;
-    first += total;
-    if (b < v.B) {
-      v.starts[b] = at;
-      if (starts_out) starts_out[b] = at;
-    }
-  }
-  __syncthreads();
-  const int top = free0 + back;
-  int taken = 0;
-  for (int b0 = 0; b0 < v.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    int n = 0, had = 0;
-    if (b < v.B) {
-      const int need = (have[b] + add[b] + kKv8Block - 1) / kKv8Block;
-      had = v.held[b];
-      n = max(need - had, 0);
-      v.held[b] = need;
-    }
-    const int at = top - 1 - (wg_scan(n, part, &total) - n + taken);
-    taken += total;
-    for (int i = 0; i < n; i++) v.table[(size_t)b * v.W + had + i] = v.stack[at - i];
-  }
-  if (tid == 0) {
-    v.starts[v.B] = first;
-    if (starts_out) starts_out[v.B] = first;
-    v.head->status = KV8_OK;
-    v.head->rows = first;
-    v.head->free_pages = top - taken;
-  }
-}
-
-// Sequence, position and slot of every row; a copy of the tables.
-__global__ __launch_bounds__(256) void k_kv8_rows(Kv8View v, int* __restrict__ pos_out, int* __restrict__ slot_out,
-                                                  int* __restrict__ tables_out) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t < v.head->rows) {
-    int lo = 0, hi = v.B;                  // the last sequence that starts at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (v.starts[mid] <= t) lo = mid; else hi = mid;
-    }
-    const int p = v.base[lo] + t - v.starts[lo];
-    const int s = v.table[(size_t)lo * v.W + p / kKv8Block] * kKv8Block + p % kKv8Block;
-    v.seq[t] = lo;
-    v.pos[t] = p;
-    v.slot[t] = s;
-    if (pos_out) pos_out[t] = p;
-    if (slot_out) slot_out[t] = s;
-  }
-  if (tables_out)
-    for (size_t i = t; i < (size_t)v.B * v.W; i += (size_t)gridDim.x * 256) tables_out[i] = v.table[i];
-}
+constexpr int kItemsAim = 512;          // workgroups of attention that fill the GPU
+constexpr size_t kFillInPlan = 8192;
 
 // Nothing but a value's own bits decides: a NaN counts as 0, an infinity as the block's largest value.
 __device__ float magnitude(float x) {
@@ -156,20 +33,21 @@ __device__ int doublings(float s, float t) {
   return __builtin_amdgcn_frexp_expf(t) - __builtin_amdgcn_frexp_expf(s) + (mt > ms ? 1 : 0);
 }
 
-// One run of rows in one block (row t and those behind it), one kv head; K for blockIdx.z = 0, else V.
+// A run of rows (blockIdx.x) of one kv head; K for blockIdx.z = 0, else V.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
-                                                    int64_t k_stride, int64_t v_stride) {
+                                                    int64_t k_stride, int64_t v_stride, int rows) {
   __shared__ float tile[kKv8Block][HD + 1];
   __shared__ float most[4];
-  const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const bool is_v = blockIdx.z != 0;
-  const int rows = v.head->rows;
-  if (t >= rows) return;
-  const int slot = v.slot[t], f = slot % kKv8Block;
-  if (f != 0 && t > 0 && v.slot[t - 1] == slot - 1) return;      // a row behind the first of its run
-  const bool next = lane < kKv8Block - f && t + lane < rows && v.slot[t + lane] == slot + lane;
-  const int m = __builtin_ctzll(~__builtin_amdgcn_ballot_w64(next));
+  if (v.head->rows > rows) {                   // replayed on a larger plan than it was launched for
+    if (tid == 0) v.head->status = KV8_STALE;
+    return;
+  }
+  if ((int)blockIdx.x >= v.head->runs) return;
+  const Kv8Run run = v.runs[blockIdx.x];
+  const int t = run.t, slot = run.slot, m = run.m, f = slot % kKv8Block;
   const T* x = (is_v ? val : k) + (int64_t)t * (is_v ? v_stride : k_stride) + g * HD;
   const int64_t ld = is_v ? v_stride : k_stride;
   float a = 0.0f;
@@ -238,47 +116,6 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8View v, int layer, const in
   val[i] = c;
 }
 
-// Attention of one row and head by one wave: a page at a time, with the running maximum and sum of the softmax.
-template <int HD, class T>
-__global__ __launch_bounds__(64) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                   int64_t q_stride, int64_t out_stride, float scale) {
-  __shared__ float qs[HD];
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, g = h / (v.H / v.KVH);
-  if (t >= v.head->rows) return;
-  for (int d = lane; d < HD; d += 64) qs[d] = (float)q[t * q_stride + h * HD + d];
-  __syncthreads();
-  const int last = v.pos[t];
-  const int* const table = v.table + (size_t)v.seq[t] * v.W;
-  float m = -__builtin_inff(), l = 0.0f, o[HD / 64] = {};
-  for (int p0 = 0; p0 <= last; p0 += kKv8Block) {
-    const size_t block = ((size_t)layer * v.pages + table[p0 / kKv8Block]) * v.KVH + g;
-    const uint8_t* const kc = v.codes + block * 2 * (kKv8Block * HD);
-    const uint8_t* const vc = kc + kKv8Block * HD;
-    const float2 s = v.scales[block];
-    const int tok = lane & 31;
-    float x = 0.0f;
-    for (int d = (lane >> 5) * (HD / 2), i = 0; i < HD / 2; i++, d++)
-      x = __builtin_fmaf(qs[d], (float)((int)kc[kv8_k_byte(HD, tok, d)] - 128), x);
-    x += __shfl_xor(x, 32);
-    x = p0 + tok <= last ? x * (s.x * scale) : -__builtin_inff();
-    float most = x;
-    for (int d = 1; d < 32; d <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
-    const float m2 = __builtin_fmaxf(m, most);
-    const float w = expf(x - m2), old = expf(m - m2);
-    float sum = w;
-    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
-    l = l * old + sum;
-    for (int c = 0; c < HD / 64; c++) o[c] *= old;
-    for (int j = 0; j < kKv8Block; j++) {
-      const float wj = __shfl(w, j) * s.y;
-      for (int c = 0; c < HD / 64; c++)
-        o[c] = __builtin_fmaf(wj, (float)((int)vc[kv8_v_byte(j, c * 64 + lane)] - 128), o[c]);
-    }
-    m = m2;
-  }
-  for (int c = 0; c < HD / 64; c++) out[t * out_stride + h * HD + c * 64 + lane] = (T)(o[c] / l);
-}
-
 // The free pages in the order in which they are taken, and a table without pages.
 __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -288,7 +125,7 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
     v.starts[i] = 0;
     if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
   }
-  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages};
+  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 1};
 }
 
 int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
@@ -314,6 +151,8 @@ int plan_error(const q4hip_kv8* kv, int status) {
     case KV8_OK: return Q4HIP_OK;
     case KV8_BAD_LENGTH: return fail(Q4HIP_EINVAL, "plan: a negative length");
     case KV8_TOO_LONG: return fail(Q4HIP_ECONTEXT, "plan: a sequence longer than %d positions", kv->v.max_len);
+    case KV8_STALE:
+      return fail(Q4HIP_ESTATE, "append or attend replayed on a plan of more rows than they were captured for");
     case KV8_ROWS: return fail(Q4HIP_EINVAL, "plan: more rows than the %d it was called for", kv->rows);
     default: return fail(Q4HIP_ECONTEXT, "plan: more than the pool's %d pages", kv->v.pages);
   }
@@ -344,7 +183,8 @@ void q4hip_kv8_destroy(q4hip_kv8* kv) {
   (void)hipSetDevice(kv->device);
   if (kv->stream) (void)hipStreamSynchronize(kv->stream);
   Kv8View& v = kv->v;
-  void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.seq, v.pos, v.slot};
+  void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
+                  v.run_at, v.item_at, v.part_at, v.runs, v.items, v.part_o, v.part_ml, v.arrived};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (kv->pin) (void)hipHostFree(kv->pin);
   if (kv->stream) (void)hipStreamDestroy(kv->stream);
@@ -373,6 +213,10 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   Kv8View& v = kv->v;
   v.layers = layers; v.H = heads; v.KVH = kv_heads; v.HD = head_dim;
   v.B = seqs; v.W = (max_len + kKv8Block - 1) / kKv8Block; v.pages = pages; v.max_len = max_len;
+  const int G = heads / kv_heads;
+  v.unit_rows = std::max(1, 16 / G);
+  v.row_tiles = (std::min(v.unit_rows, max_rows) * G + 15) / 16;
+  v.items_aim = std::max(1, kItemsAim / (kv_heads * v.row_tiles));
   const size_t blocks = (size_t)layers * pages * kv_heads, bytes = blocks * 2 * kKv8Block * head_dim;
   hipError_t e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
   auto al = [&](auto** p, size_t n) { if (e == hipSuccess) e = hipMalloc((void**)p, n * sizeof(**p)); };
@@ -384,13 +228,18 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.head, 1);
   al(&v.base, seqs);
   al(&v.lens, seqs);
-  al(&v.starts, (size_t)seqs + 1);
-  al(&v.seq, max_rows);
-  al(&v.pos, max_rows);
-  al(&v.slot, max_rows);
+  for (int** p : {&v.starts, &v.free_at, &v.take_at, &v.run_at, &v.item_at, &v.part_at}) al(p, (size_t)seqs + 1);
+  al(&v.runs, max_rows);
+  al(&v.items, (size_t)max_rows + v.items_aim);
+  // units in several parts: each has more pages than a part, so that they have at most twice the parts aimed at
+  const size_t parts = (size_t)2 * v.items_aim * kv_heads * v.row_tiles;
+  al(&v.part_o, parts * 16 * head_dim);
+  al(&v.part_ml, parts * 16);
+  al(&v.arrived, parts);
   if (e == hipSuccess) e = hipHostMalloc((void**)&kv->pin, sizeof(Kv8Head), hipHostMallocDefault);
   if (e == hipSuccess) e = hipMemsetAsync(v.codes, 128, bytes, kv->stream);
   if (e == hipSuccess) e = hipMemsetAsync(v.scales, 0, blocks * sizeof(float2), kv->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(v.arrived, 0, parts * sizeof(int), kv->stream);
   if (e == hipSuccess) {
     const size_t n = std::max({(size_t)seqs * v.W, (size_t)pages, (size_t)seqs + 1});
     k_kv8_reset<<<(unsigned)((n + 255) / 256), 256, 0, kv->stream>>>(v);
@@ -422,9 +271,12 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
     }
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   kv->rows = rows;
-  k_kv8_plan<<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts);
-  const int wgs = std::max((rows + 255) / 256, tables ? (int)std::min<size_t>(((size_t)v.B * v.W + 255) / 256, 512) : 0);
-  if (wgs) k_kv8_rows<<<wgs, 256, 0, s>>>(v, positions, slots, tables);
+  // what the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds
+  const size_t entries = std::max<size_t>(rows + std::min<size_t>(v.items_aim, rows ? (size_t)v.pages * rows : 0),
+                                          tables ? (size_t)v.B * v.W : 0);
+  const bool fill = entries <= kFillInPlan;
+  k_kv8_plan<<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
   HIPCHK(hipGetLastError());
   if (stream) return Q4HIP_OK;
   const int rc = read_head(kv, s);
@@ -453,11 +305,12 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   if (!rc) rc = check_rows(kv, v, kv->rows, w.KVH * w.HD, v_stride, type, "v");
   if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  const dim3 grid((unsigned)kv->rows, (unsigned)w.KVH, 2);
+  // runs of a sequence: its rows over 32, and two at its ends
+  const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)w.KVH, 2);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    if (w.HD == 64) k_kv8_append<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride);
-    else k_kv8_append<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride);
+    if (w.HD == 64) k_kv8_append<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
+    else k_kv8_append<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
@@ -500,13 +353,16 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   rc = check_rows(kv, q, kv->rows, w.H * w.HD, q_stride, type, "q");
   if (!rc) rc = check_rows(kv, out, kv->rows, w.H * w.HD, out_stride, type, "out");
   if (rc) return rc;
-  if (scale == 0.0f) scale = 1.0f / std::sqrt((float)w.HD);
+  // the softmax's exponentials are powers of two
+  const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  const dim3 grid((unsigned)kv->rows, (unsigned)w.H);
+  const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
+  const dim3 grid((unsigned)(units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart))),
+                  (unsigned)(w.KVH * w.row_tiles));
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    if (w.HD == 64) k_kv8_attend<64, T><<<grid, 64, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, scale);
-    else k_kv8_attend<128, T><<<grid, 64, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, scale);
+    if (w.HD == 64) k_kv8_attend<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
+    else k_kv8_attend<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
