@@ -38,6 +38,18 @@ __device__ inline float kv8_max_quarters(float x) {      // over lanes l, l ^ 16
   return __builtin_fmaxf(x, __shfl_xor(x, 32));
 }
 
+// Parts of a unit travel between workgroups, whose XCDs have L2 caches of their own: 8-byte accesses of agent scope,
+// which neither cache keeps.  A fence would write back and drop a whole L2 (30 us in a batch of 32 sequences).
+using kv8_word = unsigned long long;
+__device__ inline void kv8_send(float* p, float a, float b) {
+  const kv8_word w = (kv8_word)__float_as_uint(b) << 32 | __float_as_uint(a);
+  __hip_atomic_store((kv8_word*)p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float2 kv8_receive(const float* p) {
+  const kv8_word w = __hip_atomic_load((const kv8_word*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
+}
+
 // A page's codes in the registers of a wave.
 template <int HD>
 struct Kv8Codes {
@@ -215,33 +227,55 @@ __global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const 
         write(row, d, o, l);
       } else {
         const size_t s = slot + (size_t)it.part * gridDim.y;
-        *(kv8_f4*)(v.part_o + (s * 16 + row) * HD + d) = o;
-        if (d == 0) v.part_ml[s * 16 + row] = {m, l};
+        if (r0 + row >= it.n * G) continue;
+        float* const p = v.part_o + (s * 16 + row) * HD + d;
+        kv8_send(p, o[0], o[1]);
+        kv8_send(p + 2, o[2], o[3]);
+        if (d == 0) kv8_send((float*)(v.part_ml + s * 16 + row), m, l);
       }
     }
     if (it.parts > 1) {
-      __threadfence();                         // the part is visible before its arrival
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the part has arrived in memory before it is counted
       __syncthreads();
       if (tid == 0) {
-        last = atomicAdd(v.arrived + slot, 1) == it.parts - 1;
-        if (last) v.arrived[slot] = 0;         // for the next launch
+        last = __hip_atomic_fetch_add(v.arrived + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.parts - 1;
+        if (last) __hip_atomic_store(v.arrived + slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
       }
       __syncthreads();
       if (last) {
-        __threadfence();
+        const size_t next = (size_t)gridDim.y * 16;          // from a part's rows to the next part's
         for (int e = tid; e < 4 * HD; e += 256) {
           const int row = e / (HD / 4), d = e % (HD / 4) * 4;
           if (r0 + row >= it.n * G) continue;
+          const float* const ml = (const float*)(v.part_ml + slot * 16 + row);
+          const float* const po = v.part_o + (slot * 16 + row) * HD + d;
           float m = kKv8Lowest, l = 0.0f;
-          for (int k = 0; k < it.parts; k++) m = __builtin_fmaxf(m, v.part_ml[(slot + (size_t)k * gridDim.y) * 16 + row].x);
           kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int k = 0; k < it.parts; k++) {
-            const size_t s = (slot + (size_t)k * gridDim.y) * 16 + row;
-            const float2 ml = v.part_ml[s];
-            const float f = __builtin_amdgcn_exp2f(ml.x - m);
-            l = __builtin_fmaf(ml.y, f, l);
-            const kv8_f4 x = *(const kv8_f4*)(v.part_o + s * HD + d);
-            for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+          for (int k0 = 0; k0 < it.parts; k0 += 8) {         // 8 parts on their way at once
+            float2 a[8], x[8][2];
+            float m2 = m;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const size_t at = (size_t)min(k0 + k, it.parts - 1) * next;
+              a[k] = kv8_receive(ml + at * 2);
+              x[k][0] = kv8_receive(po + at * HD);
+              x[k][1] = kv8_receive(po + at * HD + 2);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) m2 = __builtin_fmaxf(m2, a[k].x);
+            const float f0 = __builtin_amdgcn_exp2f(m - m2);
+            l *= f0;
+            o *= f0;
+            m = m2;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const float f = k0 + k < it.parts ? __builtin_amdgcn_exp2f(a[k].x - m) : 0.0f;
+              l = __builtin_fmaf(a[k].y, f, l);
+              o[0] = __builtin_fmaf(x[k][0].x, f, o[0]);
+              o[1] = __builtin_fmaf(x[k][0].y, f, o[1]);
+              o[2] = __builtin_fmaf(x[k][1].x, f, o[2]);
+              o[3] = __builtin_fmaf(x[k][1].y, f, o[3]);
+            }
           }
           write(row, d, o, l);
         }

@@ -91,11 +91,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
                                                            int* __restrict__ pos_out, int* __restrict__ slot_out,
                                                            int* __restrict__ tables_out, bool fill) {
   __shared__ int part[kPlanThreads / 64][4];
-  __shared__ unsigned long long adds, needs, work;
-  __shared__ int bad;
+  __shared__ unsigned long long sums[kPlanThreads / 64][3];
+  __shared__ int worsts[kPlanThreads / 64];
   const int tid = threadIdx.x;
-  if (tid == 0) { adds = 0; needs = 0; work = 0; bad = KV8_OK; }
-  __syncthreads();
   unsigned long long a_sum = 0, n_sum = 0, w_sum = 0;
   int worst = KV8_OK;
   for (int b = tid; b < v.B; b += kPlanThreads) {
@@ -109,11 +107,27 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
       w_sum += (unsigned long long)kv8_units(v, a) * need;
     }
   }
-  atomicAdd(&adds, a_sum);
-  atomicAdd(&needs, n_sum);
-  atomicAdd(&work, w_sum);
-  if (worst) atomicMax(&bad, worst);
+  for (int d = 1; d < 64; d <<= 1) {
+    a_sum += __shfl_xor(a_sum, d);
+    n_sum += __shfl_xor(n_sum, d);
+    w_sum += __shfl_xor(w_sum, d);
+    worst = max(worst, __shfl_xor(worst, d));
+  }
+  if ((tid & 63) == 0) {
+    sums[tid >> 6][0] = a_sum;
+    sums[tid >> 6][1] = n_sum;
+    sums[tid >> 6][2] = w_sum;
+    worsts[tid >> 6] = worst;
+  }
   __syncthreads();
+  unsigned long long adds = 0, needs = 0, work = 0;
+  int bad = KV8_OK;
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    adds += sums[w][0];
+    needs += sums[w][1];
+    work += sums[w][2];
+    bad = max(bad, worsts[w]);
+  }
   Kv8Head head = *v.head;
   const int free0 = head.free_pages;
   head.status = bad ? bad : adds > (unsigned long long)rows ? KV8_ROWS : needs > (unsigned long long)v.pages ? KV8_PAGES : KV8_OK;
