@@ -15,15 +15,19 @@ namespace {
 constexpr int kItemsAim = 512;          // workgroups of attention that fill the GPU
 constexpr size_t kFillInPlan = 8192;
 
-// Nothing but a value's own bits decides: a NaN counts as 0, an infinity as the block's largest value.
-__device__ float magnitude(float x) {
-  const float a = __builtin_fabsf(x);
-  return a < __builtin_inff() ? a : 0.0f;
+// The quotient x / s rounded to fp32, from r = 1 / s rounded: one correction of x * r by its residual gives it
+// (P. Markstein, IBM J. Res. Dev. 34(1), 1990) where the residual is exact, which |x / s| >= 1/4 and s >= 2^-100 make
+// it; a smaller quotient has the code 0 either way.  Then rounded to the nearest even integer by the
+// addition of 1.5 * 2^23, whose last byte becomes the code.
+__device__ uint32_t code_bits(float x, float s, float r) {
+  const float q0 = x * r, q = __builtin_fmaf(__builtin_fmaf(-q0, s, x), r, q0);
+  return __float_as_uint(q + (12582912.0f + 128.0f));
 }
 
-__device__ int to_code(float x, float s) {
-  if (!(s > 0.0f) || x != x) return 0;
-  return (int)__builtin_fminf(__builtin_fmaxf(__builtin_rintf(x / s), -127.0f), 127.0f);
+// The same of any x: NaN 0, infinities the largest code.
+__device__ uint32_t code_bits_any(float x, float s) {
+  const float q = x != x || !(s > 0.0f) ? 0.0f : __builtin_fminf(__builtin_fmaxf(x / s, -127.0f), 127.0f);
+  return __float_as_uint(q + (12582912.0f + 128.0f));
 }
 
 // The smallest k >= 0 with s * 2^k >= t (s, t > 0).
@@ -33,12 +37,15 @@ __device__ int doublings(float s, float t) {
   return __builtin_amdgcn_frexp_expf(t) - __builtin_amdgcn_frexp_expf(s) + (mt > ms ? 1 : 0);
 }
 
-// A run of rows (blockIdx.x) of one kv head; K for blockIdx.z = 0, else V.
-template <int HD, class T>
+// A run of rows (blockIdx.x) of one kv head; K for blockIdx.z = 0, else V.  The rows pass through shared memory, where
+// their 32-bit values are turned into the order of the codes; a thread forms the 16 codes that lie together.
+// kWide: rows whose 16 bytes can be loaded at once.
+template <int HD, class T, bool kWide>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
                                                     int64_t k_stride, int64_t v_stride, int rows) {
   __shared__ float tile[kKv8Block][HD + 1];
   __shared__ float most[4];
+  __shared__ int odd;                          // a value that is not finite
   const int g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const bool is_v = blockIdx.z != 0;
   if (v.head->rows > rows) {                   // replayed on a larger plan than it was launched for
@@ -47,73 +54,121 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const 
   }
   if ((int)blockIdx.x >= v.head->runs) return;
   const Kv8Run run = v.runs[blockIdx.x];
-  const int t = run.t, slot = run.slot, m = run.m, f = slot % kKv8Block;
-  const T* x = (is_v ? val : k) + (int64_t)t * (is_v ? v_stride : k_stride) + g * HD;
+  const int m = run.m, f = run.slot % kKv8Block;
   const int64_t ld = is_v ? v_stride : k_stride;
+  const T* x = (is_v ? val : k) + (int64_t)run.t * ld + g * HD;
+  const size_t block = ((size_t)layer * v.pages + run.slot / kKv8Block) * v.KVH + g;
+  float* const scale = (float*)(v.scales + block) + (is_v ? 1 : 0);
+  uint4* const codes = (uint4*)(v.codes + (block * 2 + (is_v ? 1 : 0)) * (kKv8Block * HD));
+  const bool whole = m == kKv8Block;
+  const float before = *scale;
+  uint4 w[HD / 128 > 0 ? HD / 128 : 1] = {};
+  if (!whole)
+    for (int i = 0, u = tid; u < 2 * HD; i++, u += 256) w[i] = codes[u];
+  if (tid == 0) odd = 0;
+  __syncthreads();
   float a = 0.0f;
-  for (int i = tid; i < m * HD; i += 256) {
-    const int r = i / HD, c = i % HD;
-    const float y = (float)x[r * ld + c];
+  bool strange = false;
+  auto take = [&](int r, int c, float y) {
     tile[f + r][c] = y;
-    a = __builtin_fmaxf(a, magnitude(y));
+    const float z = __builtin_fabsf(y);
+    if (z < __builtin_inff()) a = __builtin_fmaxf(a, z);
+    else strange = true;
+  };
+  if constexpr (kWide) {
+    constexpr int kVec = 16 / sizeof(T), kCols = HD / kVec;
+    for (int i = tid; i < m * kCols; i += 256) {
+      const int r = i / kCols, c = i % kCols * kVec;
+      struct alignas(16) Vec { T y[kVec]; };
+      const Vec z = *(const Vec*)(x + r * ld + c);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) take(r, c + j, (float)z.y[j]);
+    }
+  } else {
+    for (int i = tid; i < m * HD; i += 256) take(i / HD, i % HD, (float)x[i / HD * ld + i % HD]);
   }
+  if (strange) odd = 1;
+#pragma unroll
   for (int d = 1; d < 64; d <<= 1) a = __builtin_fmaxf(a, __shfl_xor(a, d));
   if (lane == 0) most[tid >> 6] = a;
   __syncthreads();
   a = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
-  const size_t block = ((size_t)layer * v.pages + slot / kKv8Block) * v.KVH + g;
-  float* const scale = (float*)(v.scales + block) + (is_v ? 1 : 0);
-  const float old = f ? *scale : 0.0f, t127 = a / 127.0f, need = t127 < kKv8MinScale ? 0.0f : t127;
+  const float old = f ? before : 0.0f, t127 = a / 127.0f, need = t127 < kKv8MinScale ? 0.0f : t127;
   const int twice = old > 0.0f ? doublings(old, need) : 0;
   const float s = old > 0.0f ? __builtin_ldexpf(old, twice) : need;
-  uint4* const codes = (uint4*)(v.codes + (block * 2 + (is_v ? 1 : 0)) * (kKv8Block * HD));
-  for (int u = tid; u < 2 * HD; u += 256) {
-    uint4 w = codes[u];
-    uint8_t* const b = (uint8_t*)&w;
+  const bool any = odd != 0 || !(s > 0.0f);
+  const float r = any ? 0.0f : 1.0f / s;
+  for (int i = 0, u = tid; u < 2 * HD; i++, u += 256) {
     const int ln = u & 63, q = u >> 6;
-    bool changed = false;
-    for (int j = 0; j < 16; j++) {
+    uint32_t* const words = (uint32_t*)&w[i];
+    bool changed = whole;
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      // four codes: columns of a position of K, positions of a column of V, one after the other
       int tok, col;
       if (is_v) {
-        tok = ((j >> 2) & 1) * 16 + (ln >> 4) * 4 + (j & 3);
+        tok = ((j >> 2) & 1) * 16 + (ln >> 4) * 4;
         col = (2 * q + (j >> 3)) * 16 + (ln & 15);
       } else {
         tok = q / (HD / 64) * 16 + (ln & 15);
         col = (2 * (q % (HD / 64)) + (j >> 3)) * 32 + (ln >> 4) * 8 + (j & 7);
       }
-      if (tok >= f && tok < f + m) {
-        b[j] = (uint8_t)(to_code(tile[tok][col], s) + 128);
-        changed = true;
-      } else if (tok < f && twice) {
-        b[j] = (uint8_t)((int)__builtin_rintf(__builtin_ldexpf((float)((int)b[j] - 128), -twice)) + 128);
+      const int dt = is_v ? 1 : 0, dc = 1 - dt;
+      if (whole && !any) {
+        uint32_t c[4];
+#pragma unroll
+        for (int b = 0; b < 4; b++) c[b] = code_bits(tile[tok + b * dt][col + b * dc], s, r);
+        const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+        words[j >> 2] = lo | hi;
+        continue;
+      }
+      for (int b = 0; b < 4; b++) {
+        const int tk = tok + b * dt, sh = 8 * b;
+        uint32_t c;
+        if (tk >= f && tk < f + m) {
+          const float y = tile[tk][col + b * dc];
+          c = any ? code_bits_any(y, s) : code_bits(y, s, r);
+        } else if (tk < f && twice) {
+          const int before_code = (int)(words[j >> 2] >> sh & 255) - 128;
+          c = (uint32_t)((int)__builtin_rintf(__builtin_ldexpf((float)before_code, -twice)) + 128);
+        } else {
+          continue;
+        }
+        words[j >> 2] = (words[j >> 2] & ~(255u << sh)) | (c & 255u) << sh;
         changed = true;
       }
     }
-    if (changed) codes[u] = w;
+    if (changed) codes[u] = w[i];
   }
-  __syncthreads();                        // every thread has read the old scale
-  if (tid == 0) *scale = s;
+  if (tid == 0 && s != before) *scale = s;      // every thread has read the old one before the barriers
 }
 
-// The values that the cache stands for at n pairs of a sequence and a position; 0 where it holds none.
+// The values that the cache stands for at n pairs of a sequence and a position; 0 where it holds none.  A thread
+// forms 4 columns of K and V of one kv head.
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8View v, int layer, const int* __restrict__ seq, const int* __restrict__ pos,
                                                   int n, float* __restrict__ k, float* __restrict__ val) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = (int64_t)v.KVH * HD;
-  if (i >= n * row) return;
-  const int r = (int)(i / row), g = (int)(i % row) / HD, d = (int)(i % HD);
-  const int b = seq[r], p = pos[r];
-  float a = 0.0f, c = 0.0f;
-  if (b >= 0 && b < v.B && p >= 0 && p < v.lens[b]) {
-    const int t = p % kKv8Block;
-    const size_t block = ((size_t)layer * v.pages + v.table[(size_t)b * v.W + p / kKv8Block]) * v.KVH + g;
-    const uint8_t* codes = v.codes + block * 2 * (kKv8Block * HD);
-    const float2 s = v.scales[block];
-    a = s.x * (float)((int)codes[kv8_k_byte(HD, t, d)] - 128);
-    c = s.y * (float)((int)codes[kKv8Block * HD + kv8_v_byte(t, d)] - 128);
+  constexpr int kCols = HD / 4, kRows = 256 / kCols;
+  const int g = blockIdx.y, d = threadIdx.x % kCols * 4;
+  for (int i = blockIdx.x * kRows + threadIdx.x / kCols; i < n; i += gridDim.x * kRows) {
+    const int b = seq[i], p = pos[i];
+    float a[4] = {}, c[4] = {};
+    if (b >= 0 && b < v.B && p >= 0 && p < v.lens[b]) {
+      const int t = p % kKv8Block;
+      const size_t block = ((size_t)layer * v.pages + v.table[(size_t)b * v.W + p / kKv8Block]) * v.KVH + g;
+      const uint8_t* codes = v.codes + block * 2 * (kKv8Block * HD);
+      const float2 s = v.scales[block];
+      const uint32_t kw = *(const uint32_t*)(codes + kv8_k_byte(HD, t, d));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        a[j] = s.x * (float)((int)(kw >> 8 * j & 255) - 128);
+        c[j] = s.y * (float)((int)codes[kKv8Block * HD + kv8_v_byte(t, d + j)] - 128);
+      }
+    }
+    const size_t at = ((size_t)i * v.KVH + g) * HD + d;
+#pragma unroll
+    for (int j = 0; j < 4; j++) { k[at + j] = a[j]; val[at + j] = c[j]; }
   }
-  k[i] = a;
-  val[i] = c;
 }
 
 // The free pages in the order in which they are taken, and a table without pages.
@@ -275,7 +330,12 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
   const size_t entries = std::max<size_t>(rows + std::min<size_t>(v.items_aim, rows ? (size_t)v.pages * rows : 0),
                                           tables ? (size_t)v.B * v.W : 0);
   const bool fill = entries <= kFillInPlan;
-  k_kv8_plan<<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  if (v.B <= kPlanShared) {
+    const int threads = v.B <= 256 && entries <= 2048 ? 256 : kPlanThreads;
+    k_kv8_plan<true><<<1, threads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  } else {
+    k_kv8_plan<false><<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  }
   if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
   HIPCHK(hipGetLastError());
   if (stream) return Q4HIP_OK;
@@ -307,10 +367,13 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   // runs of a sequence: its rows over 32, and two at its ends
   const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)w.KVH, 2);
+  const bool wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * elem_size(type)) |
+                       (uintptr_t)(v_stride * elem_size(type))) % 16);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    if (w.HD == 64) k_kv8_append<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
-    else k_kv8_append<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
+    auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
+                          : (wide ? k_kv8_append<128, T, true> : k_kv8_append<128, T, false>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
@@ -331,11 +394,11 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
   if (!rc) rc = check_rows(kv, k, n, (int)row, row, Q4HIP_TYPE_F32, "k");
   if (!rc) rc = check_rows(kv, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
   if (rc) return rc;
-  const size_t wgs = (n * row + 255) / 256;
-  if (wgs > INT32_MAX) return fail(Q4HIP_EINVAL, "%d positions at once", n);
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  if (w.HD == 64) k_kv8_read<64><<<(unsigned)wgs, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
-  else k_kv8_read<128><<<(unsigned)wgs, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  const int per = 1024 / w.HD;                 // rows of a workgroup
+  const dim3 grid((unsigned)std::min((n + per - 1) / per, 16384), (unsigned)w.KVH);
+  if (w.HD == 64) k_kv8_read<64><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  else k_kv8_read<128><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;

@@ -2,34 +2,43 @@
 //
 // One workgroup sums over the sequences (pages given back and taken, rows, runs, items); whoever then wants
 // the i-th page, row, run or item finds its sequence by bisection of those sums.  So no thread walks through a
-// long sequence alone, and the second part is spread over the GPU where there is much of it.
+// long sequence alone, and the lists can be spread over the GPU where there is much of them.
+// Nothing but latency bounds it: a chain of loads, sums and bisections.  With up to kPlanShared sequences
+// the sums stay in shared memory (32 sequences 13.2 -> 7.1 us a launch).
 #pragma once
 #include "kv8.h"
 
 namespace q4 {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanShared = 1024;
 
 __device__ inline int kv8_pages(int n) { return (n + kKv8Block - 1) / kKv8Block; }
 
 // Inclusive sums of N numbers over the workgroup's threads; total[] receives the sums of all.
 template <int N>
 __device__ void wg_scan(int (&x)[N], int (&total)[N], int (*part)[N]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
   for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
     for (int k = 0; k < N; k++) {
       const int u = __shfl_up(x[k], d);
       if (lane >= d) x[k] += u;
     }
   __syncthreads();                       // `part` of the sums before has been read
   if (lane == 63)
+#pragma unroll
     for (int k = 0; k < N; k++) part[wave][k] = x[k];
   __syncthreads();
+#pragma unroll
   for (int k = 0; k < N; k++) total[k] = 0;
-  for (int w = 0; w < kPlanThreads / 64; w++)
+  for (int w = 0; w < waves; w++)
+#pragma unroll
     for (int k = 0; k < N; k++) {
-      if (w < wave) x[k] += part[w][k];
-      total[k] += part[w][k];
+      const int p = part[w][k];
+      if (w < wave) x[k] += p;
+      total[k] += p;
     }
 }
 
@@ -43,39 +52,48 @@ __device__ inline int find(const int* at, int B, int i) {
   return lo;
 }
 
-// Units of sequence b's rows, and the parts of each.
+// Units of `add` rows, and the parts of each.
 __device__ inline int kv8_units(const Kv8View& v, int add) { return (add + v.unit_rows - 1) / v.unit_rows; }
 __device__ inline int kv8_parts(int pages, int parts_of) { return (pages + parts_of - 1) / parts_of; }
 
-// Entries i, i + stride, ... of everything that a step's kernels read: rows, runs, items; the caller's copies.
-__device__ inline void kv8_fill(const Kv8View& v, const Kv8Head& h, int first, int stride, int* pos_out, int* slot_out,
-                                int* tables_out) {
-  for (int t = first; t < h.rows && (pos_out || slot_out); t += stride) {
-    const int b = find(v.starts, v.B, t), p = v.base[b] + t - v.starts[b];
-    const int s = v.table[(size_t)b * v.W + p / kKv8Block] * kKv8Block + p % kKv8Block;
-    if (pos_out) pos_out[t] = p;
-    if (slot_out) slot_out[t] = s;
-  }
+// What is known of the sequences, in shared or global memory: [B] positions before and after the step and pages
+// held so far; sums over the sequences before.
+struct Kv8Sums {
+  int *base, *lens, *held, *free_at, *take_at, *starts, *run_at, *item_at, *part_at;
+};
+__device__ inline Kv8Sums kv8_sums(const Kv8View& v) {
+  return {v.base, v.lens, v.held, v.free_at, v.take_at, v.starts, v.run_at, v.item_at, v.part_at};
+}
+
+// Entries first, first + stride, ... of everything that a step's kernels read: runs, items; the caller's copies.
+__device__ __forceinline__ void kv8_fill(const Kv8View& v, const Kv8Sums& s, const Kv8Head& h, int first, int stride, int* pos_out,
+                                         int* slot_out, int* tables_out) {
+  if (pos_out || slot_out)
+    for (int t = first; t < h.rows; t += stride) {
+      const int b = find(s.starts, v.B, t), p = s.base[b] + t - s.starts[b];
+      if (pos_out) pos_out[t] = p;
+      if (slot_out) slot_out[t] = v.table[(size_t)b * v.W + p / kKv8Block] * kKv8Block + p % kKv8Block;
+    }
   for (int i = first; i < h.runs; i += stride) {
-    const int b = find(v.run_at, v.B, i), have = v.base[b], page = have / kKv8Block + i - v.run_at[b];
-    const int p0 = max(have, page * kKv8Block), p1 = min(v.lens[b], (page + 1) * kKv8Block);
-    v.runs[i] = {v.starts[b] + p0 - have, v.table[(size_t)b * v.W + page] * kKv8Block + p0 % kKv8Block, p1 - p0, 0};
+    const int b = find(s.run_at, v.B, i), have = s.base[b], page = have / kKv8Block + i - s.run_at[b];
+    const int p0 = max(have, page * kKv8Block), p1 = min(s.lens[b], (page + 1) * kKv8Block);
+    v.runs[i] = {s.starts[b] + p0 - have, v.table[(size_t)b * v.W + page] * kKv8Block + p0 % kKv8Block, p1 - p0, 0};
   }
   for (int i = first; i < h.items; i += stride) {
-    const int b = find(v.item_at, v.B, i), have = v.base[b], add = v.lens[b] - have;
-    const int parts = kv8_parts(kv8_pages(v.lens[b]), h.parts_of);
-    const int unit = (i - v.item_at[b]) / parts, part = (i - v.item_at[b]) % parts;
+    const int b = find(s.item_at, v.B, i), have = s.base[b], add = s.lens[b] - have;
+    const int parts = kv8_parts(kv8_pages(s.lens[b]), h.parts_of), k = i - s.item_at[b];
+    const int unit = parts == 1 ? k : k / parts, part = k - unit * parts;
     Kv8Item e{};
     e.seq = b;
-    e.t = v.starts[b] + unit * v.unit_rows;
+    e.t = s.starts[b] + unit * v.unit_rows;
     e.n = min(v.unit_rows, add - unit * v.unit_rows);
     e.pos = have + unit * v.unit_rows;
-    const int pages = kv8_pages(e.pos + e.n), each = (pages + parts - 1) / parts;
+    const int pages = kv8_pages(e.pos + e.n), each = parts == 1 ? pages : (pages + parts - 1) / parts;
     e.page0 = min(part * each, pages);
     e.pages = min(each, pages - e.page0);
     e.part = part;
     e.parts = parts;
-    e.slot = parts > 1 ? v.part_at[b] + unit * parts : -1;
+    e.slot = parts > 1 ? s.part_at[b] + unit * parts : -1;
     v.items[i] = e;
   }
   if (tables_out) {
@@ -86,18 +104,24 @@ __device__ inline void kv8_fill(const Kv8View& v, const Kv8Head& h, int first, i
 
 // Pages and sums of a step from have[b] and add[b].  Pages beyond a sequence's need go back to the stack in
 // the order of the sequences, then they are taken from its top in that order.  `fill`: the lists, too.
+// kShared: v.B <= kPlanShared and one thread a sequence.
+template <bool kShared>
 __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int* __restrict__ have,
                                                            const int* __restrict__ add, int rows, int* __restrict__ starts_out,
                                                            int* __restrict__ pos_out, int* __restrict__ slot_out,
                                                            int* __restrict__ tables_out, bool fill) {
-  __shared__ int part[kPlanThreads / 64][4];
+  __shared__ int part[kPlanThreads / 64][6];
   __shared__ unsigned long long sums[kPlanThreads / 64][3];
   __shared__ int worsts[kPlanThreads / 64];
-  const int tid = threadIdx.x;
+  __shared__ int store[kShared ? 9 : 1][kShared ? kPlanShared : 1];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  Kv8Sums s = kv8_sums(v);
+  if constexpr (kShared) s = {store[0], store[1], store[2], store[3], store[4], store[5], store[6], store[7], store[8]};
+  Kv8Head head = *v.head;
   unsigned long long a_sum = 0, n_sum = 0, w_sum = 0;
-  int worst = KV8_OK;
-  for (int b = tid; b < v.B; b += kPlanThreads) {
-    const int h = have[b], a = add[b];
+  int worst = KV8_OK, mine[3] = {};
+  for (int b = tid; b < v.B; b += threads) {
+    const int h = have[b], a = add[b], had = kShared ? v.held[b] : 0;
     if (h < 0 || a < 0) worst = max(worst, (int)KV8_BAD_LENGTH);
     else if ((long long)h + a > v.max_len) worst = max(worst, (int)KV8_TOO_LONG);
     else {
@@ -106,7 +130,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
       n_sum += need;
       w_sum += (unsigned long long)kv8_units(v, a) * need;
     }
+    if constexpr (kShared) { mine[0] = h; mine[1] = a; mine[2] = had; }
   }
+#pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     a_sum += __shfl_xor(a_sum, d);
     n_sum += __shfl_xor(n_sum, d);
@@ -122,90 +148,102 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   __syncthreads();
   unsigned long long adds = 0, needs = 0, work = 0;
   int bad = KV8_OK;
-  for (int w = 0; w < kPlanThreads / 64; w++) {
+  for (int w = 0; w < threads >> 6; w++) {
     adds += sums[w][0];
     needs += sums[w][1];
     work += sums[w][2];
     bad = max(bad, worsts[w]);
   }
-  Kv8Head head = *v.head;
   const int free0 = head.free_pages;
   head.status = bad ? bad : adds > (unsigned long long)rows ? KV8_ROWS : needs > (unsigned long long)v.pages ? KV8_PAGES : KV8_OK;
   if (head.status) {
     head.rows = head.runs = head.items = 0;
-    for (int b = tid; b <= v.B; b += kPlanThreads) {
+    for (int b = tid; b <= v.B; b += threads) {
       v.starts[b] = 0;
       if (starts_out) starts_out[b] = 0;
     }
     if (tid == 0) *v.head = head;
-    if (fill) kv8_fill(v, head, tid, kPlanThreads, nullptr, nullptr, tables_out);
+    if (fill) kv8_fill(v, s, head, tid, threads, nullptr, nullptr, tables_out);
     return;
   }
   // a unit's pages are shared where there are too few units to fill the GPU
-  head.parts_of = (int)max((unsigned long long)kKv8MinPart, (work + v.items_aim - 1) / v.items_aim);
-  int sum[4] = {}, more[2] = {};
-  for (int b0 = 0; b0 < v.B; b0 += kPlanThreads) {
+  const unsigned long long share = work + v.items_aim - 1;
+  head.parts_of = max(kKv8MinPart, share < 0x100000000ull ? (int)((uint32_t)share / (uint32_t)v.items_aim) : (int)(share / v.items_aim));
+  int sum[6] = {};
+  for (int b0 = 0; b0 < v.B; b0 += threads) {
     const int b = b0 + tid;
-    int x[4] = {}, y[2] = {}, total[4], total2[2];
-    int own[4] = {}, own2[2] = {};
+    int x[6] = {}, own[6] = {}, total[6];
     if (b < v.B) {
-      const int h = have[b], a = add[b], need = kv8_pages(h + a), had = v.held[b], u = kv8_units(v, a);
-      const int parts = kv8_parts(need, head.parts_of);
+      const int h = kShared ? mine[0] : have[b], a = kShared ? mine[1] : add[b], had = kShared ? mine[2] : v.held[b];
+      const int need = kv8_pages(h + a), u = kv8_units(v, a), parts = kv8_parts(need, head.parts_of);
       v.base[b] = h;
       v.lens[b] = h + a;
+      if constexpr (kShared) {
+        s.base[b] = h;
+        s.lens[b] = h + a;
+        s.held[b] = had;
+        v.held[b] = need;
+      }
       own[0] = max(had - need, 0);
       own[1] = max(need - had, 0);
       own[2] = a;
       own[3] = a ? need - h / kKv8Block : 0;
-      own2[0] = u * parts;
-      own2[1] = parts > 1 ? u * parts : 0;
+      own[4] = u * parts;
+      own[5] = parts > 1 ? u * parts : 0;
     }
-    for (int k = 0; k < 4; k++) x[k] = own[k];
-    for (int k = 0; k < 2; k++) y[k] = own2[k];
-    wg_scan<4>(x, total, part);
-    wg_scan<2>(y, total2, (int(*)[2])part);
+#pragma unroll
+    for (int k = 0; k < 6; k++) x[k] = own[k];
+    wg_scan<6>(x, total, part);
+#pragma unroll
+    for (int k = 0; k < 6; k++) {
+      x[k] += sum[k] - own[k];
+      sum[k] += total[k];
+    }
     if (b < v.B) {
-      v.free_at[b] = sum[0] + x[0] - own[0];
-      v.take_at[b] = sum[1] + x[1] - own[1];
-      v.starts[b] = sum[2] + x[2] - own[2];
-      if (starts_out) starts_out[b] = sum[2] + x[2] - own[2];
-      v.run_at[b] = sum[3] + x[3] - own[3];
-      v.item_at[b] = more[0] + y[0] - own2[0];
-      v.part_at[b] = more[1] + y[1] - own2[1];
+      s.free_at[b] = x[0];
+      s.take_at[b] = x[1];
+      s.starts[b] = x[2];
+      s.run_at[b] = x[3];
+      s.item_at[b] = x[4];
+      s.part_at[b] = x[5];
+      if (starts_out) starts_out[b] = x[2];
+      if (kShared && !fill) { v.starts[b] = x[2]; v.run_at[b] = x[3]; v.item_at[b] = x[4]; v.part_at[b] = x[5]; }
     }
-    for (int k = 0; k < 4; k++) sum[k] += total[k];
-    for (int k = 0; k < 2; k++) more[k] += total2[k];
   }
-  __syncthreads();
-  for (int i = tid; i < sum[0]; i += kPlanThreads) {
-    const int b = find(v.free_at, v.B, i);
-    int* e = v.table + (size_t)b * v.W + kv8_pages(v.lens[b]) + i - v.free_at[b];
-    v.stack[free0 + i] = *e;
-    *e = -1;
-  }
-  __syncthreads();
-  const int top = free0 + sum[0];
-  for (int i = tid; i < sum[1]; i += kPlanThreads) {
-    const int b = find(v.take_at, v.B, i);
-    v.table[(size_t)b * v.W + v.held[b] + i - v.take_at[b]] = v.stack[top - 1 - i];
-  }
-  __syncthreads();
-  for (int b = tid; b < v.B; b += kPlanThreads) v.held[b] = kv8_pages(v.lens[b]);
   head.rows = sum[2];
-  head.free_pages = top - sum[1];
+  head.free_pages = free0 + sum[0] - sum[1];
   head.runs = sum[3];
-  head.items = more[0];
+  head.items = sum[4];
   if (tid == 0) {
-    v.starts[v.B] = sum[2];
     if (starts_out) starts_out[v.B] = sum[2];
     *v.head = head;
   }
-  if (fill) kv8_fill(v, head, tid, kPlanThreads, pos_out, slot_out, tables_out);
+  __syncthreads();
+  if (sum[0]) {
+    for (int i = tid; i < sum[0]; i += threads) {
+      const int b = find(s.free_at, v.B, i);
+      int* e = v.table + (size_t)b * v.W + kv8_pages(s.lens[b]) + i - s.free_at[b];
+      v.stack[free0 + i] = *e;
+      *e = -1;
+    }
+    __syncthreads();
+  }
+  if (sum[1]) {
+    const int top = free0 + sum[0];
+    for (int i = tid; i < sum[1]; i += threads) {
+      const int b = find(s.take_at, v.B, i);
+      v.table[(size_t)b * v.W + s.held[b] + i - s.take_at[b]] = v.stack[top - 1 - i];
+    }
+    __syncthreads();
+  }
+  if constexpr (!kShared)
+    for (int b = tid; b < v.B; b += threads) v.held[b] = kv8_pages(s.lens[b]);
+  if (fill) kv8_fill(v, s, head, tid, threads, pos_out, slot_out, tables_out);
 }
 
 __global__ __launch_bounds__(256) void k_kv8_fill(Kv8View v, int* __restrict__ pos_out, int* __restrict__ slot_out,
                                                   int* __restrict__ tables_out) {
-  kv8_fill(v, *v.head, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, pos_out, slot_out, tables_out);
+  kv8_fill(v, kv8_sums(v), *v.head, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, pos_out, slot_out, tables_out);
 }
 
 }  // namespace q4
