@@ -18,6 +18,9 @@ namespace q4 {
 
 constexpr int kKv8Block = 32;
 constexpr int kKv8MinPart = 16;               // pages of the smallest part of a unit
+constexpr int kKv8TileRows = 128;
+// Sequences that add more rows than kKv8Few are taken in tiles where these fill kKv8MinTiles workgroups.
+constexpr int kKv8Few = 16, kKv8MinTiles = 128;
 constexpr float kKv8MinScale = 0x1p-100f;     // a smaller scale is 0, and so are the values
 
 __host__ __device__ constexpr int kv8_k_byte(int HD, int t, int d) {
@@ -34,7 +37,7 @@ struct Kv8Head {
   int status;      // KV8_*
   int rows;        // rows of the plan, 0 when it failed
   int free_pages;
-  int runs, items;
+  int runs, items, tiles;
   int parts_of;    // pages from which on a unit's pages are shared among several items, and in parts of how many
 };
 enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE };
@@ -54,6 +57,13 @@ struct Kv8Item {
   int parts, unused[3];
 };
 
+// A tile: kKv8TileRows rows of attention (positions x G) of a sequence with many rows.
+struct Kv8Tile {
+  int seq, t, n;         // sequence, its first row, its rows
+  int pos;               // position of the first row
+  int tile, unused[3];
+};
+
 // The device side of a cache.
 struct Kv8View {
   uint8_t* codes;      // [layers][pages][kv_heads][K, V][32 * HD]
@@ -64,10 +74,11 @@ struct Kv8View {
   Kv8Head* head;
   int *base, *lens;    // [seqs] positions before and after the step
   int* starts;         // [seqs + 1] first row of a sequence in the step
-  int *free_at, *take_at, *run_at, *item_at, *part_at;   // [seqs + 1] sums over the sequences before: pages given back
-                       // and taken, runs, items, slots in the workspace
+  int *free_at, *take_at, *run_at, *item_at, *part_at, *tile_at;   // [seqs + 1] sums over the sequences before: pages
+                       // given back and taken, runs, items, slots in the workspace, tiles
   Kv8Run* runs;
   Kv8Item* items;
+  Kv8Tile* tiles;
   float* part_o;       // [slots][kv_heads * row tiles][16][HD] sums of a part, relative to 2^part_ml.x
   float2* part_ml;     // [slots][kv_heads * row tiles][16] reference exponent, sum of the probabilities
   int* arrived;        // [slots][kv_heads * row tiles] parts of a unit that are done (at its first slot)

@@ -180,7 +180,12 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
     v.starts[i] = 0;
     if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
   }
-  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 1};
+  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1};
+}
+
+// At most so many tiles have `rows` rows: of full ones, and of a last one of each sequence.
+size_t tiles_bound(const Kv8View& v, int rows) {
+  return (size_t)((int64_t)rows * (v.H / v.KVH) / kKv8TileRows + std::min(v.B, rows / (kKv8Few + 1)) + 1);
 }
 
 int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
@@ -239,7 +244,7 @@ void q4hip_kv8_destroy(q4hip_kv8* kv) {
   if (kv->stream) (void)hipStreamSynchronize(kv->stream);
   Kv8View& v = kv->v;
   void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
-                  v.run_at, v.item_at, v.part_at, v.runs, v.items, v.part_o, v.part_ml, v.arrived};
+                  v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (kv->pin) (void)hipHostFree(kv->pin);
   if (kv->stream) (void)hipStreamDestroy(kv->stream);
@@ -283,9 +288,10 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.head, 1);
   al(&v.base, seqs);
   al(&v.lens, seqs);
-  for (int** p : {&v.starts, &v.free_at, &v.take_at, &v.run_at, &v.item_at, &v.part_at}) al(p, (size_t)seqs + 1);
+  for (int** p : {&v.starts, &v.free_at, &v.take_at, &v.run_at, &v.item_at, &v.part_at, &v.tile_at}) al(p, (size_t)seqs + 1);
   al(&v.runs, max_rows);
   al(&v.items, (size_t)max_rows + v.items_aim);
+  al(&v.tiles, tiles_bound(v, max_rows));
   // units in several parts: each has more pages than a part, so that they have at most twice the parts aimed at
   const size_t parts = (size_t)2 * v.items_aim * kv_heads * v.row_tiles;
   al(&v.part_o, parts * 16 * head_dim);
@@ -420,10 +426,14 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
-  const dim3 grid((unsigned)(units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart))),
-                  (unsigned)(w.KVH * w.row_tiles));
+  const int64_t items = units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
+  const dim3 grid((unsigned)std::min<int64_t>(items, 8 * w.items_aim), (unsigned)(w.KVH * w.row_tiles));
+  const unsigned tiles = kv->rows > kKv8Few ? (unsigned)tiles_bound(w, kv->rows) * w.KVH : 0;
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
+    if (tiles)
+      (w.HD == 64 ? k_kv8_prompt<64, T, 2> : k_kv8_prompt<128, T, 2>)<<<tiles, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride,
+                                                                                      out_stride, log2_scale, kv->rows);
     if (w.HD == 64) k_kv8_attend<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
     else k_kv8_attend<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
   });

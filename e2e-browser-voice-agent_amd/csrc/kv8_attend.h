@@ -1,16 +1,22 @@
-// kv8_attend.h -- attention of a few rows over the paged 8-bit cache, on the matrix cores.
+// kv8_attend.h -- attention over the paged 8-bit cache, on the matrix cores.
 //
-// For the rows r of a unit (16 / G neighbouring rows of a sequence and the G heads of a kv head) and its pages:
+// For 16 rows r (a row: a position's q of one head; the heads of a kv head are rows of the same keys) and a page:
 //   S^T = K q^T      16 positions x 16 rows a tile: the operand's positions are the codes as they lie in the cache
-//   w   = 2^(S c + v - m)      c: K scale, attention scale, log2 e; v: exponent of the page's V scale; m: the row's
+//   w   = 2^(S c + v - m)      c: K scale, attention scale, log2 e; v: log2 of the page's V scale; m: the row's
 //                    largest such sum so far, less 14
 //   O^T = V^T w      16 columns x 16 rows a tile, over the 32 positions of a page
 //   l   = sum w 2^-v
 // The scale of V goes into the exponent, so that the weights that the matrix cores take in fp16 are relative to the
 // row's largest contribution and no page needs a product of its own.  The tile of scores leaves the matrix cores
 // with the positions where the second product wants them (kv8.h: the order of V), so no weight changes lanes.
-// Codes become fp16 by a byte permute (0x6400 | u = 1024 + u) and one packed subtraction: exact.  fp32 rows hold
-// q and w as sums of two fp16 numbers and multiply twice; 16-bit rows as one.
+//
+// fp32 rows (kTwo) hold q and w as sums of two fp16 numbers and multiply twice.  Their codes become fp16 by a byte permute
+// (0x6400 | u = 1024 + u) and one packed subtraction, exactly; v is a whole number there and the scale's rest a factor
+// of w, so that 2^-v is exact.
+// 16-bit rows multiply once.  Their codes are the fp16 numbers u * 2^-24, u = code + 128: the byte permute alone.  What
+// the 128 add to a score is subtracted by the product's first addend, and what they add to O in the end, from the
+// sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
+// an earlier one's: its weights may be too small for fp16 where its probabilities are not.)
 #pragma once
 #include "kv8.h"
 
@@ -22,20 +28,29 @@ using kv8_f4 = float __attribute__((ext_vector_type(4)));
 
 constexpr float kKv8Lowest = -3.402823466e38f;
 
-// 8 codes (two words) as the exact fp16 values code - 128.
+// 8 codes (two words) as fp16: code - 128 + 128 = u as u * 2^-24, or exactly code.
+template <bool kExact>
 __device__ inline kv8_h8 kv8_halves(uint32_t lo, uint32_t hi) {
-  const kv8_h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  constexpr uint32_t kHigh = kExact ? 0x64646464u : 0u;
   union { kv8_h2 h[4]; kv8_h8 v; } u;
-  u.h[0] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u)) + off;
-  u.h[1] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u)) + off;
-  u.h[2] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u)) + off;
-  u.h[3] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)) + off;
+  u.h[0] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(kHigh, lo, kExact ? 0x04010400u : 0x0c010c00u));
+  u.h[1] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(kHigh, lo, kExact ? 0x04030402u : 0x0c030c02u));
+  u.h[2] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(kHigh, hi, kExact ? 0x04010400u : 0x0c010c00u));
+  u.h[3] = __builtin_bit_cast(kv8_h2, __builtin_amdgcn_perm(kHigh, hi, kExact ? 0x04030402u : 0x0c030c02u));
+  if constexpr (kExact) {
+    const kv8_h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    for (auto& h : u.h) h += off;
+  }
   return u.v;
 }
 
 __device__ inline float kv8_max_quarters(float x) {      // over lanes l, l ^ 16, l ^ 32, l ^ 48
   x = __builtin_fmaxf(x, __shfl_xor(x, 16));
   return __builtin_fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float kv8_sum_quarters(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
 }
 
 // Parts of a unit travel between workgroups, whose XCDs have L2 caches of their own: 8-byte accesses of agent scope,
@@ -56,96 +71,229 @@ struct Kv8Codes {
   uint4 k[HD / 32], v[HD / 32];
   __device__ void load(const uint8_t* page, int lane) {
     const uint4* p = (const uint4*)page + lane;
+#pragma unroll
     for (int i = 0; i < HD / 32; i++) k[i] = p[i * 64];
+#pragma unroll
     for (int i = 0; i < HD / 32; i++) v[i] = p[(HD / 32 + i) * 64];
   }
 };
 
-// Lane l: row l % 16 of the unit, quarter l / 16 of every contraction.
-template <int HD, bool kTwo>
+// What the softmax needs of a page's scales.
+struct Kv8Scale {
+  float k, v, iv, mant;      // K scale; v, 2^-v; the V scale over 2^v
+};
+template <bool kTwo>
+__device__ inline Kv8Scale kv8_scale(float2 s) {
+  const float vs = s.y > 0.0f ? s.y : kKv8MinScale;          // codes of 0: any scale will do
+  if constexpr (kTwo) {
+    const int e = __builtin_amdgcn_frexp_expf(vs) - 1;
+    return {s.x, (float)e, __builtin_ldexpf(1.0f, -e), __builtin_ldexpf(vs, -e)};
+  } else {
+    const float v = __builtin_amdgcn_logf(vs);
+    return {s.x, v, __builtin_amdgcn_exp2f(-v), 1.0f};
+  }
+}
+
+// 16 N rows of a wave.  Lane l: rows l % 16 of each 16, quarter l / 16 of every contraction.
+template <int HD, bool kTwo, int N>
 struct Kv8Rows {
-  kv8_h8 q[kTwo ? 2 : 1][HD / 32];
-  kv8_f4 o[HD / 16];
-  float m, l, c;      // c: attention scale, log2 e and the power of two that q was divided by
+  kv8_h8 q[N][kTwo ? 2 : 1][HD / 32];
+  kv8_f4 o[N][HD / 16];
+  kv8_f4 first[kTwo ? 1 : N];                     // what the 128 add to the scores, negative
+  float m[N], l[N], c[N], sum[kTwo ? 1 : N];      // c: attention scale, log2 e and the power of two that q was divided by
 
   template <class T>
-  __device__ void init(const T* row, int quarter, bool valid, float scale) {
+  __device__ void init(int t, const T* row, int quarter, bool valid, float scale) {
     float x[HD / 32][8], most = 0.0f;
+#pragma unroll
     for (int s = 0; s < HD / 32; s++)
+#pragma unroll
       for (int i = 0; i < 8; i++) {
         x[s][i] = valid ? (float)row[s * 32 + quarter * 8 + i] : 0.0f;
         most = __builtin_fmaxf(most, __builtin_fabsf(x[s][i]));
       }
     most = kv8_max_quarters(most);
     const int e = 14 - __builtin_amdgcn_frexp_expf(most);      // the largest value becomes 2^13 .. 2^14
+    float all = 0.0f;
+#pragma unroll
     for (int s = 0; s < HD / 32; s++)
+#pragma unroll
       for (int i = 0; i < 8; i++) {
         const float y = __builtin_ldexpf(x[s][i], e);
         const _Float16 hi = (_Float16)y;
-        q[0][s][i] = hi;
-        if constexpr (kTwo) q[1][s][i] = (_Float16)(y - (float)hi);
+        q[t][0][s][i] = hi;
+        if constexpr (kTwo) q[t][1][s][i] = (_Float16)(y - (float)hi);
+        else all += (float)hi;
       }
-    c = __builtin_ldexpf(scale, -e);
-    m = kKv8Lowest;
-    l = 0.0f;
-    for (auto& t : o) t = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    c[t] = __builtin_ldexpf(scale, -e + (kTwo ? 0 : 24));
+    if constexpr (!kTwo) {
+      all = kv8_sum_quarters(all) * -0x1p-17f;                  // 128 * 2^-24
+      first[t] = kv8_f4{all, all, all, all};
+      sum[t] = 0.0f;
+    }
+    m[t] = kKv8Lowest;
+    l[t] = 0.0f;
+#pragma unroll
+    for (auto& x : o[t]) x = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // One page: its codes and scales (k, v), and the number of its positions that this lane's row looks at
-  // (masked: some lane's row does not look at all 32).
-  __device__ void page(const Kv8Codes<HD>& w, float k_scale, float v_scale, int quarter, bool masked, int seen) {
-    kv8_f4 s[2] = {};
-    for (int t = 0; t < 2; t++)
+  // One page: its codes and scales, and the number of its positions that this lane's rows look at (masked: some
+  // lane's row does not look at all 32; faint: a V scale far below that of a page before).
+  __device__ __forceinline__ void page(const Kv8Codes<HD>& w, Kv8Scale sc, int quarter, bool masked, const int (&seen)[N],
+                                       bool faint) {
+    kv8_f4 s[N][2];
+#pragma unroll
+    for (int t = 0; t < N; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if constexpr (kTwo) s[t][h] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        else s[t][h] = first[t];
+      }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
       for (int p = 0; p < HD / 64; p++) {
-        const uint4 a = w.k[t * (HD / 64) + p];
-        const kv8_h8 a0 = kv8_halves(a.x, a.y), a1 = kv8_halves(a.z, a.w);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[0][2 * p], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[0][2 * p + 1], s[t], 0, 0, 0);
-        if constexpr (kTwo) {
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[1][2 * p], s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[1][2 * p + 1], s[t], 0, 0, 0);
+        const uint4 a = w.k[h * (HD / 64) + p];
+        const kv8_h8 a0 = kv8_halves<kTwo>(a.x, a.y), a1 = kv8_halves<kTwo>(a.z, a.w);
+#pragma unroll
+        for (int t = 0; t < N; t++) {
+          s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[t][0][2 * p], s[t][h], 0, 0, 0);
+          s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[t][0][2 * p + 1], s[t][h], 0, 0, 0);
+          if constexpr (kTwo) {
+            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[t][1][2 * p], s[t][h], 0, 0, 0);
+            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[t][1][2 * p + 1], s[t][h], 0, 0, 0);
+          }
         }
       }
-    // v_scale = mant * 2^v with mant in [1, 2)
-    const float vs = v_scale > 0.0f ? v_scale : kKv8MinScale;
-    const int ve = __builtin_amdgcn_frexp_expf(vs) - 1;
-    const float v = (float)ve, mant = __builtin_ldexpf(vs, -ve), ks = k_scale * c;
-    float x[8], most = kKv8Lowest;
-    for (int i = 0; i < 8; i++) {
-      x[i] = __builtin_fmaf(s[i >> 2][i & 3], ks, v);
-      if (masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen) x[i] = -__builtin_inff();
-      most = __builtin_fmaxf(most, x[i]);
-    }
-    if (__builtin_amdgcn_ballot_w64(most - 14.0f > m) != 0) {      // rare but for the first pages
-      const float m2 = __builtin_fmaxf(kv8_max_quarters(most) - 14.0f, m), f = __builtin_amdgcn_exp2f(m - m2);
-      m = m2;
-      l *= f;
-      for (auto& t : o) t *= f;
-    }
-    float sum = 0.0f;
-    kv8_h8 hi, lo;
-    for (int i = 0; i < 8; i++) {
-      const float e = __builtin_amdgcn_exp2f(x[i] - m);
-      sum += e;
-      float y = e * mant;
-      if constexpr (kTwo) asm("" : "+v"(y));      // rounded to fp32 here: else one of its two uses takes the product rounded to fp16 at once
-      hi[i] = (_Float16)y;
-      if constexpr (kTwo) lo[i] = (_Float16)(y - (float)hi[i]);
-    }
-    l = __builtin_fmaf(sum, __builtin_ldexpf(1.0f, -ve), l);
-    for (int p = 0; p < HD / 32; p++) {
-      const kv8_h8 a0 = kv8_halves(w.v[p].x, w.v[p].y), a1 = kv8_halves(w.v[p].z, w.v[p].w);
-      o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hi, o[2 * p], 0, 0, 0);
-      o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hi, o[2 * p + 1], 0, 0, 0);
+    kv8_h8 hi[N], lo[kTwo ? N : 1];
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+      float x[8];
+      const float ks = sc.k * c[t];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[i] = s[t][i >> 2][i & 3];
+        if (masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t]) x[i] = -1e30f;
+      }
+      float most = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) most = __builtin_fmaxf(most, x[i]);
+      most = __builtin_fmaf(most, ks, sc.v);
+      // weights of up to 2^14, or 2^15.5 before m is moved again
+      if (__builtin_amdgcn_ballot_w64(most - (kTwo ? 14.0f : 15.5f) > m[t]) != 0) {
+        const float m2 = __builtin_fmaxf(kv8_max_quarters(most) - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
+        m[t] = m2;
+        l[t] *= f;
+        if constexpr (!kTwo) sum[t] *= f;
+#pragma unroll
+        for (auto& y : o[t]) y *= f;
+      }
+      const float v = sc.v - m[t];
+      [[maybe_unused]] float all = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ks, v));
+        if (masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t]) e = 0.0f;
+        if constexpr (kTwo) {
+          all += e;
+          float y = e * sc.mant;
+          asm("" : "+v"(y));      // rounded to fp32 here: else one of its two uses takes the product rounded to fp16 at once
+          hi[t][i] = (_Float16)y;
+          lo[t][i] = (_Float16)(y - (float)hi[t][i]);
+        } else {
+          hi[t][i] = (_Float16)e;
+        }
+      }
       if constexpr (kTwo) {
-        o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo, o[2 * p], 0, 0, 0);
-        o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo, o[2 * p + 1], 0, 0, 0);
+        l[t] = __builtin_fmaf(all, sc.iv, l[t]);
+      } else {
+        const kv8_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+        const kv8_f4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi[t], kv8_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        all = r[0];
+        sum[t] += all;
+        if (faint) {
+          all = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ks, v));
+            all += masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t] ? 0.0f : e;
+          }
+          all = kv8_sum_quarters(all);
+        }
+        l[t] = __builtin_fmaf(all, sc.iv, l[t]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < HD / 32; p++) {
+      const kv8_h8 a0 = kv8_halves<kTwo>(w.v[p].x, w.v[p].y), a1 = kv8_halves<kTwo>(w.v[p].z, w.v[p].w);
+#pragma unroll
+      for (int t = 0; t < N; t++) {
+        o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hi[t], o[t][2 * p], 0, 0, 0);
+        o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hi[t], o[t][2 * p + 1], 0, 0, 0);
+        if constexpr (kTwo) {
+          o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo[t], o[t][2 * p], 0, 0, 0);
+          o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo[t], o[t][2 * p + 1], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // The sums of the pages seen: o becomes sum w code, l the sum of all quarters.
+  __device__ void finish(int t) {
+    if constexpr (kTwo) {
+      l[t] = kv8_sum_quarters(l[t]);
+    } else {
+      const float f = -128.0f * sum[t];
+#pragma unroll
+      for (auto& x : o[t])
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(x[i], 0x1p24f, f);
+    }
+  }
+
+  // Pages page0 + first, + step, ... (count of them) of a sequence's table, whose first row of this wave lies
+  // at position `from`; lane's row t looks at positions up to last[t].
+  __device__ __forceinline__ void run(const Kv8View& v, int layer, int g, const int* table, int first, int step, int count, int from,
+                                      const int (&last)[N]) {
+    const int lane = threadIdx.x & 63, quarter = lane >> 4;
+    const size_t page_bytes = (size_t)2 * kKv8Block * HD;
+    float top = kKv8Lowest;
+    for (int j0 = 0; j0 < count; j0 += 64) {
+      // lane j holds the place and the scales of the j-th of the next 64 pages
+      const int n = min(64, count - j0);
+      size_t at = 0;
+      Kv8Scale sc = {};
+      if (lane < n) {
+        at = ((size_t)layer * v.pages + table[first + step * (j0 + lane)]) * v.KVH + g;
+        sc = kv8_scale<kTwo>(v.scales[at]);
+      }
+      const uint32_t at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
+      auto page_at = [&](int j) {
+        const size_t b = ((size_t)__builtin_amdgcn_readlane((int)at_hi, j) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)at_lo, j);
+        return v.codes + b * page_bytes;
+      };
+      auto lane_of = [](float x, int j) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), j)); };
+      Kv8Codes<HD> buf[2];
+      buf[0].load(page_at(0), lane);
+      auto one = [&](int j, Kv8Codes<HD>& now, Kv8Codes<HD>& next) __attribute__((always_inline)) {
+        if (j + 1 < n) next.load(page_at(j + 1), lane);
+        const Kv8Scale s = {lane_of(sc.k, j), lane_of(sc.v, j), lane_of(sc.iv, j), kTwo ? lane_of(sc.mant, j) : 1.0f};
+        const int p0 = (first + step * (j0 + j)) * kKv8Block;
+        int seen[N];
+#pragma unroll
+        for (int t = 0; t < N; t++) seen[t] = last[t] + 1 - p0;
+        page(now, s, quarter, p0 + kKv8Block - 1 > from, seen, !kTwo && s.v < top - 12.0f);
+        top = __builtin_fmaxf(top, s.v);
+      };
+      for (int j = 0; j < n; j += 2) {
+        one(j, buf[0], buf[1]);
+        if (j + 1 < n) one(j + 1, buf[1], buf[0]);
       }
     }
   }
 };
 
-// A workgroup takes items of the plan, its four waves every fourth page each, and adds up their sums in shared
+// Few rows.  A workgroup takes items of the plan, its four waves every fourth page each, and adds up their sums in shared
 // memory.  Of a unit in several parts, the workgroup that is done last adds up the parts, in their order.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
@@ -162,48 +310,18 @@ __global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const 
     if (tid == 0) v.head->status = KV8_STALE;
     return;
   }
-  const size_t page_bytes = (size_t)2 * kKv8Block * HD;
   for (int i = blockIdx.x; i < v.head->items; i += gridDim.x) {
     const Kv8Item it = v.items[i];
     const int r = r0 + n, tok = r / G, h = r % G;
     const bool valid = r < it.n * G;
-    Kv8Rows<HD, kTwo> w;
-    w.init(q + (int64_t)(it.t + (valid ? tok : 0)) * q_stride + (g * G + (valid ? h : 0)) * HD, quarter, valid, scale);
-    const int row_pos = it.pos + (valid ? tok : it.n - 1);      // the last position that this lane's row looks at
-    const int* const table = v.table + (size_t)it.seq * v.W + it.page0;
-    const int mine = (it.pages - wave + 3) >> 2;                // this wave's pages: wave, wave + 4, ...
-    for (int j0 = 0; j0 < mine; j0 += 64) {
-      // lane j holds the address and the scales of the j-th of the next 64 pages
-      const int count = min(64, mine - j0);
-      size_t at = 0;
-      float2 sc = {0.0f, 0.0f};
-      if (lane < count) {
-        at = ((size_t)layer * v.pages + table[wave + 4 * (j0 + lane)]) * v.KVH + g;
-        sc = v.scales[at];
-      }
-      const uint32_t at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
-      auto page_at = [&](int j) {
-        const size_t b = ((size_t)__builtin_amdgcn_readlane((int)at_hi, j) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)at_lo, j);
-        return v.codes + b * page_bytes;
-      };
-      Kv8Codes<HD> buf[2];
-      buf[0].load(page_at(0), lane);
-      auto step = [&](int j, Kv8Codes<HD>& now, Kv8Codes<HD>& next) {
-        if (j + 1 < count) next.load(page_at(j + 1), lane);
-        const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.x), j));
-        const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.y), j));
-        const int p0 = (it.page0 + wave + 4 * (j0 + j)) * kKv8Block;
-        w.page(now, ks, vs, quarter, p0 + kKv8Block - 1 > it.pos, row_pos + 1 - p0);
-      };
-      for (int j = 0; j < count; j += 2) {
-        step(j, buf[0], buf[1]);
-        if (j + 1 < count) step(j + 1, buf[1], buf[0]);
-      }
-    }
-    w.l += __shfl_xor(w.l, 16);
-    w.l += __shfl_xor(w.l, 32);
-    if (quarter == 0) { sm[wave][n] = w.m; sl[wave][n] = w.l; }
-    for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&so[wave][n][d * 16 + quarter * 4] = w.o[d];
+    Kv8Rows<HD, kTwo, 1> w;
+    w.init(0, q + (int64_t)(it.t + (valid ? tok : 0)) * q_stride + (g * G + (valid ? h : 0)) * HD, quarter, valid, scale);
+    const int row_last[1] = {it.pos + (valid ? tok : it.n - 1)};
+    w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
+    w.finish(0);
+    if (quarter == 0) { sm[wave][n] = w.m[0]; sl[wave][n] = w.l[0]; }
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&so[wave][n][d * 16 + quarter * 4] = w.o[0][d];
     __syncthreads();
     const size_t slot = (size_t)max(it.slot, 0) * gridDim.y + blockIdx.y;
     auto write = [&](int row, int d, kv8_f4 o, float l) {
@@ -282,6 +400,49 @@ __global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const 
       }
     }
     __syncthreads();                           // the shared sums have been read
+  }
+}
+
+// Many rows: a tile is 64 N neighbouring rows of a sequence and kv head (row r: position r / G of the step, head r % G), 16 N
+// of each wave, which passes over all the pages that they look at.  A tile's kv heads are neighbours in the grid,
+// so that the tiles of one meet on the same XCDs and find its pages in their L2.
+template <int HD, class T, int N>
+__global__ __launch_bounds__(256) void k_kv8_prompt(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
+                                                    int64_t q_stride, int64_t out_stride, float scale, int rows) {
+  constexpr bool kTwo = sizeof(T) == 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH, g = blockIdx.x % v.KVH;
+  if (v.head->rows > rows) {
+    if (threadIdx.x == 0) v.head->status = KV8_STALE;
+    return;
+  }
+  for (int i = blockIdx.x / v.KVH; i < v.head->tiles; i += gridDim.x / v.KVH) {
+    const Kv8Tile it = v.tiles[i];
+    const int64_t r0 = (int64_t)it.tile * kKv8TileRows + wave * (16 * N), end = (int64_t)it.n * G;
+    if (r0 >= end) continue;
+    Kv8Rows<HD, kTwo, N> w;
+    int last[N];
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+      const int64_t r = min(r0 + t * 16 + n, end - 1);        // rows behind the end: as the last one, not written
+      const int tok = (int)(r / G), h = (int)(r % G);
+      last[t] = it.pos + tok;
+      w.init(t, q + (int64_t)(it.t + tok) * q_stride + (g * G + h) * HD, quarter, true, scale);
+    }
+    const int from = it.pos + (int)(r0 / G), to = it.pos + (int)((min(r0 + 16 * N, end) - 1) / G);
+    w.run(v, layer, g, v.table + (size_t)it.seq * v.W, 0, 1, to / kKv8Block + 1, from, last);
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+      w.finish(t);
+      const int64_t r = r0 + t * 16 + n;
+      if (r >= end) continue;
+      T* const p = out + (int64_t)(it.t + (int)(r / G)) * out_stride + (g * G + (int)(r % G)) * HD + quarter * 4;
+      const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t];
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[d * 16 + k] = (T)(w.o[t][d][k] * il);
+    }
   }
 }
 

@@ -54,15 +54,18 @@ __device__ inline int find(const int* at, int B, int i) {
 
 // Units of `add` rows, and the parts of each.
 __device__ inline int kv8_units(const Kv8View& v, int add) { return (add + v.unit_rows - 1) / v.unit_rows; }
+__device__ inline int kv8_tiles(const Kv8View& v, int add) {
+  return add > kKv8Few ? (int)(((int64_t)add * (v.H / v.KVH) + kKv8TileRows - 1) / kKv8TileRows) : 0;
+}
 __device__ inline int kv8_parts(int pages, int parts_of) { return (pages + parts_of - 1) / parts_of; }
 
 // What is known of the sequences, in shared or global memory: [B] positions before and after the step and pages
 // held so far; sums over the sequences before.
 struct Kv8Sums {
-  int *base, *lens, *held, *free_at, *take_at, *starts, *run_at, *item_at, *part_at;
+  int *base, *lens, *held, *free_at, *take_at, *starts, *run_at, *item_at, *part_at, *tile_at;
 };
 __device__ inline Kv8Sums kv8_sums(const Kv8View& v) {
-  return {v.base, v.lens, v.held, v.free_at, v.take_at, v.starts, v.run_at, v.item_at, v.part_at};
+  return {v.base, v.lens, v.held, v.free_at, v.take_at, v.starts, v.run_at, v.item_at, v.part_at, v.tile_at};
 }
 
 // Entries first, first + stride, ... of everything that a step's kernels read: runs, items; the caller's copies.
@@ -96,6 +99,11 @@ __device__ __forceinline__ void kv8_fill(const Kv8View& v, const Kv8Sums& s, con
     e.slot = parts > 1 ? s.part_at[b] + unit * parts : -1;
     v.items[i] = e;
   }
+  for (int i = first; i < h.tiles; i += stride) {
+    const int b = find(s.tile_at, v.B, i), have = s.base[b], add = s.lens[b] - have;
+    // the longest first
+    v.tiles[i] = {b, s.starts[b], add, have, kv8_tiles(v, add) - 1 - (i - s.tile_at[b]), {}};
+  }
   if (tables_out) {
     const size_t n = (size_t)v.B * v.W;
     for (size_t i = first; i < n; i += stride) tables_out[i] = v.table[i];
@@ -110,15 +118,15 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
                                                            const int* __restrict__ add, int rows, int* __restrict__ starts_out,
                                                            int* __restrict__ pos_out, int* __restrict__ slot_out,
                                                            int* __restrict__ tables_out, bool fill) {
-  __shared__ int part[kPlanThreads / 64][6];
-  __shared__ unsigned long long sums[kPlanThreads / 64][3];
+  __shared__ int part[kPlanThreads / 64][7];
+  __shared__ unsigned long long sums[kPlanThreads / 64][5];
   __shared__ int worsts[kPlanThreads / 64];
-  __shared__ int store[kShared ? 9 : 1][kShared ? kPlanShared : 1];
+  __shared__ int store[kShared ? 10 : 1][kShared ? kPlanShared : 1];
   const int tid = threadIdx.x, threads = blockDim.x;
   Kv8Sums s = kv8_sums(v);
-  if constexpr (kShared) s = {store[0], store[1], store[2], store[3], store[4], store[5], store[6], store[7], store[8]};
+  if constexpr (kShared) s = {store[0], store[1], store[2], store[3], store[4], store[5], store[6], store[7], store[8], store[9]};
   Kv8Head head = *v.head;
-  unsigned long long a_sum = 0, n_sum = 0, w_sum = 0;
+  unsigned long long x_sum[5] = {};            // rows, pages, pages of all units and of those outside tiles, tiles
   int worst = KV8_OK, mine[3] = {};
   for (int b = tid; b < v.B; b += threads) {
     const int h = have[b], a = add[b], had = kShared ? v.held[b] : 0;
@@ -126,38 +134,41 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
     else if ((long long)h + a > v.max_len) worst = max(worst, (int)KV8_TOO_LONG);
     else {
       const int need = kv8_pages(h + a);
-      a_sum += a;
-      n_sum += need;
-      w_sum += (unsigned long long)kv8_units(v, a) * need;
+      const unsigned long long w = (unsigned long long)kv8_units(v, a) * need;
+      x_sum[0] += a;
+      x_sum[1] += need;
+      x_sum[2] += w;
+      x_sum[3] += a > kKv8Few ? 0 : w;
+      x_sum[4] += kv8_tiles(v, a);
     }
     if constexpr (kShared) { mine[0] = h; mine[1] = a; mine[2] = had; }
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    a_sum += __shfl_xor(a_sum, d);
-    n_sum += __shfl_xor(n_sum, d);
-    w_sum += __shfl_xor(w_sum, d);
+#pragma unroll
+    for (int k = 0; k < 5; k++) x_sum[k] += __shfl_xor(x_sum[k], d);
     worst = max(worst, __shfl_xor(worst, d));
   }
   if ((tid & 63) == 0) {
-    sums[tid >> 6][0] = a_sum;
-    sums[tid >> 6][1] = n_sum;
-    sums[tid >> 6][2] = w_sum;
+#pragma unroll
+    for (int k = 0; k < 5; k++) sums[tid >> 6][k] = x_sum[k];
     worsts[tid >> 6] = worst;
   }
   __syncthreads();
-  unsigned long long adds = 0, needs = 0, work = 0;
+  unsigned long long adds = 0, needs = 0, work = 0, work_few = 0, tiles = 0;
   int bad = KV8_OK;
   for (int w = 0; w < threads >> 6; w++) {
     adds += sums[w][0];
     needs += sums[w][1];
     work += sums[w][2];
+    work_few += sums[w][3];
+    tiles += sums[w][4];
     bad = max(bad, worsts[w]);
   }
   const int free0 = head.free_pages;
   head.status = bad ? bad : adds > (unsigned long long)rows ? KV8_ROWS : needs > (unsigned long long)v.pages ? KV8_PAGES : KV8_OK;
   if (head.status) {
-    head.rows = head.runs = head.items = 0;
+    head.rows = head.runs = head.items = head.tiles = 0;
     for (int b = tid; b <= v.B; b += threads) {
       v.starts[b] = 0;
       if (starts_out) starts_out[b] = 0;
@@ -167,15 +178,18 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
     return;
   }
   // a unit's pages are shared where there are too few units to fill the GPU
+  const bool in_tiles = tiles * v.KVH >= kKv8MinTiles;
+  if (in_tiles) work = work_few;
   const unsigned long long share = work + v.items_aim - 1;
   head.parts_of = max(kKv8MinPart, share < 0x100000000ull ? (int)((uint32_t)share / (uint32_t)v.items_aim) : (int)(share / v.items_aim));
-  int sum[6] = {};
+  int sum[7] = {};
   for (int b0 = 0; b0 < v.B; b0 += threads) {
     const int b = b0 + tid;
-    int x[6] = {}, own[6] = {}, total[6];
+    int x[7] = {}, own[7] = {}, total[7];
     if (b < v.B) {
       const int h = kShared ? mine[0] : have[b], a = kShared ? mine[1] : add[b], had = kShared ? mine[2] : v.held[b];
-      const int need = kv8_pages(h + a), u = kv8_units(v, a), parts = kv8_parts(need, head.parts_of);
+      const int need = kv8_pages(h + a), nt = in_tiles ? kv8_tiles(v, a) : 0;
+      const int u = nt ? 0 : kv8_units(v, a), parts = kv8_parts(need, head.parts_of);
       v.base[b] = h;
       v.lens[b] = h + a;
       if constexpr (kShared) {
@@ -190,12 +204,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
       own[3] = a ? need - h / kKv8Block : 0;
       own[4] = u * parts;
       own[5] = parts > 1 ? u * parts : 0;
+      own[6] = nt;
     }
 #pragma unroll
-    for (int k = 0; k < 6; k++) x[k] = own[k];
-    wg_scan<6>(x, total, part);
+    for (int k = 0; k < 7; k++) x[k] = own[k];
+    wg_scan<7>(x, total, part);
 #pragma unroll
-    for (int k = 0; k < 6; k++) {
+    for (int k = 0; k < 7; k++) {
       x[k] += sum[k] - own[k];
       sum[k] += total[k];
     }
@@ -206,14 +221,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
       s.run_at[b] = x[3];
       s.item_at[b] = x[4];
       s.part_at[b] = x[5];
+      s.tile_at[b] = x[6];
       if (starts_out) starts_out[b] = x[2];
-      if (kShared && !fill) { v.starts[b] = x[2]; v.run_at[b] = x[3]; v.item_at[b] = x[4]; v.part_at[b] = x[5]; }
+      if (kShared && !fill) { v.starts[b] = x[2]; v.run_at[b] = x[3]; v.item_at[b] = x[4]; v.part_at[b] = x[5]; v.tile_at[b] = x[6]; }
     }
   }
   head.rows = sum[2];
   head.free_pages = free0 + sum[0] - sum[1];
   head.runs = sum[3];
   head.items = sum[4];
+  head.tiles = sum[6];
   if (tid == 0) {
     if (starts_out) starts_out[v.B] = sum[2];
     *v.head = head;

@@ -11,6 +11,10 @@ and the factors' own few roundings.  The sums over n positions add at most (n / 
 matrix product or wave adds 32 positions at a time.  All of this is relative to A = sum_j p_j |V_j|, and a running
 rescale of earlier pages adds one rounding per page, counted in n / 32.
 
+A kernel of 16-bit rows may multiply code + 128 and subtract the 128 from the finished sums.  The summands of a score are
+then q_d s_j (code + 128), those of an output p_j v_j (code + 128), and the roundings above are relative to these:
+S and, for the sums over positions, A are formed of |K_jd| + 128 s_j and |V_j| + 128 v_j.
+
 Two absolute terms.  A kernel that holds p_j times the V scale v_j in fp16, as one number or as the sum of two,
 relative to 2^-14 of the largest such product of the row, rounds the smallest ones to multiples of 2^-24: an
 error of 2^-39 max_i(p_i v_i) for each position, times a code of at most 127.  And a product below 2^-126 of the largest
@@ -104,9 +108,10 @@ class Cache:
         return np.repeat(self.scales[idx].astype(np.float64), BLOCK, axis=0)[:n]
 
 
-def attend(q, K, V, vs, have, scale, half_eps):
-    """(out, bound) in 64 bits of rows q [n][H][hd] over K, V [have + n][KVH][hd] with V's scales vs [have + n][KVH]; half_eps:
+def attend(q, K, V, ks, vs, have, scale, half_eps):
+    """(out, bound) in 64 bits of rows q [n][H][hd] over K, V [have + n][KVH][hd] with scales ks, vs [have + n][KVH]; half_eps:
     half a step of out's type."""
+    add = 128 if half_eps > 2.0 ** -20 else 0
     n, H, hd = q.shape
     G = H // K.shape[1]
     out, bound = np.zeros((n, H, hd)), np.zeros((n, H, hd))
@@ -121,12 +126,13 @@ def attend(q, K, V, vs, have, scale, half_eps):
             l = p.sum()
             out[i, h] = p @ vv[:L] / l
             A = p @ np.abs(vv[:L]) / l
-            ds = (scale * (np.abs(kk[:L]) @ np.abs(y))).max() * ((hd + 8) * 2.0 ** -24 + 2.0 ** -22)
+            S = scale * (np.abs(kk[:L]) @ np.abs(y) + add * ks[:L, h // G] * np.abs(y).sum())
+            ds = S.max() * ((hd + 8) * 2.0 ** -24 + 2.0 ** -22)
             w = np.maximum(vs[:L, h // G], 2.0 ** -100)
-            rel = np.expm1(2 * ds) + (L / 32 + 48) * 2.0 ** -23
+            rel, sums = np.expm1(2 * ds), (L / 32 + 48) * 2.0 ** -23
             if half_eps > 2.0 ** -20:
                 rel += 2.0 ** -11
             rel += L * 2.0 ** -126 * w.max() / w.min()
-            err = A * rel + L * 2.0 ** -39 * 127 * (p * w).max() / l
+            err = A * rel + (A + add * (p @ vs[:L, h // G]) / l) * sums + L * 2.0 ** -39 * 127 * (p * w).max() / l
             bound[i, h] = err + (np.abs(out[i, h]) + err) * half_eps
     return out, bound

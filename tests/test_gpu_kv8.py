@@ -102,8 +102,8 @@ class Both:
         for b, (h, a) in enumerate(zip(self.have, self.add)):
             if a:
                 K, V = (c.values(self.pool.tables[b], h + a) for c in self.ref[layer])
-                vs = self.ref[layer][1].scale_of(self.pool.tables[b], h + a)
-                want, bound = kv8_ref.attend(q[at:at + a], K, V, vs, h, scale or self.hd ** -0.5, HALF[dtype])
+                ks, vs = (c.scale_of(self.pool.tables[b], h + a) for c in self.ref[layer])
+                want, bound = kv8_ref.attend(q[at:at + a], K, V, ks, vs, h, scale or self.hd ** -0.5, HALF[dtype])
                 err = np.abs(got[at:at + a] - want)
                 assert (err <= bound).all(), (b, h, a, float((err / np.maximum(bound, 1e-300)).max()))
             at += a
