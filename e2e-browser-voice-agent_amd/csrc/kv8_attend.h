@@ -69,10 +69,13 @@ __device__ inline float2 kv8_receive(const float* p) {
 template <int HD>
 struct Kv8Codes {
   uint4 k[HD / 32], v[HD / 32];
-  __device__ void load(const uint8_t* page, int lane) {
+  __device__ void load_k(const uint8_t* page, int lane) {
     const uint4* p = (const uint4*)page + lane;
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) k[i] = p[i * 64];
+  }
+  __device__ void load_v(const uint8_t* page, int lane) {
+    const uint4* p = (const uint4*)page + lane;
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) v[i] = p[(HD / 32 + i) * 64];
   }
@@ -137,11 +140,7 @@ struct Kv8Rows {
     for (auto& x : o[t]) x = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // One page: its codes and scales, and the number of its positions that this lane's rows look at (masked: some
-  // lane's row does not look at all 32; faint: a V scale far below that of a page before).
-  __device__ __forceinline__ void page(const Kv8Codes<HD>& w, Kv8Scale sc, int quarter, bool masked, const int (&seen)[N],
-                                       bool faint) {
-    kv8_f4 s[N][2];
+  __device__ __forceinline__ void scores(const Kv8Codes<HD>& w, kv8_f4 (&s)[N][2]) const {
 #pragma unroll
     for (int t = 0; t < N; t++)
 #pragma unroll
@@ -165,35 +164,65 @@ struct Kv8Rows {
           }
         }
       }
-    kv8_h8 hi[N], lo[kTwo ? N : 1];
+  }
+
+  // Scores of positions that a row does not look at.  (ks of at least 2^-60, as 0 would make them NaN: it changes no
+  // exponent by more than 2^-25.)
+  __device__ __forceinline__ void mask(kv8_f4 (&s)[N][2], float (&ks)[N], int quarter, const int (&seen)[N]) const {
 #pragma unroll
     for (int t = 0; t < N; t++) {
-      float x[8];
-      const float ks = sc.k * c[t];
+      ks[t] = __builtin_fmaxf(ks[t], 0x1p-60f);
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[i] = s[t][i >> 2][i & 3];
-        if (masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t]) x[i] = -1e30f;
-      }
-      float most = x[0];
+      for (int i = 0; i < 8; i++)
+        if ((i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t]) s[t][i >> 2][i & 3] = -__builtin_inff();
+    }
+  }
+
+  // One page from its scores: the number of its positions that this lane's rows look at (masked: not all rows look at
+  // all 32); faint: its weights may be too small for fp16, so that its share of l is formed in fp32.
+  __device__ __forceinline__ void page(kv8_f4 (&s)[N][2], const Kv8Codes<HD>& w, Kv8Scale sc, int quarter, bool masked,
+                                       const int (&seen)[N], bool faint) {
+    float ks[N], most[N];
 #pragma unroll
-      for (int i = 1; i < 8; i++) most = __builtin_fmaxf(most, x[i]);
-      most = __builtin_fmaf(most, ks, sc.v);
+    for (int t = 0; t < N; t++) ks[t] = sc.k * c[t];
+    if (masked) mask(s, ks, quarter, seen);
+    bool move = false;
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+      most[t] = s[t][0][0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) most[t] = __builtin_fmaxf(most[t], s[t][i >> 2][i & 3]);
+      most[t] = __builtin_fmaf(most[t], ks[t], sc.v);
       // weights of up to 2^14, or 2^15.5 before m is moved again
-      if (__builtin_amdgcn_ballot_w64(most - (kTwo ? 14.0f : 15.5f) > m[t]) != 0) {
-        const float m2 = __builtin_fmaxf(kv8_max_quarters(most) - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
+      move = move || most[t] - (kTwo ? 14.0f : 15.5f) > m[t];
+    }
+    if (__builtin_amdgcn_ballot_w64(move) != 0)
+#pragma unroll
+      for (int t = 0; t < N; t++) {
+        const float m2 = __builtin_fmaxf(kv8_max_quarters(most[t]) - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
         m[t] = m2;
         l[t] *= f;
         if constexpr (!kTwo) sum[t] *= f;
 #pragma unroll
         for (auto& y : o[t]) y *= f;
       }
+    if (faint)
+#pragma unroll
+      for (int t = 0; t < N; t++) {
+        float all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) all += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], ks[t], sc.v - m[t]));
+        l[t] = __builtin_fmaf(kv8_sum_quarters(all), sc.iv, l[t]);
+      }
+    const float l_scale = faint ? 0.0f : sc.iv;
+    kv8_h8 hi[N], lo[kTwo ? N : 1];
+#pragma unroll
+    for (int t = 0; t < N; t++) {
       const float v = sc.v - m[t];
-      [[maybe_unused]] float all = 0.0f;
+      float all = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ks, v));
-        if (masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t]) e = 0.0f;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], ks[t], v));
         if constexpr (kTwo) {
           all += e;
           float y = e * sc.mant;
@@ -204,24 +233,13 @@ struct Kv8Rows {
           hi[t][i] = (_Float16)e;
         }
       }
-      if constexpr (kTwo) {
-        l[t] = __builtin_fmaf(all, sc.iv, l[t]);
-      } else {
+      if constexpr (!kTwo) {
         const kv8_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
         const kv8_f4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi[t], kv8_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        sum[t] += r[0];
         all = r[0];
-        sum[t] += all;
-        if (faint) {
-          all = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ks, v));
-            all += masked && (i >> 2) * 16 + quarter * 4 + (i & 3) >= seen[t] ? 0.0f : e;
-          }
-          all = kv8_sum_quarters(all);
-        }
-        l[t] = __builtin_fmaf(all, sc.iv, l[t]);
       }
+      l[t] = __builtin_fmaf(all, l_scale, l[t]);
     }
 #pragma unroll
     for (int p = 0; p < HD / 32; p++) {
@@ -251,8 +269,9 @@ struct Kv8Rows {
     }
   }
 
-  // Pages page0 + first, + step, ... (count of them) of a sequence's table, whose first row of this wave lies
-  // at position `from`; lane's row t looks at positions up to last[t].
+  // Pages first, first + step, ... (count of them) of a sequence's table, whose first row of this wave lies at
+  // position `from`; lane's row t looks at positions up to last[t].  A page's K is loaded when the scores of the page
+  // before are formed, its V when that page's are used up.
   __device__ __forceinline__ void run(const Kv8View& v, int layer, int g, const int* table, int first, int step, int count, int from,
                                       const int (&last)[N]) {
     const int lane = threadIdx.x & 63, quarter = lane >> 4;
@@ -273,21 +292,22 @@ struct Kv8Rows {
         return v.codes + b * page_bytes;
       };
       auto lane_of = [](float x, int j) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), j)); };
-      Kv8Codes<HD> buf[2];
-      buf[0].load(page_at(0), lane);
-      auto one = [&](int j, Kv8Codes<HD>& now, Kv8Codes<HD>& next) __attribute__((always_inline)) {
-        if (j + 1 < n) next.load(page_at(j + 1), lane);
-        const Kv8Scale s = {lane_of(sc.k, j), lane_of(sc.v, j), lane_of(sc.iv, j), kTwo ? lane_of(sc.mant, j) : 1.0f};
+      Kv8Codes<HD> w;
+      w.load_k(page_at(0), lane);
+      w.load_v(page_at(0), lane);
+      for (int j = 0; j < n; j++) {
+        const uint8_t* const next = page_at(min(j + 1, n - 1));
+        kv8_f4 s[N][2];
+        scores(w, s);
+        w.load_k(next, lane);
+        const Kv8Scale y = {lane_of(sc.k, j), lane_of(sc.v, j), lane_of(sc.iv, j), kTwo ? lane_of(sc.mant, j) : 1.0f};
         const int p0 = (first + step * (j0 + j)) * kKv8Block;
         int seen[N];
 #pragma unroll
         for (int t = 0; t < N; t++) seen[t] = last[t] + 1 - p0;
-        page(now, s, quarter, p0 + kKv8Block - 1 > from, seen, !kTwo && s.v < top - 12.0f);
-        top = __builtin_fmaxf(top, s.v);
-      };
-      for (int j = 0; j < n; j += 2) {
-        one(j, buf[0], buf[1]);
-        if (j + 1 < n) one(j + 1, buf[1], buf[0]);
+        page(s, w, y, quarter, p0 + kKv8Block - 1 > from, seen, !kTwo && y.v < top - 12.0f);
+        w.load_v(next, lane);
+        top = __builtin_fmaxf(top, y.v);
       }
     }
   }
