@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kItemsAim = 512;          // workgroups of attention that fill the GPU
 constexpr size_t kFillInPlan = 8192;
+constexpr int64_t kMostWorkgroups = 8192;   // of attention; a workgroup takes every so-manieth tile or item
 
 // The quotient x / s rounded to fp32, from r = 1 / s rounded: one correction of x * r by its residual gives it
 // (P. Markstein, IBM J. Res. Dev. 34(1), 1990) where the residual is exact, which |x / s| >= 1/4 and s >= 2^-100 make
@@ -427,15 +428,14 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
   const int64_t items = units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
-  const dim3 grid((unsigned)std::min<int64_t>(items, 8 * w.items_aim), (unsigned)(w.KVH * w.row_tiles));
-  const unsigned tiles = kv->rows > kKv8Few ? (unsigned)tiles_bound(w, kv->rows) * w.KVH : 0;
+  const bool few = kv->rows <= kKv8Few;        // no sequence is taken in tiles
+  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);
+  const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    if (tiles)
-      (w.HD == 64 ? k_kv8_prompt<64, T, 2> : k_kv8_prompt<128, T, 2>)<<<tiles, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride,
-                                                                                      out_stride, log2_scale, kv->rows);
-    if (w.HD == 64) k_kv8_attend<64, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
-    else k_kv8_attend<128, T><<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
+    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
+                          : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));

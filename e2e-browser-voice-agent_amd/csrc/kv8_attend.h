@@ -313,156 +313,194 @@ struct Kv8Rows {
   }
 };
 
-// Few rows.  A workgroup takes items of the plan, its four waves every fourth page each, and adds up their sums in shared
-// memory.  Of a unit in several parts, the workgroup that is done last adds up the parts, in their order.
-template <int HD, class T>
-__global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                    int64_t q_stride, int64_t out_stride, float scale, int rows) {
-  constexpr bool kTwo = sizeof(T) == 4;
-  constexpr int kLd = HD + 4;
-  __shared__ float so[4][16][kLd];
-  __shared__ float sm[4][16], sl[4][16];
-  __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
-  const int g = blockIdx.y / v.row_tiles, r0 = (blockIdx.y % v.row_tiles) * 16;
-  if (v.head->rows > rows) {                   // replayed on a larger plan than it was launched for
-    if (tid == 0) v.head->status = KV8_STALE;
-    return;
-  }
-  for (int i = blockIdx.x; i < v.head->items; i += gridDim.x) {
-    const Kv8Item it = v.items[i];
-    const int r = r0 + n, tok = r / G, h = r % G;
-    const bool valid = r < it.n * G;
-    Kv8Rows<HD, kTwo, 1> w;
-    w.init(0, q + (int64_t)(it.t + (valid ? tok : 0)) * q_stride + (g * G + (valid ? h : 0)) * HD, quarter, valid, scale);
-    const int row_last[1] = {it.pos + (valid ? tok : it.n - 1)};
-    w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
-    w.finish(0);
-    if (quarter == 0) { sm[wave][n] = w.m[0]; sl[wave][n] = w.l[0]; }
+// 4 columns of a row of the sums of `parts` parts at `slot`, `slot + step`, ...: o, l relative to 2^m.
+template <int HD>
+__device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int parts, int row, int d, kv8_f4& o, float& m, float& l) {
+  const float* const ml = (const float*)(v.part_ml + slot * 16 + row);
+  const float* const po = v.part_o + (slot * 16 + row) * HD + d;
+  m = kKv8Lowest;
+  l = 0.0f;
+  o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = 0; k0 < parts; k0 += 8) {         // 8 parts on their way at once
+    float2 a[8], x[8][2];
+    float m2 = m;
 #pragma unroll
-    for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&so[wave][n][d * 16 + quarter * 4] = w.o[0][d];
-    __syncthreads();
-    const size_t slot = (size_t)max(it.slot, 0) * gridDim.y + blockIdx.y;
-    auto write = [&](int row, int d, kv8_f4 o, float l) {
-      const int tk = (r0 + row) / G, hh = (r0 + row) % G;
-      if (r0 + row >= it.n * G) return;
-      T* p = out + (int64_t)(it.t + tk) * out_stride + (g * G + hh) * HD + d;
-      for (int k = 0; k < 4; k++) p[k] = (T)(l == 0.0f ? 0.0f : o[k] / l);
-    };
-    for (int e = tid; e < 4 * HD; e += 256) {
-      const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-      const float m = __builtin_fmaxf(__builtin_fmaxf(sm[0][row], sm[1][row]), __builtin_fmaxf(sm[2][row], sm[3][row]));
-      kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-      float l = 0.0f;
-      for (int k = 0; k < 4; k++) {
-        const float f = __builtin_amdgcn_exp2f(sm[k][row] - m);
-        l = __builtin_fmaf(sl[k][row], f, l);
-        const kv8_f4 x = *(const kv8_f4*)&so[k][row][d];
-        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
-      }
-      if (it.parts == 1) {
-        write(row, d, o, l);
-      } else {
-        const size_t s = slot + (size_t)it.part * gridDim.y;
-        if (r0 + row >= it.n * G) continue;
-        float* const p = v.part_o + (s * 16 + row) * HD + d;
-        kv8_send(p, o[0], o[1]);
-        kv8_send(p + 2, o[2], o[3]);
-        if (d == 0) kv8_send((float*)(v.part_ml + s * 16 + row), m, l);
-      }
+    for (int k = 0; k < 8; k++) {
+      const size_t at = (size_t)min(k0 + k, parts - 1) * step * 16;
+      a[k] = kv8_receive(ml + at * 2);
+      x[k][0] = kv8_receive(po + at * HD);
+      x[k][1] = kv8_receive(po + at * HD + 2);
     }
-    if (it.parts > 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the part has arrived in memory before it is counted
-      __syncthreads();
-      if (tid == 0) {
-        last = __hip_atomic_fetch_add(v.arrived + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.parts - 1;
-        if (last) __hip_atomic_store(v.arrived + slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
-      }
-      __syncthreads();
-      if (last) {
-        const size_t next = (size_t)gridDim.y * 16;          // from a part's rows to the next part's
-        for (int e = tid; e < 4 * HD; e += 256) {
-          const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-          if (r0 + row >= it.n * G) continue;
-          const float* const ml = (const float*)(v.part_ml + slot * 16 + row);
-          const float* const po = v.part_o + (slot * 16 + row) * HD + d;
-          float m = kKv8Lowest, l = 0.0f;
-          kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int k0 = 0; k0 < it.parts; k0 += 8) {         // 8 parts on their way at once
-            float2 a[8], x[8][2];
-            float m2 = m;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const size_t at = (size_t)min(k0 + k, it.parts - 1) * next;
-              a[k] = kv8_receive(ml + at * 2);
-              x[k][0] = kv8_receive(po + at * HD);
-              x[k][1] = kv8_receive(po + at * HD + 2);
-            }
+    for (int k = 0; k < 8; k++) m2 = __builtin_fmaxf(m2, a[k].x);
+    const float f0 = __builtin_amdgcn_exp2f(m - m2);
+    l *= f0;
+    o *= f0;
+    m = m2;
 #pragma unroll
-            for (int k = 0; k < 8; k++) m2 = __builtin_fmaxf(m2, a[k].x);
-            const float f0 = __builtin_amdgcn_exp2f(m - m2);
-            l *= f0;
-            o *= f0;
-            m = m2;
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const float f = k0 + k < it.parts ? __builtin_amdgcn_exp2f(a[k].x - m) : 0.0f;
-              l = __builtin_fmaf(a[k].y, f, l);
-              o[0] = __builtin_fmaf(x[k][0].x, f, o[0]);
-              o[1] = __builtin_fmaf(x[k][0].y, f, o[1]);
-              o[2] = __builtin_fmaf(x[k][1].x, f, o[2]);
-              o[3] = __builtin_fmaf(x[k][1].y, f, o[3]);
-            }
-          }
-          write(row, d, o, l);
-        }
-      }
+    for (int k = 0; k < 8; k++) {
+      const float f = k0 + k < parts ? __builtin_amdgcn_exp2f(a[k].x - m) : 0.0f;
+      l = __builtin_fmaf(a[k].y, f, l);
+      o[0] = __builtin_fmaf(x[k][0].x, f, o[0]);
+      o[1] = __builtin_fmaf(x[k][0].y, f, o[1]);
+      o[2] = __builtin_fmaf(x[k][1].x, f, o[2]);
+      o[3] = __builtin_fmaf(x[k][1].y, f, o[3]);
     }
-    __syncthreads();                           // the shared sums have been read
   }
 }
 
-// Many rows: a tile is 64 N neighbouring rows of a sequence and kv head (row r: position r / G of the step, head r % G), 16 N
-// of each wave, which passes over all the pages that they look at.  A tile's kv heads are neighbours in the grid,
-// so that the tiles of one meet on the same XCDs and find its pages in their L2.
+template <int HD>
+__device__ inline void kv8_send_part(const Kv8View& v, size_t slot, int row, int d, kv8_f4 o, float m, float l) {
+  float* const p = v.part_o + (slot * 16 + row) * HD + d;
+  kv8_send(p, o[0], o[1]);
+  kv8_send(p + 2, o[2], o[3]);
+  if (d == 0) kv8_send((float*)(v.part_ml + slot * 16 + row), m, l);
+}
+
+template <int HD>
+struct Kv8Shared {
+  float o[4][16][HD + 4];
+  float m[4][16], l[4][16];
+  int last;
+};
+
+// Whether this workgroup is the last of `count` to arrive at *counter, with what it sent in memory before.
+template <class S>
+__device__ inline bool kv8_last(S& sh, int* counter, int count) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sh.last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
+    if (sh.last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+  }
+  __syncthreads();
+  return sh.last != 0;
+}
+
+// Few rows: an item of the plan and 16 of its unit's rows of a kv head (y).  The four waves take every fourth page each
+// and add up their sums in shared memory.  A unit in several parts: the last workgroup of each 16 parts to be done adds
+// those up, and the last of these the sums of 16, always in the order of the parts.
+template <int HD, class T>
+__device__ __forceinline__ void kv8_item(const Kv8View& v, Kv8Shared<HD>& sh, int layer, const T* q, T* out, int64_t q_stride,
+                                         int64_t out_stride, float scale, int item, int y) {
+  constexpr bool kTwo = sizeof(T) == 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
+  const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * 16;
+  const Kv8Item it = v.items[item];
+  const int r = r0 + n, tok = r / G, h = r % G;
+  const bool valid = r < it.n * G;
+  Kv8Rows<HD, kTwo, 1> w;
+  w.init(0, q + (int64_t)(it.t + (valid ? tok : 0)) * q_stride + (g * G + (valid ? h : 0)) * HD, quarter, valid, scale);
+  const int row_last[1] = {it.pos + (valid ? tok : it.n - 1)};
+  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
+  w.finish(0);
+  if (quarter == 0) { sh.m[wave][n] = w.m[0]; sh.l[wave][n] = w.l[0]; }
+#pragma unroll
+  for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&sh.o[wave][n][d * 16 + quarter * 4] = w.o[0][d];
+  __syncthreads();
+  const int ys = v.KVH * v.row_tiles;
+  const size_t slot = (size_t)max(it.slot, 0) * ys + y;         // of the unit's first part
+  const int rows = min(16, it.n * G - r0);                      // of this tile
+  auto write = [&](int row, int d, kv8_f4 o, float l) {
+    T* p = out + (int64_t)(it.t + (r0 + row) / G) * out_stride + (g * G + (r0 + row) % G) * HD + d;
+    for (int k = 0; k < 4; k++) p[k] = (T)(l == 0.0f ? 0.0f : o[k] / l);
+  };
+  for (int e = tid; e < rows * (HD / 4); e += 256) {
+    const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+    const float m = __builtin_fmaxf(__builtin_fmaxf(sh.m[0][row], sh.m[1][row]), __builtin_fmaxf(sh.m[2][row], sh.m[3][row]));
+    kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int k = 0; k < 4; k++) {
+      const float f = __builtin_amdgcn_exp2f(sh.m[k][row] - m);
+      l = __builtin_fmaf(sh.l[k][row], f, l);
+      const kv8_f4 x = *(const kv8_f4*)&sh.o[k][row][d];
+      for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+    }
+    if (it.parts == 1) write(row, d, o, l);
+    else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, row, d, o, m, l);
+  }
+  if (it.parts > 1) {
+    const int first = it.part & ~15, mine = min(16, it.parts - first), sixteens = (it.parts + 15) >> 4;
+    const size_t own = slot + (size_t)first * ys;
+    if (kv8_last(sh, v.arrived + own, mine)) {
+      for (int e = tid; e < rows * (HD / 4); e += 256) {
+        const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+        kv8_f4 o;
+        float m, l;
+        kv8_join<HD>(v, own, ys, mine, row, d, o, m, l);
+        if (sixteens == 1) write(row, d, o, l);
+        else kv8_send_part<HD>(v, own, row, d, o, m, l);        // over the first part, which only these threads read
+      }
+      if (sixteens > 1 && kv8_last(sh, v.arrived + slot + ys, sixteens))      // counted at the second part
+        for (int e = tid; e < rows * (HD / 4); e += 256) {
+          const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+          kv8_f4 o;
+          float m, l;
+          kv8_join<HD>(v, slot, (size_t)16 * ys, sixteens, row, d, o, m, l);
+          write(row, d, o, l);
+        }
+    }
+  }
+  __syncthreads();                           // the shared sums have been read
+}
+
+// Many rows: 64 N neighbouring rows of a sequence and kv head (row r: position r / G of the step, head r % G), 16 N of each
+// wave, which passes over all the pages that they look at.
 template <int HD, class T, int N>
-__global__ __launch_bounds__(256) void k_kv8_prompt(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                    int64_t q_stride, int64_t out_stride, float scale, int rows) {
+__device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q, T* out, int64_t q_stride, int64_t out_stride, float scale,
+                                         int tile, int g) {
   constexpr bool kTwo = sizeof(T) == 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH, g = blockIdx.x % v.KVH;
-  if (v.head->rows > rows) {
+  const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
+  const Kv8Tile it = v.tiles[tile];
+  const int64_t r0 = (int64_t)it.tile * kKv8TileRows + wave * (16 * N), end = (int64_t)it.n * G;
+  if (r0 >= end) return;
+  Kv8Rows<HD, kTwo, N> w;
+  int last[N];
+#pragma unroll
+  for (int t = 0; t < N; t++) {
+    const int64_t r = min(r0 + t * 16 + n, end - 1);        // rows behind the end: as the last one, not written
+    const int tok = (int)(r / G), h = (int)(r % G);
+    last[t] = it.pos + tok;
+    w.init(t, q + (int64_t)(it.t + tok) * q_stride + (g * G + h) * HD, quarter, true, scale);
+  }
+  const int from = it.pos + (int)(r0 / G), to = it.pos + (int)((min(r0 + 16 * N, end) - 1) / G);
+  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, 0, 1, to / kKv8Block + 1, from, last);
+#pragma unroll
+  for (int t = 0; t < N; t++) {
+    w.finish(t);
+    const int64_t r = r0 + t * 16 + n;
+    if (r >= end) continue;
+    T* const p = out + (int64_t)(it.t + (int)(r / G)) * out_stride + (g * G + (int)(r % G)) * HD + quarter * 4;
+    const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t];
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) p[d * 16 + k] = (T)(w.o[t][d][k] * il);
+  }
+}
+
+// A step's tiles, the longest first, then its items.  The kv heads are neighbours in the grid, so that the tiles of one
+// meet on the same XCDs and find its pages in their L2.
+template <int HD, class T, int N>
+__global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
+                                                    int64_t q_stride, int64_t out_stride, float scale, int rows) {
+  __shared__ Kv8Shared<HD> sh;
+  const Kv8Head head = *v.head;
+  if (head.rows > rows) {                      // replayed on a larger plan than it was launched for
     if (threadIdx.x == 0) v.head->status = KV8_STALE;
     return;
   }
-  for (int i = blockIdx.x / v.KVH; i < v.head->tiles; i += gridDim.x / v.KVH) {
-    const Kv8Tile it = v.tiles[i];
-    const int64_t r0 = (int64_t)it.tile * kKv8TileRows + wave * (16 * N), end = (int64_t)it.n * G;
-    if (r0 >= end) continue;
-    Kv8Rows<HD, kTwo, N> w;
-    int last[N];
-#pragma unroll
-    for (int t = 0; t < N; t++) {
-      const int64_t r = min(r0 + t * 16 + n, end - 1);        // rows behind the end: as the last one, not written
-      const int tok = (int)(r / G), h = (int)(r % G);
-      last[t] = it.pos + tok;
-      w.init(t, q + (int64_t)(it.t + tok) * q_stride + (g * G + h) * HD, quarter, true, scale);
-    }
-    const int from = it.pos + (int)(r0 / G), to = it.pos + (int)((min(r0 + 16 * N, end) - 1) / G);
-    w.run(v, layer, g, v.table + (size_t)it.seq * v.W, 0, 1, to / kKv8Block + 1, from, last);
-#pragma unroll
-    for (int t = 0; t < N; t++) {
-      w.finish(t);
-      const int64_t r = r0 + t * 16 + n;
-      if (r >= end) continue;
-      T* const p = out + (int64_t)(it.t + (int)(r / G)) * out_stride + (g * G + (int)(r % G)) * HD + quarter * 4;
-      const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t];
-#pragma unroll
-      for (int d = 0; d < HD / 16; d++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) p[d * 16 + k] = (T)(w.o[t][d][k] * il);
-    }
+  const int ys = v.KVH * v.row_tiles, tiles = N ? head.tiles * v.KVH : 0, all = tiles + head.items * ys;
+  for (int i = blockIdx.x; i < all; i += gridDim.x) {
+    if constexpr (N > 0)
+      if (i < tiles) {
+        kv8_tile<HD, T, N>(v, layer, q, out, q_stride, out_stride, scale, i / v.KVH, i % v.KVH);
+        continue;
+      }
+    const int k = i - tiles;
+    kv8_item<HD, T>(v, sh, layer, q, out, q_stride, out_stride, scale, k / ys, k % ys);
   }
 }
 
