@@ -19,8 +19,9 @@ namespace q4 {
 constexpr int kKv8Block = 32;
 constexpr int kKv8MinPart = 16;               // pages of the smallest part of a unit
 constexpr int kKv8TileRows = 128;
-// Sequences that add more rows than kKv8Few are taken in tiles where these fill kKv8MinTiles workgroups.
-constexpr int kKv8Few = 16, kKv8MinTiles = 128;
+// Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
+// kKv8MinTiles workgroups.
+constexpr int kKv8MinTiles = 640;
 constexpr float kKv8MinScale = 0x1p-100f;     // a smaller scale is 0, and so are the values
 
 __host__ __device__ constexpr int kv8_k_byte(int HD, int t, int d) {
@@ -48,13 +49,14 @@ struct Kv8Run {
 };
 
 // Attention's work.  A unit is up to 16 / G neighbouring rows of a sequence (G query heads to a kv head; one row
-// where G > 16), so that they fill 16 rows of a matrix core; an item is one of the `parts` that share a unit's pages.
+// where G > 16), so that they fill 16 rows of a matrix core, or up to 32 / G of one that adds more than 16 / G; an
+// item is one of the `parts` that share a unit's pages.
 struct Kv8Item {
   int seq, t, n;         // sequence, first row, rows
   int pos;               // position of the first row
   int page0, pages;      // of the sequence's table
   int part, slot;        // slot: of the unit's first part in the workspace, -1 for a unit in one part
-  int parts, unused[3];
+  int parts, wide, unused[2];
 };
 
 // A tile: kKv8TileRows rows of attention (positions x G) of a sequence with many rows.
@@ -79,12 +81,13 @@ struct Kv8View {
   Kv8Run* runs;
   Kv8Item* items;
   Kv8Tile* tiles;
-  float* part_o;       // [slots][kv_heads * row tiles][16][HD] sums of a part, relative to 2^part_ml.x
-  float2* part_ml;     // [slots][kv_heads * row tiles][16] reference exponent, sum of the probabilities
+  float* part_o;       // [slots][kv_heads * row tiles][32][HD] sums of a part, relative to 2^part_ml.x
+  float2* part_ml;     // [slots][kv_heads * row tiles][32] reference exponent, sum of the probabilities
   int* arrived;        // [slots][kv_heads * row tiles] parts of a unit that are done (at its first slot)
   int layers, H, KVH, HD, B, W, pages, max_len;
-  int unit_rows;       // rows of a unit
-  int row_tiles;       // 16-row tiles of a unit
+  uint32_t g_magic;    // 2^32 / G rounded up (0 for G = 1): r / G = r * g_magic >> 32 while r * G < 2^32
+  int unit_rows, wide_rows;       // rows of a unit
+  int row_tiles;       // of a unit: 16 rows (32 of a wide one, which has no more of them)
   int items_aim;       // items that fill the GPU
 };
 

@@ -186,10 +186,15 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
 
 // At most so many tiles have `rows` rows: of full ones, and of a last one of each sequence.
 size_t tiles_bound(const Kv8View& v, int rows) {
-  return (size_t)((int64_t)rows * (v.H / v.KVH) / kKv8TileRows + std::min(v.B, rows / (kKv8Few + 1)) + 1);
+  return (size_t)((int64_t)rows * (v.H / v.KVH) / kKv8TileRows + std::min(v.B, rows / (v.unit_rows + 1)) + 1);
 }
 
 int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
+
+// Whether 16 bytes of any row can be loaded at once.
+bool aligned16(const void* p, int64_t stride, int type) {
+  return ((uintptr_t)p | (uintptr_t)(stride * elem_size(type))) % 16 == 0;
+}
 
 int check_layer(const q4hip_kv8* kv, int layer, int type) {
   if (layer < 0 || layer >= kv->v.layers) return fail(Q4HIP_EINVAL, "layer %d of %d", layer, kv->v.layers);
@@ -261,6 +266,7 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   if (heads % kv_heads) return fail(Q4HIP_EINVAL, "heads must be a multiple of kv_heads");
   if (head_dim != 64 && head_dim != 128) return fail(Q4HIP_EINVAL, "head_dim %d unsupported (64 or 128)", head_dim);
   if (heads > 65535 || layers > 65535) return fail(Q4HIP_EINVAL, "bad configuration");
+  if (heads / kv_heads > 1024) return fail(Q4HIP_EINVAL, "more than 1024 heads to a kv head");
   if (pages > INT32_MAX / kKv8Block) return fail(Q4HIP_EINVAL, "%d pages: at most %d", pages, INT32_MAX / kKv8Block);
   if (max_len > INT32_MAX - kKv8Block) return fail(Q4HIP_EINVAL, "sequences of %d positions", max_len);
   int ndev = 0;
@@ -275,7 +281,13 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   v.layers = layers; v.H = heads; v.KVH = kv_heads; v.HD = head_dim;
   v.B = seqs; v.W = (max_len + kKv8Block - 1) / kKv8Block; v.pages = pages; v.max_len = max_len;
   const int G = heads / kv_heads;
+  if ((int64_t)max_rows * G * G > UINT32_MAX) {
+    delete kv;
+    return fail(Q4HIP_EINVAL, "plans of %d rows with %d heads to a kv head: at most %u", max_rows, G, UINT32_MAX / (G * G));
+  }
+  v.g_magic = G == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + G - 1) / G);
   v.unit_rows = std::max(1, 16 / G);
+  v.wide_rows = std::max(1, 32 / G);
   v.row_tiles = (std::min(v.unit_rows, max_rows) * G + 15) / 16;
   v.items_aim = std::max(1, kItemsAim / (kv_heads * v.row_tiles));
   const size_t blocks = (size_t)layers * pages * kv_heads, bytes = blocks * 2 * kKv8Block * head_dim;
@@ -295,8 +307,8 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.tiles, tiles_bound(v, max_rows));
   // units in several parts: each has more pages than a part, so that they have at most twice the parts aimed at
   const size_t parts = (size_t)2 * v.items_aim * kv_heads * v.row_tiles;
-  al(&v.part_o, parts * 16 * head_dim);
-  al(&v.part_ml, parts * 16);
+  al(&v.part_o, parts * 32 * head_dim);
+  al(&v.part_ml, parts * 32);
   al(&v.arrived, parts);
   if (e == hipSuccess) e = hipHostMalloc((void**)&kv->pin, sizeof(Kv8Head), hipHostMallocDefault);
   if (e == hipSuccess) e = hipMemsetAsync(v.codes, 128, bytes, kv->stream);
@@ -374,8 +386,7 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   // runs of a sequence: its rows over 32, and two at its ends
   const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)w.KVH, 2);
-  const bool wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * elem_size(type)) |
-                       (uintptr_t)(v_stride * elem_size(type))) % 16);
+  const bool wide = aligned16(k, k_stride, type) && aligned16(v, v_stride, type);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
@@ -428,14 +439,15 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
   const int64_t items = units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
-  const bool few = kv->rows <= kKv8Few;        // no sequence is taken in tiles
+  const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
+  const bool few = kv->rows <= w.unit_rows;    // neither wide units nor tiles
   const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);
   const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
                           : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows, wide);
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));

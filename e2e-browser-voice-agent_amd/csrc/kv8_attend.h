@@ -65,6 +65,23 @@ __device__ inline float2 kv8_receive(const float* p) {
   return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
 }
 
+__device__ inline int kv8_div_g(const Kv8View& v, int r) { return v.g_magic ? (int)__umulhi((uint32_t)r, v.g_magic) : r; }
+
+// 4 neighbouring values of a row; wide: its 16 bytes can be stored at once.
+template <class T>
+__device__ __forceinline__ void kv8_put4(T* p, bool wide, const kv8_f4& x) {
+  union { uint64_t w[sizeof(T) / 2]; T y[4]; } u;
+#pragma unroll
+  for (int i = 0; i < 4; i++) u.y[i] = (T)x[i];
+  if (wide) {
+    if constexpr (sizeof(T) == 4) *(uint4*)p = *(const uint4*)&u;
+    else *(uint64_t*)p = u.w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = u.y[i];
+  }
+}
+
 // A page's codes in the registers of a wave.
 template <int HD>
 struct Kv8Codes {
@@ -105,16 +122,43 @@ struct Kv8Rows {
   kv8_f4 first[kTwo ? 1 : N];                     // what the 128 add to the scores, negative
   float m[N], l[N], c[N], sum[kTwo ? 1 : N];      // c: attention scale, log2 e and the power of two that q was divided by
 
+  // The rows at row[t]; wide: 16 bytes of a row can be loaded at once.  All loads before any use: they wait for one another
+  // otherwise.
   template <class T>
-  __device__ void init(int t, const T* row, int quarter, bool valid, float scale) {
-    float x[HD / 32][8], most = 0.0f;
+  __device__ __forceinline__ void init(const T* const (&row)[N], int quarter, bool wide, float scale) {
+    union Raw { uint4 w[sizeof(T) / 2]; T y[8]; } raw[N][HD / 32];
+    if (wide) {
+#pragma unroll
+      for (int t = 0; t < N; t++)
+#pragma unroll
+        for (int s = 0; s < HD / 32; s++)
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[t][s].w[i] = ((const uint4*)(row[t] + s * 32 + quarter * 8))[i];
+    } else {
+#pragma unroll
+      for (int t = 0; t < N; t++)
+#pragma unroll
+        for (int s = 0; s < HD / 32; s++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) raw[t][s].y[i] = row[t][s * 32 + quarter * 8 + i];
+    }
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+      float x[HD / 32][8];
+#pragma unroll
+      for (int s = 0; s < HD / 32; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[s][i] = (float)raw[t][s].y[i];
+      init_row(t, x, scale);
+    }
+  }
+
+  __device__ __forceinline__ void init_row(int t, const float (&x)[HD / 32][8], float scale) {
+    float most = 0.0f;
 #pragma unroll
     for (int s = 0; s < HD / 32; s++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[s][i] = valid ? (float)row[s * 32 + quarter * 8 + i] : 0.0f;
-        most = __builtin_fmaxf(most, __builtin_fabsf(x[s][i]));
-      }
+      for (int i = 0; i < 8; i++) most = __builtin_fmaxf(most, __builtin_fabsf(x[s][i]));
     most = kv8_max_quarters(most);
     const int e = 14 - __builtin_amdgcn_frexp_expf(most);      // the largest value becomes 2^13 .. 2^14
     float all = 0.0f;
@@ -149,21 +193,16 @@ struct Kv8Rows {
         else s[t][h] = first[t];
       }
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int p = 0; p < HD / 32; p++)       // the 2 N sums in turn, as each addition waits for the one before
 #pragma unroll
-      for (int p = 0; p < HD / 64; p++) {
-        const uint4 a = w.k[h * (HD / 64) + p];
-        const kv8_h8 a0 = kv8_halves<kTwo>(a.x, a.y), a1 = kv8_halves<kTwo>(a.z, a.w);
+      for (int part = 0; part < (kTwo ? 2 : 1); part++)
 #pragma unroll
-        for (int t = 0; t < N; t++) {
-          s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[t][0][2 * p], s[t][h], 0, 0, 0);
-          s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[t][0][2 * p + 1], s[t][h], 0, 0, 0);
-          if constexpr (kTwo) {
-            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[t][1][2 * p], s[t][h], 0, 0, 0);
-            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[t][1][2 * p + 1], s[t][h], 0, 0, 0);
-          }
+        for (int h = 0; h < 2; h++) {
+          const uint4 a = w.k[h * (HD / 64) + p / 2];
+          const kv8_h8 x = p % 2 ? kv8_halves<kTwo>(a.z, a.w) : kv8_halves<kTwo>(a.x, a.y);
+#pragma unroll
+          for (int t = 0; t < N; t++) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[t][part][p], s[t][h], 0, 0, 0);
         }
-      }
   }
 
   // Scores of positions that a row does not look at.  (ks of at least 2^-60, as 0 would make them NaN: it changes no
@@ -316,8 +355,8 @@ struct Kv8Rows {
 // 4 columns of a row of the sums of `parts` parts at `slot`, `slot + step`, ...: o, l relative to 2^m.
 template <int HD>
 __device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int parts, int row, int d, kv8_f4& o, float& m, float& l) {
-  const float* const ml = (const float*)(v.part_ml + slot * 16 + row);
-  const float* const po = v.part_o + (slot * 16 + row) * HD + d;
+  const float* const ml = (const float*)(v.part_ml + slot * 32 + row);
+  const float* const po = v.part_o + (slot * 32 + row) * HD + d;
   m = kKv8Lowest;
   l = 0.0f;
   o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -326,7 +365,7 @@ __device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int 
     float m2 = m;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      const size_t at = (size_t)min(k0 + k, parts - 1) * step * 16;
+      const size_t at = (size_t)min(k0 + k, parts - 1) * step * 32;
       a[k] = kv8_receive(ml + at * 2);
       x[k][0] = kv8_receive(po + at * HD);
       x[k][1] = kv8_receive(po + at * HD + 2);
@@ -351,10 +390,10 @@ __device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int 
 
 template <int HD>
 __device__ inline void kv8_send_part(const Kv8View& v, size_t slot, int row, int d, kv8_f4 o, float m, float l) {
-  float* const p = v.part_o + (slot * 16 + row) * HD + d;
+  float* const p = v.part_o + (slot * 32 + row) * HD + d;
   kv8_send(p, o[0], o[1]);
   kv8_send(p + 2, o[2], o[3]);
-  if (d == 0) kv8_send((float*)(v.part_ml + slot * 16 + row), m, l);
+  if (d == 0) kv8_send((float*)(v.part_ml + slot * 32 + row), m, l);
 }
 
 template <int HD>
@@ -377,48 +416,58 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
   return sh.last != 0;
 }
 
-// Few rows: an item of the plan and 16 of its unit's rows of a kv head (y).  The four waves take every fourth page each
-// and add up their sums in shared memory.  A unit in several parts: the last workgroup of each 16 parts to be done adds
-// those up, and the last of these the sums of 16, always in the order of the parts.
-template <int HD, class T>
-__device__ __forceinline__ void kv8_item(const Kv8View& v, Kv8Shared<HD>& sh, int layer, const T* q, T* out, int64_t q_stride,
-                                         int64_t out_stride, float scale, int item, int y) {
+// An item of the plan and 16 N of its unit's rows of a kv head (y).  The four waves take every fourth page each and
+// add up their sums in shared memory, 16 rows at a time.  A unit in several parts: the last workgroup of each 16 parts to be
+// done adds those up, and the last of these the sums of 16, always in the order of the parts.
+template <int HD, class T, int N>
+__device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,
+                                         int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {
   constexpr bool kTwo = sizeof(T) == 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
-  const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * 16;
-  const Kv8Item it = v.items[item];
-  const int r = r0 + n, tok = r / G, h = r % G;
-  const bool valid = r < it.n * G;
-  Kv8Rows<HD, kTwo, 1> w;
-  w.init(0, q + (int64_t)(it.t + (valid ? tok : 0)) * q_stride + (g * G + (valid ? h : 0)) * HD, quarter, valid, scale);
-  const int row_last[1] = {it.pos + (valid ? tok : it.n - 1)};
-  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
-  w.finish(0);
-  if (quarter == 0) { sh.m[wave][n] = w.m[0]; sh.l[wave][n] = w.l[0]; }
+  const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * (16 * N);
+  const int rows = min(16 * N, it.n * G - r0);                  // of this tile
+  if (rows <= 0) return;
+  Kv8Rows<HD, kTwo, N> w;
+  int row_last[N];
+  const T* row[N];
 #pragma unroll
-  for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&sh.o[wave][n][d * 16 + quarter * 4] = w.o[0][d];
-  __syncthreads();
+  for (int t = 0; t < N; t++) {
+    const int r = r0 + min(t * 16 + n, rows - 1), tok = kv8_div_g(v, r);      // rows behind the end: as the last one, not written
+    row[t] = q + (int64_t)(it.t + tok) * q_stride + (g * G + r - tok * G) * HD;
+    row_last[t] = it.pos + tok;
+  }
+  w.init(row, quarter, wide, scale);
+  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
   const int ys = v.KVH * v.row_tiles;
   const size_t slot = (size_t)max(it.slot, 0) * ys + y;         // of the unit's first part
-  const int rows = min(16, it.n * G - r0);                      // of this tile
   auto write = [&](int row, int d, kv8_f4 o, float l) {
-    T* p = out + (int64_t)(it.t + (r0 + row) / G) * out_stride + (g * G + (r0 + row) % G) * HD + d;
-    for (int k = 0; k < 4; k++) p[k] = (T)(l == 0.0f ? 0.0f : o[k] / l);
+    const int r = r0 + row, tok = kv8_div_g(v, r);
+    o *= l == 0.0f ? 0.0f : 1.0f / l;
+    kv8_put4(out + (int64_t)(it.t + tok) * out_stride + (g * G + r - tok * G) * HD + d, wide, o);
   };
-  for (int e = tid; e < rows * (HD / 4); e += 256) {
-    const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-    const float m = __builtin_fmaxf(__builtin_fmaxf(sh.m[0][row], sh.m[1][row]), __builtin_fmaxf(sh.m[2][row], sh.m[3][row]));
-    kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (int k = 0; k < 4; k++) {
-      const float f = __builtin_amdgcn_exp2f(sh.m[k][row] - m);
-      l = __builtin_fmaf(sh.l[k][row], f, l);
-      const kv8_f4 x = *(const kv8_f4*)&sh.o[k][row][d];
-      for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+#pragma unroll
+  for (int t = 0; t < N; t++) {
+    w.finish(t);
+    __syncthreads();                         // the shared sums before have been read
+    if (quarter == 0) { sh.m[wave][n] = w.m[t]; sh.l[wave][n] = w.l[t]; }
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&sh.o[wave][n][d * 16 + quarter * 4] = w.o[t][d];
+    __syncthreads();
+    for (int e = tid; e < min(16, rows - t * 16) * (HD / 4); e += 256) {
+      const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+      const float m = __builtin_fmaxf(__builtin_fmaxf(sh.m[0][row], sh.m[1][row]), __builtin_fmaxf(sh.m[2][row], sh.m[3][row]));
+      kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      float l = 0.0f;
+      for (int k = 0; k < 4; k++) {
+        const float f = __builtin_amdgcn_exp2f(sh.m[k][row] - m);
+        l = __builtin_fmaf(sh.l[k][row], f, l);
+        const kv8_f4 x = *(const kv8_f4*)&sh.o[k][row][d];
+        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+      }
+      if (it.parts == 1) write(t * 16 + row, d, o, l);
+      else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, m, l);
     }
-    if (it.parts == 1) write(row, d, o, l);
-    else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, row, d, o, m, l);
   }
   if (it.parts > 1) {
     const int first = it.part & ~15, mine = min(16, it.parts - first), sixteens = (it.parts + 15) >> 4;
@@ -430,7 +479,7 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, Kv8Shared<HD>& sh, in
         float m, l;
         kv8_join<HD>(v, own, ys, mine, row, d, o, m, l);
         if (sixteens == 1) write(row, d, o, l);
-        else kv8_send_part<HD>(v, own, row, d, o, m, l);        // over the first part, which only these threads read
+        else kv8_send_part<HD>(v, own, row, d, o, m, l);        // over the first part: a row's threads are of one wave
       }
       if (sixteens > 1 && kv8_last(sh, v.arrived + slot + ys, sixteens))      // counted at the second part
         for (int e = tid; e < rows * (HD / 4); e += 256) {
@@ -442,50 +491,48 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, Kv8Shared<HD>& sh, in
         }
     }
   }
-  __syncthreads();                           // the shared sums have been read
 }
 
 // Many rows: 64 N neighbouring rows of a sequence and kv head (row r: position r / G of the step, head r % G), 16 N of each
 // wave, which passes over all the pages that they look at.
 template <int HD, class T, int N>
-__device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q, T* out, int64_t q_stride, int64_t out_stride, float scale,
-                                         int tile, int g) {
+__device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q, T* out, int64_t q_stride, int64_t out_stride,
+                                         float scale, bool wide, int tile, int g) {
   constexpr bool kTwo = sizeof(T) == 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const Kv8Tile it = v.tiles[tile];
-  const int64_t r0 = (int64_t)it.tile * kKv8TileRows + wave * (16 * N), end = (int64_t)it.n * G;
+  const int r0 = it.tile * kKv8TileRows + wave * (16 * N), end = it.n * G;
   if (r0 >= end) return;
   Kv8Rows<HD, kTwo, N> w;
   int last[N];
+  const T* row[N];
 #pragma unroll
   for (int t = 0; t < N; t++) {
-    const int64_t r = min(r0 + t * 16 + n, end - 1);        // rows behind the end: as the last one, not written
-    const int tok = (int)(r / G), h = (int)(r % G);
+    const int r = min(r0 + t * 16 + n, end - 1), tok = kv8_div_g(v, r);      // rows behind the end: as the last one, not written
     last[t] = it.pos + tok;
-    w.init(t, q + (int64_t)(it.t + tok) * q_stride + (g * G + h) * HD, quarter, true, scale);
+    row[t] = q + (int64_t)(it.t + tok) * q_stride + (g * G + r - tok * G) * HD;
   }
-  const int from = it.pos + (int)(r0 / G), to = it.pos + (int)((min(r0 + 16 * N, end) - 1) / G);
+  w.init(row, quarter, wide, scale);
+  const int from = it.pos + kv8_div_g(v, r0), to = it.pos + kv8_div_g(v, min(r0 + 16 * N, end) - 1);
   w.run(v, layer, g, v.table + (size_t)it.seq * v.W, 0, 1, to / kKv8Block + 1, from, last);
 #pragma unroll
   for (int t = 0; t < N; t++) {
     w.finish(t);
-    const int64_t r = r0 + t * 16 + n;
+    const int r = r0 + t * 16 + n, tok = kv8_div_g(v, r);
     if (r >= end) continue;
-    T* const p = out + (int64_t)(it.t + (int)(r / G)) * out_stride + (g * G + (int)(r % G)) * HD + quarter * 4;
+    T* const p = out + (int64_t)(it.t + tok) * out_stride + (g * G + r - tok * G) * HD + quarter * 4;
     const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t];
 #pragma unroll
-    for (int d = 0; d < HD / 16; d++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) p[d * 16 + k] = (T)(w.o[t][d][k] * il);
+    for (int d = 0; d < HD / 16; d++) kv8_put4(p + d * 16, wide, w.o[t][d] * il);
   }
 }
 
 // A step's tiles, the longest first, then its items.  The kv heads are neighbours in the grid, so that the tiles of one
 // meet on the same XCDs and find its pages in their L2.
 template <int HD, class T, int N>
-__global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                    int64_t q_stride, int64_t out_stride, float scale, int rows) {
+__global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
+                                                    int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide) {
   __shared__ Kv8Shared<HD> sh;
   const Kv8Head head = *v.head;
   if (head.rows > rows) {                      // replayed on a larger plan than it was launched for
@@ -496,11 +543,17 @@ __global__ __launch_bounds__(256) void k_kv8_attend(Kv8View v, int layer, const 
   for (int i = blockIdx.x; i < all; i += gridDim.x) {
     if constexpr (N > 0)
       if (i < tiles) {
-        kv8_tile<HD, T, N>(v, layer, q, out, q_stride, out_stride, scale, i / v.KVH, i % v.KVH);
+        kv8_tile<HD, T, N>(v, layer, q, out, q_stride, out_stride, scale, wide, i / v.KVH, i % v.KVH);
         continue;
       }
-    const int k = i - tiles;
-    kv8_item<HD, T>(v, sh, layer, q, out, q_stride, out_stride, scale, k / ys, k % ys);
+    const int k = i - tiles, y = k % ys;
+    const Kv8Item it = v.items[k / ys];
+    if constexpr (N > 0)
+      if (it.wide) {
+        kv8_item<HD, T, N>(v, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+        continue;
+      }
+    kv8_item<HD, T, 1>(v, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
   }
 }
 

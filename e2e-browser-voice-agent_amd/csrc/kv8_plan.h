@@ -52,10 +52,14 @@ __device__ inline int find(const int* at, int B, int i) {
   return lo;
 }
 
-// Units of `add` rows, and the parts of each.
-__device__ inline int kv8_units(const Kv8View& v, int add) { return (add + v.unit_rows - 1) / v.unit_rows; }
+// Rows of the units of a sequence that adds `add` rows, units, tiles, and the parts of a unit.
+__device__ inline int kv8_unit_rows(const Kv8View& v, int add) { return add > v.unit_rows ? v.wide_rows : v.unit_rows; }
+__device__ inline int kv8_units(const Kv8View& v, int add) {
+  const int r = kv8_unit_rows(v, add);
+  return (add + r - 1) / r;
+}
 __device__ inline int kv8_tiles(const Kv8View& v, int add) {
-  return add > kKv8Few ? (int)(((int64_t)add * (v.H / v.KVH) + kKv8TileRows - 1) / kKv8TileRows) : 0;
+  return add > v.unit_rows ? (int)(((int64_t)add * (v.H / v.KVH) + kKv8TileRows - 1) / kKv8TileRows) : 0;
 }
 __device__ inline int kv8_parts(int pages, int parts_of) { return (pages + parts_of - 1) / parts_of; }
 
@@ -85,12 +89,13 @@ __device__ __forceinline__ void kv8_fill(const Kv8View& v, const Kv8Sums& s, con
   for (int i = first; i < h.items; i += stride) {
     const int b = find(s.item_at, v.B, i), have = s.base[b], add = s.lens[b] - have;
     const int parts = kv8_parts(kv8_pages(s.lens[b]), h.parts_of), k = i - s.item_at[b];
-    const int unit = parts == 1 ? k : k / parts, part = k - unit * parts;
+    const int unit = parts == 1 ? k : k / parts, part = k - unit * parts, rows = kv8_unit_rows(v, add);
     Kv8Item e{};
     e.seq = b;
-    e.t = s.starts[b] + unit * v.unit_rows;
-    e.n = min(v.unit_rows, add - unit * v.unit_rows);
-    e.pos = have + unit * v.unit_rows;
+    e.t = s.starts[b] + unit * rows;
+    e.n = min(rows, add - unit * rows);
+    e.pos = have + unit * rows;
+    e.wide = add > v.unit_rows;
     const int pages = kv8_pages(e.pos + e.n), each = parts == 1 ? pages : (pages + parts - 1) / parts;
     e.page0 = min(part * each, pages);
     e.pages = min(each, pages - e.page0);
@@ -126,7 +131,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   Kv8Sums s = kv8_sums(v);
   if constexpr (kShared) s = {store[0], store[1], store[2], store[3], store[4], store[5], store[6], store[7], store[8], store[9]};
   Kv8Head head = *v.head;
-  unsigned long long x_sum[5] = {};            // rows, pages, pages of all units and of those outside tiles, tiles
+  unsigned long long x_sum[5] = {};            // rows, pages, pages of all units and of those outside tiles, tiles and
+                                               // units outside
   int worst = KV8_OK, mine[3] = {};
   for (int b = tid; b < v.B; b += threads) {
     const int h = have[b], a = add[b], had = kShared ? v.held[b] : 0;
@@ -138,8 +144,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
       x_sum[0] += a;
       x_sum[1] += need;
       x_sum[2] += w;
-      x_sum[3] += a > kKv8Few ? 0 : w;
-      x_sum[4] += kv8_tiles(v, a);
+      x_sum[3] += a > v.unit_rows ? 0 : w;
+      x_sum[4] += a > v.unit_rows ? kv8_tiles(v, a) : a > 0;
     }
     if constexpr (kShared) { mine[0] = h; mine[1] = a; mine[2] = had; }
   }
