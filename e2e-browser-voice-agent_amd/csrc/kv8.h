@@ -17,7 +17,9 @@
 namespace q4 {
 
 constexpr int kKv8Block = 32;
-constexpr int kKv8MinPart = 16;               // pages of the smallest part of a unit
+// A unit of more than kKv8Whole pages is shared among several workgroups, in parts of at least kKv8MinPart pages and, while
+// that leaves no more than kKv8MoreItems times the items aimed at, at most kKv8MaxPart.
+constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups.

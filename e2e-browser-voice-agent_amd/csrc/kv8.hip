@@ -12,7 +12,7 @@
 namespace q4 {
 namespace {
 
-constexpr int kItemsAim = 512;          // workgroups of attention that fill the GPU
+constexpr int kItemsAim = 256;          // workgroups of attention: one for each CU
 constexpr size_t kFillInPlan = 8192;
 constexpr int64_t kMostWorkgroups = 8192;   // of attention; a workgroup takes every so-manieth tile or item
 
@@ -303,10 +303,11 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.lens, seqs);
   for (int** p : {&v.starts, &v.free_at, &v.take_at, &v.run_at, &v.item_at, &v.part_at, &v.tile_at}) al(p, (size_t)seqs + 1);
   al(&v.runs, max_rows);
-  al(&v.items, (size_t)max_rows + v.items_aim);
+  const size_t most_items = (size_t)kKv8MoreItems * v.items_aim;      // beyond one for each unit
+  al(&v.items, max_rows + most_items);
   al(&v.tiles, tiles_bound(v, max_rows));
-  // units in several parts: each has more pages than a part, so that they have at most twice the parts aimed at
-  const size_t parts = (size_t)2 * v.items_aim * kv_heads * v.row_tiles;
+  // units in several parts: each has more pages than a part, so that the last one's part at most doubles them
+  const size_t parts = 2 * most_items * kv_heads * v.row_tiles;
   al(&v.part_o, parts * 32 * head_dim);
   al(&v.part_ml, parts * 32);
   al(&v.arrived, parts);
@@ -346,7 +347,7 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   kv->rows = rows;
   // what the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds
-  const size_t entries = std::max<size_t>(rows + std::min<size_t>(v.items_aim, rows ? (size_t)v.pages * rows : 0),
+  const size_t entries = std::max<size_t>(rows + std::min<size_t>(kKv8MoreItems * v.items_aim, rows ? (size_t)v.pages * rows / kKv8MinPart : 0),
                                           tables ? (size_t)v.B * v.W : 0);
   const bool fill = entries <= kFillInPlan;
   if (v.B <= kPlanShared) {
@@ -438,7 +439,7 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
-  const int64_t items = units + std::min<int64_t>(w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
+  const int64_t items = units + std::min<int64_t>(kKv8MoreItems * w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
   const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
   const bool few = kv->rows <= w.unit_rows;    // neither wide units nor tiles
   const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);

@@ -61,7 +61,7 @@ __device__ inline int kv8_units(const Kv8View& v, int add) {
 __device__ inline int kv8_tiles(const Kv8View& v, int add) {
   return add > v.unit_rows ? (int)(((int64_t)add * (v.H / v.KVH) + kKv8TileRows - 1) / kKv8TileRows) : 0;
 }
-__device__ inline int kv8_parts(int pages, int parts_of) { return (pages + parts_of - 1) / parts_of; }
+__device__ inline int kv8_parts(int pages, int parts_of) { return pages <= kKv8Whole ? 1 : (pages + parts_of - 1) / parts_of; }
 
 // What is known of the sequences, in shared or global memory: [B] positions before and after the step and pages
 // held so far; sums over the sequences before.
@@ -187,7 +187,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   const bool in_tiles = tiles * v.KVH >= kKv8MinTiles;
   if (in_tiles) work = work_few;
   const unsigned long long share = work + v.items_aim - 1;
-  head.parts_of = max(kKv8MinPart, share < 0x100000000ull ? (int)((uint32_t)share / (uint32_t)v.items_aim) : (int)(share / v.items_aim));
+  const int each = share < 0x100000000ull ? (int)((uint32_t)share / (uint32_t)v.items_aim) : (int)(share / v.items_aim);
+  head.parts_of = max(max(kKv8MinPart, (each + kKv8MoreItems - 1) / kKv8MoreItems), min(each, kKv8MaxPart));
   int sum[7] = {};
   for (int b0 = 0; b0 < v.B; b0 += threads) {
     const int b = b0 + tid;
