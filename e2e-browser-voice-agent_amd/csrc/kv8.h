@@ -102,3 +102,17 @@ struct q4hip_kv8 {
   hipStream_t stream = nullptr;
   q4::Kv8Head* pin = nullptr;  // pinned copy of v.head
 };
+
+namespace q4 {
+
+// The operators' launches without the checks of their arguments (include/q4hip.h); q and out, k and v of `type`.
+void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
+                     int* tables);
+// heads [g0, g0 + heads) of the cache from heads 0.. of the rows
+void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
+                       int64_t v_stride, int g0, int heads);
+void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
+                       int64_t out_stride, float scale);
+void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v);
+
+}  // namespace q4

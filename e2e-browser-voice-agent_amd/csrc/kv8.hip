@@ -43,11 +43,11 @@ __device__ int doublings(float s, float t) {
 // kWide: rows whose 16 bytes can be loaded at once.
 template <int HD, class T, bool kWide>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
-                                                    int64_t k_stride, int64_t v_stride, int rows) {
+                                                    int64_t k_stride, int64_t v_stride, int rows, int g0) {
   __shared__ float tile[kKv8Block][HD + 1];
   __shared__ float most[4];
   __shared__ int odd;                          // a value that is not finite
-  const int g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int g = g0 + blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const bool is_v = blockIdx.z != 0;
   if (v.head->rows > rows) {                   // replayed on a larger plan than it was launched for
     if (tid == 0) v.head->status = KV8_STALE;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const 
   const Kv8Run run = v.runs[blockIdx.x];
   const int m = run.m, f = run.slot % kKv8Block;
   const int64_t ld = is_v ? v_stride : k_stride;
-  const T* x = (is_v ? val : k) + (int64_t)run.t * ld + g * HD;
+  const T* x = (is_v ? val : k) + (int64_t)run.t * ld + (int)blockIdx.y * HD;
   const size_t block = ((size_t)layer * v.pages + run.slot / kKv8Block) * v.KVH + g;
   float* const scale = (float*)(v.scales + block) + (is_v ? 1 : 0);
   uint4* const codes = (uint4*)(v.codes + (block * 2 + (is_v ? 1 : 0)) * (kKv8Block * HD));
@@ -238,6 +238,67 @@ void by_type(int type, F f) {
 }
 
 }  // namespace
+
+void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
+                     int* tables) {
+  const Kv8View& v = kv->v;
+  kv->rows = rows;
+  // what the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds
+  const size_t items = rows + std::min<size_t>(kKv8MoreItems * v.items_aim, rows ? (size_t)v.pages * rows / kKv8MinPart : 0);
+  const size_t entries = std::max<size_t>(items, tables ? (size_t)v.B * v.W : 0);
+  const bool fill = entries <= kFillInPlan;
+  if (v.B <= kPlanShared) {
+    const int threads = v.B <= 256 && entries <= 2048 ? 256 : kPlanThreads;
+    k_kv8_plan<true><<<1, threads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  } else {
+    k_kv8_plan<false><<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
+  }
+  if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
+}
+
+void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
+                       int64_t v_stride, int g0, int heads) {
+  const Kv8View& w = kv->v;
+  if (!kv->rows) return;
+  // runs of a sequence: its rows over 32, and two at its ends
+  const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)heads, 2);
+  const bool wide = aligned16(k, k_stride, type) && aligned16(v, v_stride, type);
+  by_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
+                          : (wide ? k_kv8_append<128, T, true> : k_kv8_append<128, T, false>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0);
+  });
+}
+
+void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
+                       int64_t out_stride, float scale) {
+  const Kv8View& w = kv->v;
+  if (!kv->rows) return;
+  // the softmax's exponentials are powers of two
+  const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
+  const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
+  const int64_t items = units + std::min<int64_t>(kKv8MoreItems * w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
+  const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
+  const bool few = kv->rows <= w.unit_rows;    // neither wide units nor tiles
+  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);
+  const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
+  by_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
+                          : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows, wide);
+  });
+}
+
+void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v) {
+  const Kv8View& w = kv->v;
+  const int per = 1024 / w.HD;                 // rows of a workgroup
+  const dim3 grid((unsigned)std::min((n + per - 1) / per, 16384), (unsigned)w.KVH);
+  if (w.HD == 64) k_kv8_read<64><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  else k_kv8_read<128><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+}
+
 }  // namespace q4
 
 using namespace q4;
@@ -345,18 +406,7 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
       if (rc) return rc;
     }
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  kv->rows = rows;
-  // what the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds
-  const size_t entries = std::max<size_t>(rows + std::min<size_t>(kKv8MoreItems * v.items_aim, rows ? (size_t)v.pages * rows / kKv8MinPart : 0),
-                                          tables ? (size_t)v.B * v.W : 0);
-  const bool fill = entries <= kFillInPlan;
-  if (v.B <= kPlanShared) {
-    const int threads = v.B <= 256 && entries <= 2048 ? 256 : kPlanThreads;
-    k_kv8_plan<true><<<1, threads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
-  } else {
-    k_kv8_plan<false><<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
-  }
-  if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
+  kv8_launch_plan(kv, s, have, add, rows, starts, positions, slots, tables);
   HIPCHK(hipGetLastError());
   if (stream) return Q4HIP_OK;
   const int rc = read_head(kv, s);
@@ -385,15 +435,7 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   if (!rc) rc = check_rows(kv, v, kv->rows, w.KVH * w.HD, v_stride, type, "v");
   if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  // runs of a sequence: its rows over 32, and two at its ends
-  const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)w.KVH, 2);
-  const bool wide = aligned16(k, k_stride, type) && aligned16(v, v_stride, type);
-  by_type(type, [&](auto zero) {
-    using T = decltype(zero);
-    auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
-                          : (wide ? k_kv8_append<128, T, true> : k_kv8_append<128, T, false>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows);
-  });
+  kv8_launch_append(kv, s, layer, k, v, type, k_stride, v_stride, 0, w.KVH);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;
@@ -414,10 +456,7 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
   if (!rc) rc = check_rows(kv, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
   if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  const int per = 1024 / w.HD;                 // rows of a workgroup
-  const dim3 grid((unsigned)std::min((n + per - 1) / per, 16384), (unsigned)w.KVH);
-  if (w.HD == 64) k_kv8_read<64><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
-  else k_kv8_read<128><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
+  kv8_launch_read(kv, s, layer, seq, pos, n, k, v);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;
@@ -435,21 +474,8 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   rc = check_rows(kv, q, kv->rows, w.H * w.HD, q_stride, type, "q");
   if (!rc) rc = check_rows(kv, out, kv->rows, w.H * w.HD, out_stride, type, "out");
   if (rc) return rc;
-  // the softmax's exponentials are powers of two
-  const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
-  const int64_t items = units + std::min<int64_t>(kKv8MoreItems * w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
-  const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
-  const bool few = kv->rows <= w.unit_rows;    // neither wide units nor tiles
-  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);
-  const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
-  by_type(type, [&](auto zero) {
-    using T = decltype(zero);
-    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
-                          : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows, wide);
-  });
+  kv8_launch_attend(kv, s, layer, q, out, type, q_stride, out_stride, scale);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;

@@ -23,6 +23,7 @@
 #include "gemm_tile.h"
 #include "host.h"
 #include "kernels.h"
+#include "kv8.h"
 #include "persistent.h"
 #include "q4hip.h"
 #include "route.h"
@@ -1157,6 +1158,16 @@ __global__ void k_rope_kv_list(float* __restrict__ qkv, int QKV, int D, int H, i
     vc[off + i] = (KT)vs[i];
     vc[off + i + half] = (KT)vs[i + half];
   }
+}
+
+// RoPE of token m's q and k heads at position pos[m], in place (kernels.c:337-345).  Grid (H + KVH, M), HD/2 threads.
+__global__ void k_rope_rows(float* __restrict__ qkv, int QKV, int HD, const float* __restrict__ rope, const int* __restrict__ pos) {
+  const int m = blockIdx.y, i = threadIdx.x, half = HD / 2;
+  float* v = qkv + (size_t)m * QKV + blockIdx.x * HD;
+  const float* cs = rope + (size_t)pos[m] * HD;
+  const float c = cs[2 * i], s = cs[2 * i + 1], x0 = v[i], x1 = v[i + half];
+  v[i] = x0 * c - x1 * s;
+  v[i + half] = x1 * c + x0 * s;
 }
 
 // Attention of token b over positions [0, pos[b]] of sequence b's cache (kernels.c:355-377), in
@@ -2538,6 +2549,18 @@ bool attn_list_ok(int H, int KVH, int HD, int ctx) {
   return true;
 }
 
+// The logits of the last of a pass's M tokens and the greedy next one.
+void enqueue_next(q4hip* h, int M) {
+  hipStream_t s = h->stream;
+  prof_mark(h, Q4HIP_PROF_NORM_Q);
+  launch_quant<QM_NORM>(s, 1, h->x, h->D, h->D, h->out_norm, h->eps, h->xq, h->xstride, M - 1);
+  prof_mark(h, Q4HIP_PROF_OUT);
+  launch_head(s, h->head, h->xq, h->logits);
+  prof_mark(h, Q4HIP_PROF_SAMPLE);
+  k_argmax1<<<h->am_parts, 256, 0, s>>>(h->logits, h->V, h->am_v, h->am_i);
+  k_argmax2<<<1, 256, 0, s>>>(h->am_v, h->am_i, h->am_parts, h->tokens, h->st, M);
+}
+
 // One pass over M <= MT tokens at device position st->pos0 (forward_pass, kernels.c:306-415), within sp.
 void enqueue_pass(q4hip* h, int M, bool want_logits, AttnSpan sp) {
   const int D = h->D, F = h->F, HD = h->HD, QKV = h->QKV;
@@ -2626,15 +2649,7 @@ void enqueue_pass(q4hip* h, int M, bool want_logits, AttnSpan sp) {
     prof_mark(h, Q4HIP_PROF_DOWN);
     launch_matvec<OP_ADD>(s, y.down, h->xq, h->xstride, M, h->x, D, nullptr, xh_act);
   }
-  if (want_logits) {
-    prof_mark(h, Q4HIP_PROF_NORM_Q);
-    launch_quant<QM_NORM>(s, 1, h->x, D, D, h->out_norm, h->eps, h->xq, h->xstride, M - 1);
-    prof_mark(h, Q4HIP_PROF_OUT);
-    launch_head(s, h->head, h->xq, h->logits);
-    prof_mark(h, Q4HIP_PROF_SAMPLE);
-    k_argmax1<<<h->am_parts, 256, 0, s>>>(h->logits, h->V, h->am_v, h->am_i);
-    k_argmax2<<<1, 256, 0, s>>>(h->am_v, h->am_i, h->am_parts, h->tokens, h->st, M);
-  }
+  if (want_logits) enqueue_next(h, M);
   prof_mark(h, -1);
 }
 
@@ -3386,9 +3401,73 @@ struct q4hip_batch {
   int *am_i = nullptr, *tok = nullptr, *pos = nullptr, *out = nullptr;
   int out_cap = 0;           // ints of `out`
   int* pin = nullptr;        // pinned staging: B tokens, B positions
+  // a batch on the paged 8-bit cache (kc, vc and sc are null)
+  q4hip_kv8* kv8 = nullptr;
+  std::vector<int> len;      // positions of a sequence in the cache
+  int pages = 0;
+  int *have = nullptr, *add = nullptr;   // [B] positions and rows of a step; `ones`: a row of each
+  int* ones = nullptr;
+  int* at = nullptr;         // [2][MT] sequences and positions to read back
 };
 
 namespace {
+
+// Positions and rows of a step of one sequence; the others keep theirs.
+__global__ void k_step_of(int* have, int* add, int B, int seq, int pos, int rows) {
+  for (int b = threadIdx.x; b < B; b += blockDim.x) {
+    if (b == seq) have[b] = pos;
+    add[b] = b == seq ? rows : 0;
+  }
+}
+
+// n positions from pos0 on of sequence seq.
+__global__ void k_positions_of(int* at_seq, int* at_pos, int seq, int pos0, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) { at_seq[i] = seq; at_pos[i] = pos0 + i; }
+}
+
+int pages_of(int n) { return (n + Q4HIP_KV8_BLOCK - 1) / Q4HIP_KV8_BLOCK; }
+
+// Whether the pool holds every sequence's positions when sequence `seq` has `len` of them.
+int check_pages(const q4hip_batch* bt, int seq, int len) {
+  int64_t need = 0;
+  for (int b = 0; b < bt->B; b++) need += pages_of(b == seq ? len : bt->len[b]);
+  if (need > bt->pages) return fail(Q4HIP_ECONTEXT, "cache full: %lld pages needed, the pool has %d", (long long)need, bt->pages);
+  return Q4HIP_OK;
+}
+
+// A step of `rows` rows of sequence seq at pos..: its pages and rows.
+void plan_of(q4hip_batch* bt, int seq, int pos, int rows) {
+  k_step_of<<<1, 256, 0, bt->h->stream>>>(bt->have, bt->add, bt->B, seq, pos, rows);
+  kv8_launch_plan(bt->kv8, bt->h->stream, bt->have, bt->add, rows, nullptr, nullptr, nullptr, nullptr);
+}
+
+// The layers of the M planned rows in h->x, whose positions are pos[] (device), on the 8-bit cache.
+void enqueue_kv8_layers(q4hip_batch* bt, int M, const int* pos) {
+  q4hip* h = bt->h;
+  const int D = h->D, F = h->F, HD = h->HD, QKV = h->QKV;
+  hipStream_t s = h->stream;
+  uint4* xh = M > 1 ? h->xh : nullptr;
+  for (int l = 0; l < h->NL; l++) {
+    Layer& y = h->L[l];
+    launch_quant<QM_NORM>(s, M, h->x, D, D, y.attn_norm, h->eps, h->xq, h->xstride, 0, xh);
+    launch_matvec<OP_BIAS>(s, y.qkv, h->xq, h->xstride, M, h->qkv, QKV, y.bqkv, xh);
+    k_rope_rows<<<dim3(h->H + h->KVH, M), HD / 2, 0, s>>>(h->qkv, QKV, HD, h->rope, pos);
+    kv8_launch_append(bt->kv8, s, l, h->qkv + D, h->qkv + D + h->KVH * HD, Q4HIP_TYPE_F32, QKV, QKV, 0, h->KVH);
+    kv8_launch_attend(bt->kv8, s, l, h->qkv, h->att, Q4HIP_TYPE_F32, QKV, D, 0.0f);
+    launch_quant<QM_PLAIN>(s, M, h->att, D, D, nullptr, 0.0f, h->xq, h->xstride, 0, xh);
+    launch_matvec<OP_ADD>(s, y.o, h->xq, h->xstride, M, h->x, D, nullptr, xh);
+    launch_quant<QM_NORM>(s, M, h->x, D, D, y.ffn_norm, h->eps, h->xq, h->xstride, 0, xh);
+    uint4* xh_act = xh;
+    if (launch_gu_swiglu(s, y.gu, xh, h->xstride, M, h->xq, h->xh2, F)) {
+      xh_act = h->xh2;
+    } else {
+      launch_matvec<OP_STORE>(s, y.gu, h->xq, h->xstride, M, h->gu, 2 * F, nullptr, xh);
+      launch_quant<QM_SWIGLU>(s, M, h->gu, 2 * F, F, nullptr, 0.0f, h->xq, h->xstride, 0, xh);
+    }
+    launch_matvec<OP_ADD>(s, y.down, h->xq, h->xstride, M, h->x, D, nullptr, xh_act);
+  }
+}
 
 // One decode step of all B sequences: tokens bt->tok at positions bt->pos; the greedy tokens go to
 // bt->tok (and out[0..B) when given) and every position advances by one, within sp.
@@ -3398,7 +3477,11 @@ void enqueue_batch_step(q4hip_batch* bt, int* out, AttnSpan sp) {
   hipStream_t s = h->stream;
   uint4* xh = B > 1 ? h->xh : nullptr;
   k_embed_list<<<B, 256, 0, s>>>(h->embd, D, bt->tok, h->x);
-  for (int l = 0; l < h->NL; l++) {
+  if (bt->kv8) {
+    kv8_launch_plan(bt->kv8, s, bt->pos, bt->ones, B, nullptr, nullptr, nullptr, nullptr);
+    enqueue_kv8_layers(bt, B, bt->pos);
+  }
+  for (int l = 0; !bt->kv8 && l < h->NL; l++) {
     Layer& y = h->L[l];
     launch_quant<QM_NORM>(s, B, h->x, D, D, y.attn_norm, h->eps, h->xq, h->xstride, 0, xh);
     SkRope rp;
@@ -3456,21 +3539,27 @@ void q4hip_batch_destroy(q4hip_batch* bt) {
   if (!bt) return;
   (void)hipSetDevice(bt->h->device);
   (void)hipStreamSynchronize(bt->h->stream);
-  void* bufs[] = {bt->kc, bt->vc, bt->logits, bt->am_v, bt->am_i, bt->tok, bt->pos, bt->out, bt->sc};
+  q4hip_kv8_destroy(bt->kv8);
+  void* bufs[] = {bt->kc, bt->vc, bt->logits, bt->am_v, bt->am_i, bt->tok, bt->pos, bt->out, bt->sc, bt->have, bt->add, bt->ones,
+                  bt->at};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (bt->pin) (void)hipHostFree(bt->pin);
   delete bt;
 }
 
-int q4hip_batch_create(q4hip_batch** out, q4hip* h, int B) {
+// pages > 0: a batch on the 8-bit cache.
+static int create_batch(q4hip_batch** out, q4hip* h, int B, int pages) {
   if (!out || !h) return fail(Q4HIP_EINVAL, "null argument");
   *out = nullptr;
   if (B <= 0 || B > h->MT) return fail(Q4HIP_EINVAL, "%d sequences: a batch holds 1..%d (the context's pass size)", B, h->MT);
-  if (h->H / h->KVH > kMaxGroup) return fail(Q4HIP_EINVAL, "more than %d query heads per kv head", kMaxGroup);
   HIPCHK(hipSetDevice(h->device));
-  const size_t lds = attn_pv_lds(h->H, h->KVH, h->ctx);
-  if (!attn_list_ok(h->H, h->KVH, h->HD, h->ctx))
-    return fail(Q4HIP_EINVAL, "ctx %d: batched attention needs %zu bytes of shared memory", h->ctx, lds);
+  size_t lds = 0;
+  if (!pages) {
+    if (h->H / h->KVH > kMaxGroup) return fail(Q4HIP_EINVAL, "more than %d query heads per kv head", kMaxGroup);
+    lds = attn_pv_lds(h->H, h->KVH, h->ctx);
+    if (!attn_list_ok(h->H, h->KVH, h->HD, h->ctx))
+      return fail(Q4HIP_EINVAL, "ctx %d: batched attention needs %zu bytes of shared memory", h->ctx, lds);
+  }
   q4hip_batch* bt = new q4hip_batch();
   bt->h = h;
   bt->B = B;
@@ -3480,16 +3569,28 @@ int q4hip_batch_create(q4hip_batch** out, q4hip* h, int B) {
   const size_t kvbytes = (size_t)B * bt->seq_stride * h->kvb;
   hipError_t e = hipSuccess;
   auto al = [&](void** p, size_t bytes) { if (e == hipSuccess) e = hipMalloc(p, bytes); };
-  al((void**)&bt->kc, kvbytes);
-  al((void**)&bt->vc, kvbytes);
+  if (!pages) {
+    al((void**)&bt->kc, kvbytes);
+    al((void**)&bt->vc, kvbytes);
+    al((void**)&bt->sc, (size_t)B * h->H * score_stride(h->ctx) * 4);
+  } else {
+    al((void**)&bt->have, (size_t)B * 4);
+    al((void**)&bt->add, (size_t)B * 4);
+    al((void**)&bt->ones, (size_t)B * 4);
+    al((void**)&bt->at, (size_t)2 * h->MT * 4);
+  }
   al((void**)&bt->logits, (size_t)B * h->V * 4);
   al((void**)&bt->am_v, (size_t)B * bt->P * 4);
   al((void**)&bt->am_i, (size_t)B * bt->P * 4);
   al((void**)&bt->tok, (size_t)B * 4);
   al((void**)&bt->pos, (size_t)B * 4);
-  al((void**)&bt->sc, (size_t)B * h->H * score_stride(h->ctx) * 4);
-  if (e == hipSuccess) e = hipMemsetAsync(bt->kc, 0, kvbytes, h->stream);
-  if (e == hipSuccess) e = hipMemsetAsync(bt->vc, 0, kvbytes, h->stream);
+  if (!pages) {
+    if (e == hipSuccess) e = hipMemsetAsync(bt->kc, 0, kvbytes, h->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(bt->vc, 0, kvbytes, h->stream);
+  } else {
+    if (e == hipSuccess) e = hipMemsetAsync(bt->have, 0, (size_t)B * 4, h->stream);
+    if (e == hipSuccess) e = hipMemsetD32Async((hipDeviceptr_t)bt->ones, 1, B, h->stream);
+  }
   if (e == hipSuccess) e = hipHostMalloc((void**)&bt->pin, (size_t)2 * B * 4, hipHostMallocDefault);
   if (e == hipSuccess) e = hipStreamSynchronize(h->stream);   // caches zeroed before q4hip_batch_set_kv
   if (e != hipSuccess) {
@@ -3497,7 +3598,99 @@ int q4hip_batch_create(q4hip_batch** out, q4hip* h, int B) {
     q4hip_batch_destroy(bt);
     return rc;
   }
+  if (pages) {
+    bt->pages = pages;
+    bt->len.assign(B, 0);
+    const int rc = q4hip_kv8_create(&bt->kv8, h->NL, h->H, h->KVH, h->HD, B, h->ctx, pages, std::max(h->MT, h->ctx), h->device);
+    if (rc != Q4HIP_OK) {
+      q4hip_batch_destroy(bt);
+      return rc;
+    }
+  }
   *out = bt;
+  return Q4HIP_OK;
+}
+
+int q4hip_batch_create(q4hip_batch** out, q4hip* h, int B) { return create_batch(out, h, B, 0); }
+
+int q4hip_batch_create_kv8(q4hip_batch** out, q4hip* h, int B, int pages) {
+  if (pages <= 0) return fail(Q4HIP_EINVAL, "a pool of %d pages", pages);
+  return create_batch(out, h, B, pages);
+}
+
+// K and V rows of positions from pos0 on of one kv head.
+static int set_kv8(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, int n, const float* k, const float* v) {
+  q4hip* h = bt->h;
+  const int HD = h->HD;
+  if (pos0 > bt->len[seq]) return fail(Q4HIP_EINVAL, "position %d: sequence %d holds %d", pos0, seq, bt->len[seq]);
+  if (pos0 + n < bt->len[seq])
+    return fail(Q4HIP_EINVAL, "positions %d..%d: sequence %d holds %d, and the 8-bit cache is written to the end", pos0, pos0 + n, seq,
+                bt->len[seq]);
+  const int rc = check_pages(bt, seq, pos0 + n);
+  if (rc) return rc;
+  // all at once: a step that ended before the sequence does would give its last pages back
+  float* rows = nullptr;
+  const size_t bytes = (size_t)n * HD * 4;
+  HIPCHK(hipMalloc(&rows, 2 * bytes));
+  hipError_t e = hipMemcpyAsync(rows, k, bytes, hipMemcpyHostToDevice, h->stream);
+  if (e == hipSuccess) e = hipMemcpyAsync(rows + (size_t)n * HD, v, bytes, hipMemcpyHostToDevice, h->stream);
+  if (e == hipSuccess) {
+    plan_of(bt, seq, pos0, n);
+    kv8_launch_append(bt->kv8, h->stream, layer, rows, rows + (size_t)n * HD, Q4HIP_TYPE_F32, HD, HD, kv_head, 1);
+    k_step_of<<<1, 256, 0, h->stream>>>(bt->have, bt->add, bt->B, seq, pos0 + n, 0);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
+  (void)hipFree(rows);
+  if (e != hipSuccess) return fail(Q4HIP_EHIP, "K/V rows: %s", hipGetErrorString(e));
+  bt->len[seq] = pos0 + n;
+  return Q4HIP_OK;
+}
+
+int q4hip_batch_get_kv(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, int n, float* k, float* v) {
+  if (!bt || !k || !v) return fail(Q4HIP_EINVAL, "null argument");
+  q4hip* h = bt->h;
+  const int HD = h->HD, row = h->KVH * HD;
+  if (!bt->kv8) return fail(Q4HIP_EINVAL, "a batch on the 8-bit cache expected");
+  if (seq < 0 || seq >= bt->B) return fail(Q4HIP_EINVAL, "sequence %d of %d", seq, bt->B);
+  if (layer < 0 || layer >= h->NL) return fail(Q4HIP_EINVAL, "layer %d of %d", layer, h->NL);
+  if (kv_head < 0 || kv_head >= h->KVH) return fail(Q4HIP_EINVAL, "kv head %d of %d", kv_head, h->KVH);
+  if (n <= 0 || pos0 < 0 || (int64_t)pos0 + n > bt->len[seq])
+    return fail(Q4HIP_ECONTEXT, "positions %d..%lld: sequence %d holds %d", pos0, (long long)pos0 + n, seq, bt->len[seq]);
+  HIPCHK(hipSetDevice(h->device));
+  HIPCHK(hipStreamSynchronize(h->stream));
+  plan_of(bt, seq, bt->len[seq], 0);
+  for (int i = 0; i < n; i += h->MT) {
+    const int m = std::min(n - i, h->MT);
+    float* const dv = h->qkv + (size_t)m * row;
+    k_positions_of<<<(m + 255) / 256, 256, 0, h->stream>>>(bt->at, bt->at + h->MT, seq, pos0 + i, m);
+    kv8_launch_read(bt->kv8, h->stream, layer, bt->at, bt->at + h->MT, m, h->qkv, dv);
+    HIPCHK(hipGetLastError());
+    HIPCHK(hipStreamSynchronize(h->stream));
+    const size_t line = (size_t)HD * 4;
+    HIPCHK(hipMemcpy2D(k + (size_t)i * HD, line, h->qkv + kv_head * HD, row * 4, line, m, hipMemcpyDeviceToHost));
+    HIPCHK(hipMemcpy2D(v + (size_t)i * HD, line, dv + kv_head * HD, row * 4, line, m, hipMemcpyDeviceToHost));
+  }
+  return Q4HIP_OK;
+}
+
+int q4hip_batch_release(q4hip_batch* bt, int seq) {
+  if (!bt) return fail(Q4HIP_EINVAL, "null argument");
+  if (!bt->kv8) return fail(Q4HIP_EINVAL, "a batch on the 8-bit cache expected");
+  if (seq < 0 || seq >= bt->B) return fail(Q4HIP_EINVAL, "sequence %d of %d", seq, bt->B);
+  HIPCHK(hipSetDevice(bt->h->device));
+  plan_of(bt, seq, 0, 0);
+  HIPCHK(hipGetLastError());
+  HIPCHK(hipStreamSynchronize(bt->h->stream));
+  bt->len[seq] = 0;
+  return Q4HIP_OK;
+}
+
+int q4hip_batch_free_pages(q4hip_batch* bt, int* pages) {
+  if (!bt || !pages) return fail(Q4HIP_EINVAL, "null argument");
+  if (!bt->kv8) return fail(Q4HIP_EINVAL, "a batch on the 8-bit cache expected");
+  *pages = bt->pages;
+  for (int n : bt->len) *pages -= pages_of(n);
   return Q4HIP_OK;
 }
 
@@ -3511,8 +3704,35 @@ int q4hip_batch_set_kv(q4hip_batch* bt, int seq, int layer, int kv_head, int pos
   if (n <= 0 || pos0 < 0 || (int64_t)pos0 + n > h->ctx) return fail(Q4HIP_ECONTEXT, "positions %d..%lld outside 0..%d", pos0, (long long)pos0 + n, h->ctx);
   HIPCHK(hipSetDevice(h->device));
   HIPCHK(hipStreamSynchronize(h->stream));
+  if (bt->kv8) return set_kv8(bt, seq, layer, kv_head, pos0, n, k, v);
   const size_t off = (size_t)seq * bt->seq_stride + (((size_t)layer * h->KVH + kv_head) * h->ctx + pos0) * h->HD;
   return upload_kv(h, (char*)bt->kc + off * h->kvb, (char*)bt->vc + off * h->kvb, k, v, (size_t)n * h->HD);
+}
+
+static int prefill_kv8(q4hip_batch* bt, int seq, const int* ids, int n, int pos, int* next) {
+  q4hip* h = bt->h;
+  hipStream_t s = h->stream;
+  if (pos > bt->len[seq]) return fail(Q4HIP_EINVAL, "position %d: sequence %d holds %d", pos, seq, bt->len[seq]);
+  const int rc = check_pages(bt, seq, pos + n);
+  if (rc) return rc;
+  memcpy(h->pin_ids, ids, (size_t)n * 4);
+  HIPCHK(hipMemcpyAsync(h->tokens + pos, h->pin_ids, (size_t)n * 4, hipMemcpyHostToDevice, s));
+  for (int c = 0; c < n; c += h->MT) {
+    const int k = std::min(h->MT, n - c);
+    k_set_pos<<<1, 64, 0, s>>>(h->st, pos + c);
+    k_embed<<<k, 256, 0, s>>>(h->embd, h->D, h->tokens, h->st, h->x);
+    k_pass_pos<<<(k + 255) / 256, 256, 0, s>>>(h->st, k, h->tpos);
+    plan_of(bt, seq, pos + c, k);
+    enqueue_kv8_layers(bt, k, h->tpos);
+    if (c + k >= n) enqueue_next(h, k);
+  }
+  k_step_of<<<1, 256, 0, s>>>(bt->have, bt->add, bt->B, seq, pos + n, 0);
+  HIPCHK(hipGetLastError());
+  HIPCHK(hipMemcpyAsync(h->pin_next, &h->st->next, 4, hipMemcpyDeviceToHost, s));
+  HIPCHK(hipStreamSynchronize(s));
+  bt->len[seq] = pos + n;
+  *next = h->pin_next[0];
+  return Q4HIP_OK;
 }
 
 int q4hip_batch_prefill(q4hip_batch* bt, int seq, const int* ids, int n, int pos, int* next) {
@@ -3526,6 +3746,7 @@ int q4hip_batch_prefill(q4hip_batch* bt, int seq, const int* ids, int n, int pos
   rc = check_ids(h, ids, n);
   if (rc) return rc;
   HIPCHK(hipSetDevice(h->device));
+  if (bt->kv8) return prefill_kv8(bt, seq, ids, n, pos, next);
   prepare_attention(h);
   // the passes run eagerly against this sequence's cache; the context's own cache is untouched
   void* kc = h->kc;
@@ -3560,6 +3781,14 @@ static int run_batch(q4hip_batch* bt, const int* first, const int* pos, int step
   if (rc) return rc;
   rc = check_ids(h, first, B);
   if (rc) return rc;
+  if (bt->kv8) {
+    int64_t need = 0;
+    for (int b = 0; b < B; b++) {
+      if (pos[b] > bt->len[b]) return fail(Q4HIP_EINVAL, "position %d: sequence %d holds %d", pos[b], b, bt->len[b]);
+      need += pages_of(pos[b] + steps);
+    }
+    if (need > bt->pages) return fail(Q4HIP_ECONTEXT, "cache full: %lld pages needed, the pool has %d", (long long)need, bt->pages);
+  }
   HIPCHK(hipSetDevice(h->device));
   if ((int64_t)steps * B > bt->out_cap) {
     if (bt->out) HIPCHK(hipFree(bt->out));
@@ -3581,8 +3810,11 @@ static int run_batch(q4hip_batch* bt, const int* first, const int* pos, int step
   const AttnSpan sp = batch_span(pos, B, h->KVH, steps);
   for (int i = 0; i < steps; i++) enqueue_batch_step(bt, bt->out + (size_t)i * B, sp);
   if (ms) HIPCHK(hipEventRecord(e1, h->stream));
+  if (bt->kv8) HIPCHK(hipMemcpyAsync(bt->have, bt->pos, (size_t)B * 4, hipMemcpyDeviceToDevice, h->stream));
   HIPCHK(hipGetLastError());
   HIPCHK(hipStreamSynchronize(h->stream));
+  if (bt->kv8)
+    for (int b = 0; b < B; b++) bt->len[b] = pos[b] + steps;
   if (ms) {
     HIPCHK(hipEventElapsedTime(ms, e0, e1));
     (void)hipEventDestroy(e0);

@@ -82,9 +82,13 @@ const DECODE_NAMES = { 0: null, 1: "graph", 2: "persistent" };
 //                                  at position pos[b]
 //   readLogits() -> Float32Array(B * vocab), the last step's logits, sequence by sequence
 //   destroy()
+// With kv8Pages the sequences share that many pages of 32 positions of an 8-bit cache instead
+// (q4hip_batch_create_kv8 in include/q4hip.h says what differs):
+//   release(seq)   gives the sequence's pages back
+//   freePages()    pages that no sequence holds
 // Calls on a batch and on its backend share the backend's buffers and run one at a time.
-function makeBatch(a, h, B, vocab, ctx) {
-  const bt = a.batchCreate(h, B);
+function makeBatch(a, h, B, vocab, ctx, kv8Pages) {
+  const bt = kv8Pages === undefined ? a.batchCreate(h, B) : a.batchCreate(h, B, kv8Pages);
   const ints = (xs, what) => {
     if (xs.length !== B) throw new Error(`${what}: ${B} entries expected, got ${xs.length}`);
     return Int32Array.from(xs);
@@ -113,6 +117,8 @@ function makeBatch(a, h, B, vocab, ctx) {
       a.batchReadLogits(bt, lg);
       return lg;
     },
+    release(seq) { a.batchRelease(bt, seq); },
+    freePages() { return a.batchFreePages(bt); },
     destroy() { a.batchDestroy(bt); },
   };
 }
@@ -223,7 +229,7 @@ async function createHIP(gguf, bytes, cfg, opts = {}) {
     },
     // The path of the last decode step: "persistent", "graph", or null before any.
     decodeModeUsed() { return DECODE_NAMES[a.decodeModeUsed(h)]; },
-    createBatch(B) { return makeBatch(a, h, B, vocab, ctx); },
+    createBatch(B, { kv8Pages } = {}) { return makeBatch(a, h, B, vocab, ctx, kv8Pages); },
     destroy() { a.destroy(h); },
   };
 }

@@ -377,20 +377,22 @@ static napi_value js_decode_mode_used(napi_env env, napi_callback_info info) {
   return out;
 }
 
-/* batchCreate(handle, B) -> batch handle: B sequences with their own K/V caches, decoded together
- * with the context's weights (q4hip_batch_create).  Released by batchDestroy, by destroy of the
- * context, or when collected. */
+/* batchCreate(handle, B[, pages]) -> batch handle: B sequences with their own K/V caches, or sharing
+ * `pages` pages of an 8-bit one, decoded together with the context's weights (q4hip_batch_create,
+ * q4hip_batch_create_kv8).  Released by batchDestroy, by destroy of the context, or when collected. */
 static napi_value js_batch_create(napi_env env, napi_callback_info info) {
-  size_t argc = 2;
-  napi_value a[2];
+  size_t argc = 3;
+  napi_value a[3];
   NAPI_CALL(env, napi_get_cb_info(env, info, &argc, a, NULL, NULL));
   if (argc < 2) { napi_throw_type_error(env, NULL, "batchCreate: 2 arguments"); return NULL; }
   ctx_slot* c = get_slot(env, a[0]);
   if (!c) return NULL;
   int32_t B;
   if (!get_i32(env, a[1], &B)) { napi_throw_type_error(env, NULL, "batchCreate: integer B expected"); return NULL; }
+  int32_t pages = 0;
+  if (argc > 2 && !get_i32(env, a[2], &pages)) { napi_throw_type_error(env, NULL, "batchCreate: integer pages expected"); return NULL; }
   q4hip_batch* bt = NULL;
-  int rc = q4hip_batch_create(&bt, c->h, B);
+  int rc = argc > 2 ? q4hip_batch_create_kv8(&bt, c->h, B, pages) : q4hip_batch_create(&bt, c->h, B);
   if (rc) return throw_status(env, rc);
   batch_slot* b = (batch_slot*)calloc(1, sizeof *b);
   if (!b) { q4hip_batch_destroy(bt); napi_throw_error(env, NULL, "out of memory"); return NULL; }
@@ -424,6 +426,37 @@ static napi_value js_batch_destroy(napi_env env, napi_callback_info info) {
   b->bt = NULL;
   unlink_batch(b);
   return NULL;
+}
+
+/* batchRelease(batch, seq): gives the sequence's pages back (8-bit cache) */
+static napi_value js_batch_release(napi_env env, napi_callback_info info) {
+  size_t argc = 2;
+  napi_value a[2];
+  NAPI_CALL(env, napi_get_cb_info(env, info, &argc, a, NULL, NULL));
+  if (argc < 2) { napi_throw_type_error(env, NULL, "batchRelease: 2 arguments"); return NULL; }
+  batch_slot* b = get_batch(env, a[0]);
+  if (!b) return NULL;
+  int32_t seq;
+  if (!get_i32(env, a[1], &seq)) { napi_throw_type_error(env, NULL, "batchRelease: integer seq expected"); return NULL; }
+  int rc = q4hip_batch_release(b->bt, seq);
+  if (rc) return throw_status(env, rc);
+  return NULL;
+}
+
+/* batchFreePages(batch) -> pages that no sequence holds (8-bit cache) */
+static napi_value js_batch_free_pages(napi_env env, napi_callback_info info) {
+  size_t argc = 1;
+  napi_value a[1];
+  NAPI_CALL(env, napi_get_cb_info(env, info, &argc, a, NULL, NULL));
+  if (argc < 1) { napi_throw_type_error(env, NULL, "batchFreePages: 1 argument"); return NULL; }
+  batch_slot* b = get_batch(env, a[0]);
+  if (!b) return NULL;
+  int pages = 0;
+  int rc = q4hip_batch_free_pages(b->bt, &pages);
+  if (rc) return throw_status(env, rc);
+  napi_value out;
+  NAPI_CALL(env, napi_create_int32(env, pages, &out));
+  return out;
 }
 
 /* batchPrefill(batch, seq, Int32Array ids, pos) -> next id of sequence seq */
@@ -540,6 +573,8 @@ static napi_value init(napi_env env, napi_value exports) {
       {"decodeModeUsed", NULL, js_decode_mode_used, NULL, NULL, NULL, napi_enumerable, NULL},
       {"batchCreate", NULL, js_batch_create, NULL, NULL, NULL, napi_enumerable, NULL},
       {"batchDestroy", NULL, js_batch_destroy, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"batchRelease", NULL, js_batch_release, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"batchFreePages", NULL, js_batch_free_pages, NULL, NULL, NULL, napi_enumerable, NULL},
       {"batchPrefill", NULL, js_batch_prefill, NULL, NULL, NULL, napi_enumerable, NULL},
       {"batchSetKv", NULL, js_batch_set_kv, NULL, NULL, NULL, napi_enumerable, NULL},
       {"batchGenerate", NULL, js_batch_generate, NULL, NULL, NULL, napi_enumerable, NULL},

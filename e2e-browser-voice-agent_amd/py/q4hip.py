@@ -35,6 +35,7 @@ EXPORTS = [
     "q4hip_batch_prefill", "q4hip_batch_set_kv", "q4hip_batch_generate", "q4hip_batch_time_generate",
     "q4hip_batch_read_logits", "q4hip_mv_time_cold", "q4hip_check_division", "q4hip_mv_run_noalloc",
     "q4hip_attn_ring_rows", "q4hip_check_ordered_sum", "q4hip_kv8_create", "q4hip_kv8_destroy", "q4hip_kv8_plan",
+    "q4hip_batch_create_kv8", "q4hip_batch_release", "q4hip_batch_free_pages", "q4hip_batch_get_kv",
     "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend",
 ]
 
@@ -88,6 +89,10 @@ def lib() -> ctypes.CDLL:
         "q4hip_batch_read_logits": (I, [P, P, I64]),
         "q4hip_mv_time_cold": (I, [P, I64, I, ctypes.POINTER(F), ctypes.POINTER(I)]),
         "q4hip_mv_run_noalloc": (I, [P, P, P, P]),
+        "q4hip_batch_create_kv8": (I, [ctypes.POINTER(P), P, I, I]),
+        "q4hip_batch_release": (I, [P, I]),
+        "q4hip_batch_free_pages": (I, [P, ctypes.POINTER(I)]),
+        "q4hip_batch_get_kv": (I, [P, I, I, I, I, I, P, P]),
         "q4hip_kv8_create": (I, [ctypes.POINTER(P), I, I, I, I, I, I, I, I, I]),
         "q4hip_kv8_destroy": (None, [P]),
         "q4hip_kv8_plan": (I, [P, P, P, I, P, P, P, P, P]),
@@ -286,13 +291,17 @@ class Model:
 
 
 class Batch:
-    """B sequences decoded together with one Model's weights, each with its own K/V cache.
+    """B sequences decoded together with one Model's weights, each with its own K/V cache, or sharing
+    kv8_pages pages of an 8-bit one (q4hip_batch_create_kv8).
     Holds a reference to the model; close the batch before closing the model explicitly."""
 
-    def __init__(self, model: Model, B: int):
+    def __init__(self, model: Model, B: int, kv8_pages: int = 0):
         self.model, self.B = model, B
         h = ctypes.c_void_p()
-        _check(lib().q4hip_batch_create(ctypes.byref(h), model.h, B))
+        if kv8_pages:
+            _check(lib().q4hip_batch_create_kv8(ctypes.byref(h), model.h, B, kv8_pages))
+        else:
+            _check(lib().q4hip_batch_create(ctypes.byref(h), model.h, B))
         self.h = h
         if not hasattr(model, "_batches"):
             model._batches = weakref.WeakSet()
@@ -310,6 +319,21 @@ class Batch:
         v = np.ascontiguousarray(v, dtype=np.float32)
         assert k.shape == v.shape and k.shape[1] == self.model.shape.head_dim
         _check(lib().q4hip_batch_set_kv(self.h, seq, layer, kv_head, pos0, k.shape[0], _ptr(k), _ptr(v)))
+
+    def get_kv(self, seq: int, layer: int, kv_head: int, pos0: int, n: int) -> tuple:
+        """K and V rows [n][head_dim] that an 8-bit cache stands for at positions pos0.."""
+        k, v = (np.empty((max(n, 0), self.model.shape.head_dim), np.float32) for _ in range(2))
+        _check(lib().q4hip_batch_get_kv(self.h, seq, layer, kv_head, pos0, n, _ptr(k), _ptr(v)))
+        return k, v
+
+    def release(self, seq: int) -> None:
+        """Give the pages of a sequence back to an 8-bit cache's pool."""
+        _check(lib().q4hip_batch_release(self.h, seq))
+
+    def free_pages(self) -> int:
+        n = ctypes.c_int(0)
+        _check(lib().q4hip_batch_free_pages(self.h, ctypes.byref(n)))
+        return n.value
 
     def _args(self, first, pos):
         f = np.ascontiguousarray(first, dtype=np.int32)

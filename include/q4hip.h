@@ -200,6 +200,23 @@ int q4hip_batch_time_generate(q4hip_batch* bt, const int* first, const int* pos,
 /* Logits of the last step, [B][vocab] floats; n >= B * vocab. */
 int q4hip_batch_read_logits(q4hip_batch* bt, float* out, int64_t n);
 
+/* A batch on the paged 8-bit cache (q4hip_kv8_* below) instead: its sequences share a pool of `pages` pages of
+ * Q4HIP_KV8_BLOCK positions, 2 * layers * kv_heads * (32 * head_dim + 4) bytes each -- a quarter of the fp32
+ * cache's bytes, and only for positions that are held.  The calls above work on it with these differences:
+ * K and V are rounded to 8 bits as q4hip_kv8_append does, and attention is q4hip_kv8_attend's (not the
+ * reference's order of operations: results are close to, not equal to those of the other caches, and of a prompt cut into passes at
+ * other positions); a call that needs more pages than the pool has fails with Q4HIP_ECONTEXT before anything
+ * runs; positions are written in order: `pos` (pos0 of q4hip_batch_set_kv) is at most the number of positions that the
+ * sequence holds, and afterwards it ends with the call's last position (q4hip_batch_set_kv refuses one
+ * before its end); any number of query heads per kv head and any ctx of the context. */
+int q4hip_batch_create_kv8(q4hip_batch** out, q4hip* h, int B, int pages);
+/* Give a sequence's pages back (8-bit cache): it holds no position afterwards. */
+int q4hip_batch_release(q4hip_batch* bt, int seq);
+/* Pages of the pool that no sequence holds (8-bit cache). */
+int q4hip_batch_free_pages(q4hip_batch* bt, int* pages);
+/* The K and V [n][head_dim] fp32 that the 8-bit cache stands for at positions pos0.. of a sequence. */
+int q4hip_batch_get_kv(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, int n, float* k, float* v);
+
 /* ---- isolated Q4_0 matvec (the kernel of every projection) ---------------------------------
  * y[n] = W[n] . x for an N x K Q4_0 matrix given in GGUF layout, with x quantized to int8 per
  * 32-block exactly as quantize_row (engine/kernels.c:90-114) and each output accumulated as
