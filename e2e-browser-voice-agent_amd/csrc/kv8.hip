@@ -39,22 +39,23 @@ __device__ int doublings(float s, float t) {
 }
 
 // A run of rows (blockIdx.x) of one kv head; K for blockIdx.z = 0, else V.  The rows pass through shared memory, where
-// their 32-bit values are turned into the order of the codes; a thread forms the 16 codes that lie together.
+// their 32-bit values are turned into the order of the codes; a thread forms 16 codes that lie together.
 // kWide: rows whose 16 bytes can be loaded at once.
 template <int HD, class T, bool kWide>
-__global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
+__global__ __launch_bounds__(2 * HD) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
                                                     int64_t k_stride, int64_t v_stride, int rows, int g0) {
   __shared__ float tile[kKv8Block][HD + 1];
-  __shared__ float most[4];
-  __shared__ int odd;                          // a value that is not finite
+  __shared__ float most[HD / 32];
+  __shared__ int odd[HD / 32];                 // of a wave's values, whether one is not finite
   const int g = g0 + blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const bool is_v = blockIdx.z != 0;
-  if (v.head->rows > rows) {                   // replayed on a larger plan than it was launched for
+  const Kv8Head head = *v.head;
+  const Kv8Run run = v.runs[blockIdx.x];       // on its way together with the head: the grid is no larger than the list
+  if (head.rows > rows) {                      // replayed on a larger plan than it was launched for
     if (tid == 0) v.head->status = KV8_STALE;
     return;
   }
-  if ((int)blockIdx.x >= v.head->runs) return;
-  const Kv8Run run = v.runs[blockIdx.x];
+  if ((int)blockIdx.x >= head.runs) return;
   const int m = run.m, f = run.slot % kKv8Block;
   const int64_t ld = is_v ? v_stride : k_stride;
   const T* x = (is_v ? val : k) + (int64_t)run.t * ld + (int)blockIdx.y * HD;
@@ -63,11 +64,8 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const 
   uint4* const codes = (uint4*)(v.codes + (block * 2 + (is_v ? 1 : 0)) * (kKv8Block * HD));
   const bool whole = m == kKv8Block;
   const float before = *scale;
-  uint4 w[HD / 128 > 0 ? HD / 128 : 1] = {};
-  if (!whole)
-    for (int i = 0, u = tid; u < 2 * HD; i++, u += 256) w[i] = codes[u];
-  if (tid == 0) odd = 0;
-  __syncthreads();
+  uint4 w = {};
+  if (!whole) w = codes[tid];
   float a = 0.0f;
   bool strange = false;
   auto take = [&](int r, int c, float y) {
@@ -78,7 +76,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const 
   };
   if constexpr (kWide) {
     constexpr int kVec = 16 / sizeof(T), kCols = HD / kVec;
-    for (int i = tid; i < m * kCols; i += 256) {
+    for (int i = tid; i < m * kCols; i += 2 * HD) {
       const int r = i / kCols, c = i % kCols * kVec;
       struct alignas(16) Vec { T y[kVec]; };
       const Vec z = *(const Vec*)(x + r * ld + c);
@@ -86,61 +84,65 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8View v, int layer, const 
       for (int j = 0; j < kVec; j++) take(r, c + j, (float)z.y[j]);
     }
   } else {
-    for (int i = tid; i < m * HD; i += 256) take(i / HD, i % HD, (float)x[i / HD * ld + i % HD]);
+    for (int i = tid; i < m * HD; i += 2 * HD) take(i / HD, i % HD, (float)x[i / HD * ld + i % HD]);
   }
-  if (strange) odd = 1;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) a = __builtin_fmaxf(a, __shfl_xor(a, d));
-  if (lane == 0) most[tid >> 6] = a;
+  const bool any_strange = __builtin_amdgcn_ballot_w64(strange) != 0;
+  if (lane == 0) { most[tid >> 6] = a; odd[tid >> 6] = any_strange; }
   __syncthreads();
-  a = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
+  int any_odd = 0;
+  a = 0.0f;
+#pragma unroll
+  for (int i = 0; i < HD / 32; i++) {
+    a = __builtin_fmaxf(a, most[i]);
+    any_odd |= odd[i];
+  }
   const float old = f ? before : 0.0f, t127 = a / 127.0f, need = t127 < kKv8MinScale ? 0.0f : t127;
   const int twice = old > 0.0f ? doublings(old, need) : 0;
   const float s = old > 0.0f ? __builtin_ldexpf(old, twice) : need;
-  const bool any = odd != 0 || !(s > 0.0f);
+  const bool any = any_odd || !(s > 0.0f);
   const float r = any ? 0.0f : 1.0f / s;
-  for (int i = 0, u = tid; u < 2 * HD; i++, u += 256) {
-    const int ln = u & 63, q = u >> 6;
-    uint32_t* const words = (uint32_t*)&w[i];
-    bool changed = whole;
+  const int q = tid >> 6;
+  uint32_t* const words = (uint32_t*)&w;
+  bool changed = whole;
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      // four codes: columns of a position of K, positions of a column of V, one after the other
-      int tok, col;
-      if (is_v) {
-        tok = ((j >> 2) & 1) * 16 + (ln >> 4) * 4;
-        col = (2 * q + (j >> 3)) * 16 + (ln & 15);
+  for (int j = 0; j < 16; j += 4) {
+    // four codes: columns of a position of K, positions of a column of V, one after the other
+    int tok, col;
+    if (is_v) {
+      tok = ((j >> 2) & 1) * 16 + (lane >> 4) * 4;
+      col = (2 * q + (j >> 3)) * 16 + (lane & 15);
+    } else {
+      tok = q / (HD / 64) * 16 + (lane & 15);
+      col = (2 * (q % (HD / 64)) + (j >> 3)) * 32 + (lane >> 4) * 8 + (j & 7);
+    }
+    const int dt = is_v ? 1 : 0, dc = 1 - dt;
+    if (whole && !any) {
+      uint32_t c[4];
+#pragma unroll
+      for (int b = 0; b < 4; b++) c[b] = code_bits(tile[tok + b * dt][col + b * dc], s, r);
+      const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+      words[j >> 2] = lo | hi;
+      continue;
+    }
+    for (int b = 0; b < 4; b++) {
+      const int tk = tok + b * dt, sh = 8 * b;
+      uint32_t c;
+      if (tk >= f && tk < f + m) {
+        const float y = tile[tk][col + b * dc];
+        c = any ? code_bits_any(y, s) : code_bits(y, s, r);
+      } else if (tk < f && twice) {
+        const int before_code = (int)(words[j >> 2] >> sh & 255) - 128;
+        c = (uint32_t)((int)__builtin_rintf(__builtin_ldexpf((float)before_code, -twice)) + 128);
       } else {
-        tok = q / (HD / 64) * 16 + (ln & 15);
-        col = (2 * (q % (HD / 64)) + (j >> 3)) * 32 + (ln >> 4) * 8 + (j & 7);
-      }
-      const int dt = is_v ? 1 : 0, dc = 1 - dt;
-      if (whole && !any) {
-        uint32_t c[4];
-#pragma unroll
-        for (int b = 0; b < 4; b++) c[b] = code_bits(tile[tok + b * dt][col + b * dc], s, r);
-        const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
-        words[j >> 2] = lo | hi;
         continue;
       }
-      for (int b = 0; b < 4; b++) {
-        const int tk = tok + b * dt, sh = 8 * b;
-        uint32_t c;
-        if (tk >= f && tk < f + m) {
-          const float y = tile[tk][col + b * dc];
-          c = any ? code_bits_any(y, s) : code_bits(y, s, r);
-        } else if (tk < f && twice) {
-          const int before_code = (int)(words[j >> 2] >> sh & 255) - 128;
-          c = (uint32_t)((int)__builtin_rintf(__builtin_ldexpf((float)before_code, -twice)) + 128);
-        } else {
-          continue;
-        }
-        words[j >> 2] = (words[j >> 2] & ~(255u << sh)) | (c & 255u) << sh;
-        changed = true;
-      }
+      words[j >> 2] = (words[j >> 2] & ~(255u << sh)) | (c & 255u) << sh;
+      changed = true;
     }
-    if (changed) codes[u] = w[i];
   }
+  if (changed) codes[tid] = w;
   if (tid == 0 && s != before) *scale = s;      // every thread has read the old one before the barriers
 }
 
@@ -267,7 +269,7 @@ void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, c
     using T = decltype(zero);
     auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
                           : (wide ? k_kv8_append<128, T, true> : k_kv8_append<128, T, false>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0);
+    fn<<<grid, 2 * w.HD, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0);
   });
 }
 

@@ -534,12 +534,15 @@ template <int HD, class T, int N>
 __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
                                                     int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide) {
   __shared__ Kv8Shared<HD> sh;
+  const int ys = v.KVH * v.row_tiles;
   const Kv8Head head = *v.head;
+  Kv8Item it;
+  if constexpr (N == 0) it = v.items[blockIdx.x / ys];      // on its way together with the head: the grid is no larger than the list
   if (head.rows > rows) {                      // replayed on a larger plan than it was launched for
     if (threadIdx.x == 0) v.head->status = KV8_STALE;
     return;
   }
-  const int ys = v.KVH * v.row_tiles, tiles = N ? head.tiles * v.KVH : 0, all = tiles + head.items * ys;
+  const int tiles = N ? head.tiles * v.KVH : 0, all = tiles + head.items * ys;
   for (int i = blockIdx.x; i < all; i += gridDim.x) {
     if constexpr (N > 0)
       if (i < tiles) {
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, con
         continue;
       }
     const int k = i - tiles, y = k % ys;
-    const Kv8Item it = v.items[k / ys];
+    if (N > 0 || i != (int)blockIdx.x) it = v.items[k / ys];
     if constexpr (N > 0)
       if (it.wide) {
         kv8_item<HD, T, N>(v, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
