@@ -214,6 +214,27 @@ int check_rows(const q4hip_kv8* kv, const void* p, int rows, int width, int64_t 
   return check_device_span(p, ((size_t)(rows - 1) * stride + width) * es, kv->device, what);
 }
 
+// Rows that one call reads and another buffer's that it writes must not share a byte.  Neighbouring columns of the same
+// rows may: where the strides differ, the whole spans count.
+int check_apart(const void* p, int64_t p_stride, const void* out, int64_t out_stride, int rows, int width, int type) {
+  const int es = elem_size(type);
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)out, w = (uintptr_t)width * es;
+  const uintptr_t a_end = a + (uintptr_t)(rows - 1) * p_stride * es + w, b_end = b + (uintptr_t)(rows - 1) * out_stride * es + w;
+  if (a_end <= b || b_end <= a) return Q4HIP_OK;
+  if (p_stride == out_stride) {
+    const uintptr_t s = (uintptr_t)p_stride * es, d = b >= a ? (b - a) % s : (s - (a - b) % s) % s;
+    if (d >= w && s - d >= w) return Q4HIP_OK;
+  }
+  return fail(Q4HIP_EINVAL, "q and out overlap");
+}
+
+// int32 arrays of n elements; NULL or an empty one is not looked at.
+int check_ints(const q4hip_kv8* kv, const void* p, size_t n, const char* what) {
+  if (!p || !n) return Q4HIP_OK;
+  if ((uintptr_t)p % 4) return fail(Q4HIP_EINVAL, "%s: not aligned to its type", what);
+  return check_device_span(p, n * 4, kv->device, what);
+}
+
 int plan_error(const q4hip_kv8* kv, int status) {
   switch (status) {
     case KV8_OK: return Q4HIP_OK;
@@ -402,11 +423,10 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
   const struct { const void* p; size_t n; const char* what; } spans[] = {
       {have, (size_t)v.B, "have"}, {add, (size_t)v.B, "add"}, {starts, (size_t)v.B + 1, "starts"},
       {positions, (size_t)rows, "positions"}, {slots, (size_t)rows, "slots"}, {tables, (size_t)v.B * v.W, "tables"}};
-  for (const auto& a : spans)
-    if (a.p && a.n) {
-      const int rc = check_device_span(a.p, a.n * 4, kv->device, a.what);
-      if (rc) return rc;
-    }
+  for (const auto& a : spans) {
+    const int rc = check_ints(kv, a.p, a.n, a.what);
+    if (rc) return rc;
+  }
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   kv8_launch_plan(kv, s, have, add, rows, starts, positions, slots, tables);
   HIPCHK(hipGetLastError());
@@ -452,8 +472,8 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
   HIPCHK(hipSetDevice(kv->device));
   const Kv8View& w = kv->v;
   const size_t row = (size_t)w.KVH * w.HD;
-  rc = check_device_span(seq, (size_t)n * 4, kv->device, "seq");
-  if (!rc) rc = check_device_span(pos, (size_t)n * 4, kv->device, "pos");
+  rc = check_ints(kv, seq, n, "seq");
+  if (!rc) rc = check_ints(kv, pos, n, "pos");
   if (!rc) rc = check_rows(kv, k, n, (int)row, row, Q4HIP_TYPE_F32, "k");
   if (!rc) rc = check_rows(kv, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
   if (rc) return rc;
@@ -475,6 +495,7 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   const Kv8View& w = kv->v;
   rc = check_rows(kv, q, kv->rows, w.H * w.HD, q_stride, type, "q");
   if (!rc) rc = check_rows(kv, out, kv->rows, w.H * w.HD, out_stride, type, "out");
+  if (!rc) rc = check_apart(q, q_stride, out, out_stride, kv->rows, w.H * w.HD, type);
   if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   kv8_launch_attend(kv, s, layer, q, out, type, q_stride, out_stride, scale);

@@ -172,7 +172,8 @@ struct Kv8Rows {
         if constexpr (kTwo) q[t][1][s][i] = (_Float16)(y - (float)hi);
         else all += (float)hi;
       }
-    c[t] = __builtin_ldexpf(scale, -e + (kTwo ? 0 : 24));
+    // finite also for q of 2^119 and more, as the product with a page's K scale of 0 is 0
+    c[t] = __builtin_fminf(__builtin_ldexpf(scale, -e + (kTwo ? 0 : 24)), -kKv8Lowest);
     if constexpr (!kTwo) {
       all = kv8_sum_quarters(all) * -0x1p-17f;                  // 128 * 2^-24
       first[t] = kv8_f4{all, all, all, all};

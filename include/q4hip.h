@@ -262,7 +262,9 @@ int q4hip_mv_run_noalloc(q4hip_mv* m, const float* x, float* y, void* stream);
  * stream, so that it can be captured into a HIP graph.  `stream` (a hipStream_t) NULL: the handle's own
  * stream, and the call waits for its end.  Pointers are device memory of the handle's device and are
  * checked, with the bytes behind them, before anything is launched.  Calls on one handle are serialized by the caller, also on the GPU: calls on
- * several streams, or graphs that hold them, are ordered by events or waits.  Handles are independent. */
+ * several streams, or graphs that hold them, are ordered by events or waits.  Handles are independent.  A captured
+ * append or attend serves plans of up to the `rows` of the plan that it was captured after; replayed on a larger
+ * one it does nothing, and q4hip_kv8_status returns Q4HIP_ESTATE. */
 typedef struct q4hip_kv8 q4hip_kv8;
 #define Q4HIP_KV8_BLOCK 32
 /* A cache of `pages` pages for `seqs` sequences of up to max_len positions; plans hold up to max_rows
@@ -303,7 +305,7 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
 /* out = softmax(scale * q . K) V of the step's rows, each over the positions of its sequence up to its own: row t, head h,
  * column d at q[t * q_stride + h * head_dim + d], `out` alike; head h reads kv head h / (heads / kv_heads).
  * Scores, the softmax and the sums are fp32; `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
- * the step's are left as they were. */
+ * the step's are left as they were.  q and out may be columns of the same rows, but not the same ones. */
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
 

@@ -116,23 +116,25 @@ def attend(q, K, V, ks, vs, have, scale, half_eps):
     G = H // K.shape[1]
     out, bound = np.zeros((n, H, hd)), np.zeros((n, H, hd))
     K, V = K.astype(np.float64), V.astype(np.float64)
+    L = have + 1 + np.arange(n)                        # positions that a row looks at
+    seen = np.arange(have + n)[None, :] < L[:, None]
     for h in range(H):
-        kk, vv = K[:, h // G], V[:, h // G]
-        for i in range(n):
-            L = have + i + 1
-            y = q[i, h].astype(np.float64)
-            s = scale * (kk[:L] @ y)
-            p = np.exp(s - s.max())
-            l = p.sum()
-            out[i, h] = p @ vv[:L] / l
-            A = p @ np.abs(vv[:L]) / l
-            S = scale * (np.abs(kk[:L]) @ np.abs(y) + add * ks[:L, h // G] * np.abs(y).sum())
-            ds = S.max() * ((hd + 8) * 2.0 ** -24 + 2.0 ** -22)
-            w = np.maximum(vs[:L, h // G], 2.0 ** -100)
-            rel, sums = np.expm1(2 * ds), (L / 32 + 48) * 2.0 ** -23
-            if half_eps > 2.0 ** -20:
-                rel += 2.0 ** -11
-            rel += L * 2.0 ** -126 * w.max() / w.min()
-            err = A * rel + (A + add * (p @ vs[:L, h // G]) / l) * sums + L * 2.0 ** -39 * 127 * (p * w).max() / l
-            bound[i, h] = err + (np.abs(out[i, h]) + err) * half_eps
+        kk, vv, k_s, v_s = K[:have + n, h // G], V[:have + n, h // G], ks[:have + n, h // G], vs[:have + n, h // G]
+        y = q[:, h].astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            s = np.where(seen, scale * (y @ kk.T), -np.inf)
+            p = np.exp(s - s.max(1, keepdims=True))
+        l = p.sum(1, keepdims=True)
+        out[:, h] = p @ vv / l
+        A = p @ np.abs(vv) / l
+        S = np.where(seen, scale * (np.abs(y) @ np.abs(kk).T + add * k_s[None, :] * np.abs(y).sum(1, keepdims=True)), 0)
+        ds = S.max(1, keepdims=True) * ((hd + 8) * 2.0 ** -24 + 2.0 ** -22)
+        w = np.where(seen, np.maximum(v_s, 2.0 ** -100)[None, :], np.nan)
+        rel, sums = np.expm1(2 * ds), (L[:, None] / 32 + 48) * 2.0 ** -23
+        if half_eps > 2.0 ** -20:
+            rel = rel + 2.0 ** -11
+        rel = rel + L[:, None] * 2.0 ** -126 * np.nanmax(w, 1, keepdims=True) / np.nanmin(w, 1, keepdims=True)
+        err = A * rel + (A + add * (p @ v_s)[:, None] / l) * sums
+        err = err + L[:, None] * 2.0 ** -39 * 127 * np.nanmax(p * w, 1, keepdims=True) / l
+        bound[:, h] = err + (np.abs(out[:, h]) + err) * half_eps
     return out, bound

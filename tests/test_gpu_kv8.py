@@ -279,6 +279,46 @@ def test_attend_long(H, KVH, hd, dtype):
     t.attend(rng, dtype, size=4.0)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("H,KVH,hd,add", [(32, 32, 64, [300, 1, 129, 65, 700, 0, 1500, 2]), (44, 11, 64, [200, 33, 1000, 1, 700]),
+                                          (20, 10, 128, [1, 900, 1800, 2, 1200]), (99, 3, 64, [500, 1, 330, 40])])
+def test_attend_tiles(H, KVH, hd, add, dtype):
+    """Rows enough for tiles (kKv8MinTiles workgroups), of prompts behind other positions and beside tokens."""
+    rng = np.random.default_rng(H)
+    G = H // KVH
+    assert KVH * sum(-(-a * G // 128) if a > max(1, 16 // G) else a > 0 for a in add) >= 640
+    have = [int(h) for h in rng.integers(0, 100, len(add))]
+    t = Both(H, KVH, hd, len(add), 2000, 250, sum(add))
+    t.plan([0] * len(add), have)
+    t.fill(rng, dtype)
+    t.plan(have, add)
+    t.fill(rng, dtype)
+    t.attend(rng, dtype)
+
+
+def test_attend_many_sequences_and_rows():
+    """More sequences than the plan's shared memory holds; lists that are filled by a second launch."""
+    rng = np.random.default_rng(3)
+    t = Both(4, 2, 64, 1300, 100, 4000, 40000)
+    have = rng.integers(0, 60, 1300)
+    have[::7] = 0
+    t.plan([0] * 1300, have.tolist())
+    t.fill(rng, "f32")
+    add = np.where(rng.random(1300) < 0.2, 0, 1)
+    add[5], add[1111] = 40, 33
+    t.plan(have.tolist(), add.tolist())
+    t.fill(rng, "f32")
+    t.check_values()
+    t.attend(rng, "f32")
+    t = Both(2, 1, 64, 2, 9000, 400, 9000)
+    t.plan([0, 0], [8600, 100])
+    t.fill(rng, "bf16")
+    t.check_values()
+    t.plan([300, 100], [50, 7])
+    t.fill(rng, "bf16")
+    t.attend(rng, "bf16")
+
+
 def test_attend_is_the_same_every_time():
     rng = np.random.default_rng(2)
     t = Both(14, 2, 64, 3, 5000, 400, 9000)
@@ -304,6 +344,20 @@ def test_attend_large_and_small_values(dtype):
     t.fill(rng, dtype)
     for size in (1e-4, 1.0, 50.0):
         t.attend(rng, dtype, size=size)
+
+
+def test_the_largest_queries_of_bf16_on_a_cache_of_zeros():
+    """Scores of 0: the mean of V, however large q is."""
+    rng = np.random.default_rng(14)
+    t = Both(14, 2, 64, 2, 700, 30, 700)
+    t.plan([0, 0], [600, 40])
+    v = rng.standard_normal((640, 2, 64)).astype(np.float32)
+    t.append(np.zeros_like(v), v, "bf16")
+    t.plan([600, 40], [1, 1])
+    v = rng.standard_normal((2, 2, 64)).astype(np.float32)
+    t.append(np.zeros_like(v), v, "bf16")
+    t.attend(rng, "bf16", size=1e35)
+    t.attend(rng, "bf16", size=2e37)
 
 
 def test_nan_and_infinite_queries_stay_in_their_rows():
@@ -416,6 +470,42 @@ def test_a_step_of_a_server_captured_and_replayed():
         lens = [a + b for a, b in zip(lens, more)]
 
 
+def test_a_graph_on_a_plan_that_is_too_large():
+    """append and attend captured for 8 rows do nothing on a plan of 20, and the status says so."""
+    rng = np.random.default_rng(10)
+    t = Both(4, 2, 64, 2, 300, 20, 300)
+    t.plan([0, 0], [30, 0])
+    t.fill(rng, "f32")
+    t.plan([30, 0], [4, 4])
+    w = 8 * 64
+    x, out = torch.randn(20, w, device="cuda"), torch.full((20, 256), 7.0, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        st = torch.cuda.current_stream().cuda_stream
+        t.kv.append(0, x[:, 256:].data_ptr(), x[:, 384:].data_ptr(), q4hip.F32, w, w, st)
+        t.kv.attend(0, x.data_ptr(), out.data_ptr(), q4hip.F32, w, 256, st)
+    t.plan([30, 0], [10, 10])
+    t.fill(rng, "f32")
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    with pytest.raises(q4hip.Q4Error) as e:
+        t.kv.status()
+    assert e.value.code == q4hip.ESTATE
+    t.check_values()
+    t.plan([30, 0], [4, 4])
+    g.replay()
+    torch.cuda.synchronize()
+    y = x[:8].cpu().numpy()
+    for c, at in ((0, 4), (1, 6)):
+        t.ref[0][c].append(y[:, at * 64:(at + 2) * 64].reshape(8, 2, 64), t.slots)
+    assert (out[8:] == 7).all()
+    t.compare(out[:8].double().cpu().numpy().reshape(8, 4, 64), y[:, :256].reshape(8, 4, 64), "f32")
+    assert t.kv.status()[0] == 8
+
+
 def test_two_handles_on_two_streams():
     rng = np.random.default_rng(12)
     ts = [Both(14, 2, 64, 2, 3000, 200, 4000) for _ in range(2)]
@@ -443,7 +533,8 @@ def test_refusals():
     d = torch.zeros(16 * 256 + 1, device="cuda")
     i = ints([0, 0, 0])
     host = torch.zeros(4096)
-    one = ints([1, 0])
+    one, four = ints([1, 0]), ints([4, 0])
+    both = torch.zeros(16 * 1024, device="cuda")
     torch.cuda.synchronize()
     p, ip, hp = d.data_ptr(), i.data_ptr(), host.data_ptr()
 
@@ -479,6 +570,20 @@ def test_refusals():
     refused(q4hip.EINVAL, kv.attend, 0, p, hp, q4hip.F32, 256, 256)
     refused(q4hip.EINVAL, kv.attend, 0, p, p, q4hip.F32, 255, 256)
     refused(q4hip.EINVAL, kv.attend, 0, p, p, q4hip.F32, 256, 255)
+    a, wide = both.data_ptr(), 1024
+    kv.plan(ip, four.data_ptr(), 4)
+    refused(q4hip.EINVAL, kv.attend, 0, a, a, q4hip.F32, 256, 256)
+    refused(q4hip.EINVAL, kv.attend, 0, a, a + 4, q4hip.F32, wide, wide)
+    refused(q4hip.EINVAL, kv.attend, 0, a + 4 * 255, a, q4hip.F32, wide, wide)
+    refused(q4hip.EINVAL, kv.attend, 0, a, a + 4 * (wide + 255), q4hip.F32, wide, wide)
+    refused(q4hip.EINVAL, kv.attend, 0, a, a + 4 * 256, q4hip.F32, wide, 256)
+    kv.attend(0, a, a + 4 * 256, q4hip.F32, wide, wide)
+    kv.attend(0, a + 4 * 256, a, q4hip.F32, wide, wide)
+    kv.attend(0, a, a + 4 * 1024, q4hip.F32, 256, 256)
+    kv.plan(ip, one.data_ptr(), 1)
+    refused(q4hip.EINVAL, kv.plan, ip + 2, ip, 1)
+    refused(q4hip.EINVAL, kv.plan, ip, ip, 1, 0, ip + 1)
+    refused(q4hip.EINVAL, kv.read, 0, ip, ip + 2, 1, p, p)
     for scale in (float("nan"), float("inf"), -1.0):
         refused(q4hip.EINVAL, kv.attend, 0, p, p, q4hip.F32, 256, 256, 0, scale)
     refused(q4hip.EINVAL, kv.read, 0, ip, ip, -1, p, p)
