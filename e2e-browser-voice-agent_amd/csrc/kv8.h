@@ -91,6 +91,7 @@ struct Kv8View {
   int unit_rows, wide_rows;       // rows of a unit
   int row_tiles;       // of a unit: 16 rows (32 of a wide one, which has no more of them)
   int items_aim;       // items that fill the GPU
+  double aim_inverse;  // 1 / items_aim, not rounded down
 };
 
 }  // namespace q4

@@ -13,7 +13,10 @@ namespace q4 {
 namespace {
 
 constexpr int kItemsAim = 256;          // workgroups of attention: one for each CU
-constexpr size_t kFillInPlan = 8192;
+// Entries of a plan's lists (rows, the caller's tables) up to which one workgroup fills them, with the sums in shared memory (one
+// launch against two: 200 sequences with tables, 6,400 entries, 9.0 us and 11.1; 48 with 2,171 rows 7.2 and 8.4) and in
+// global memory (6,000 sequences 63 us and 38).
+constexpr size_t kFillInPlan = 8192, kFillInPlanGlobal = 2048;
 constexpr int64_t kMostWorkgroups = 8192;   // of attention; a workgroup takes every so-manieth tile or item
 
 // The quotient x / s rounded to fp32, from r = 1 / s rounded: one correction of x * r by its residual gives it
@@ -266,12 +269,13 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
                      int* tables) {
   const Kv8View& v = kv->v;
   kv->rows = rows;
-  // what the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds
+  // What the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds, which takes less
+  // than a second launch does.
   const size_t items = rows + std::min<size_t>(kKv8MoreItems * v.items_aim, rows ? (size_t)v.pages * rows / kKv8MinPart : 0);
   const size_t entries = std::max<size_t>(items, tables ? (size_t)v.B * v.W : 0);
-  const bool fill = entries <= kFillInPlan;
-  if (v.B <= kPlanShared) {
-    const int threads = v.B <= 256 && entries <= 2048 ? 256 : kPlanThreads;
+  const bool shared = v.B <= kPlanShared, fill = entries <= (shared ? kFillInPlan : kFillInPlanGlobal);
+  if (shared) {
+    const int threads = v.B <= 512 && (!fill || entries <= 2048) ? 512 : kPlanThreads;
     k_kv8_plan<true><<<1, threads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
   } else {
     k_kv8_plan<false><<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
@@ -374,6 +378,7 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   v.wide_rows = std::max(1, 32 / G);
   v.row_tiles = (std::min(v.unit_rows, max_rows) * G + 15) / 16;
   v.items_aim = std::max(1, kItemsAim / (kv_heads * v.row_tiles));
+  v.aim_inverse = std::nextafter(1.0 / v.items_aim, 2.0);
   const size_t blocks = (size_t)layers * pages * kv_heads, bytes = blocks * 2 * kKv8Block * head_dim;
   hipError_t e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
   auto al = [&](auto** p, size_t n) { if (e == hipSuccess) e = hipMalloc((void**)p, n * sizeof(**p)); };
