@@ -17,7 +17,17 @@
 // the 128 add to a score is subtracted by the product's first addend, and what they add to O in the end, from the
 // sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
 // an earlier one's: its weights may be too small for fp16 where its probabilities are not.)
+//
+// What bounds it.  One token of a short text: the launch and one chain of loads (5.5 us at 300 positions).  Many tokens: the
+// cache's bytes, 1.12 GB in 212 us, 5.3 TB/s (64 sequences of up to 16,000 positions, 8 kv heads of 128 columns); a 1 GiB copy
+// moves 5.15.  Prompts: the vector instructions that turn codes into fp16 (64 of some 150 for a page and 32 rows), form the
+// exponentials (16, at a quarter of the rate) and find the largest, 67% of the issue slots, beside matrix instructions that are
+// busy 45% of the time: 8,192 bf16 rows, 32 heads of 128, in 577 us, 953 TFLOP/s; a large bf16 product reaches 1,221.
+// Not kept: raised priority around the matrix instructions (0 to 8% slower); a page's scores formed beside the weights of the page
+// before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7% slower).
 #pragma once
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace q4 {
@@ -98,6 +108,14 @@ struct Kv8Codes {
   }
 };
 
+// Whether weights are sums of two fp16 numbers: of fp32 rows, and of fp16 rows by 16 (tokens).  One fp16 number is off by up to
+// 2^-11.  Over 131,072 positions of similar weight that made the error of fp16 outputs 2.8e-4 where their own
+// rounding is 2.0e-4; the second number takes it back to 2.0e-4 for 1 to 5% of the time.  In a prompt, whose first
+// rows see few positions, it is 1.8 to 2.3e-4 with one number and 1.8 to 2.2e-4 with two, for 17 to 33% of the time: there it is one.  In bf16
+// outputs, rounded by 2^-8, it does not show.
+template <class T, int N>
+constexpr bool kLowWeights = sizeof(T) == 4 || (std::is_same_v<T, _Float16> && N == 1);
+
 // What the softmax needs of a page's scales.
 struct Kv8Scale {
   float k, v, iv, mant;      // K scale; v, 2^-v; the V scale over 2^v
@@ -115,7 +133,7 @@ __device__ inline Kv8Scale kv8_scale(float2 s) {
 }
 
 // 16 N rows of a wave.  Lane l: rows l % 16 of each 16, quarter l / 16 of every contraction.
-template <int HD, bool kTwo, int N>
+template <int HD, bool kTwo, bool kLow, int N>
 struct Kv8Rows {
   kv8_h8 q[N][kTwo ? 2 : 1][HD / 32];
   kv8_f4 o[N][HD / 16];
@@ -255,7 +273,7 @@ struct Kv8Rows {
         l[t] = __builtin_fmaf(kv8_sum_quarters(all), sc.iv, l[t]);
       }
     const float l_scale = faint ? 0.0f : sc.iv;
-    kv8_h8 hi[N], lo[kTwo ? N : 1];
+    kv8_h8 hi[N], lo[kLow ? N : 1];
 #pragma unroll
     for (int t = 0; t < N; t++) {
       const float v = sc.v - m[t];
@@ -271,11 +289,13 @@ struct Kv8Rows {
           lo[t][i] = (_Float16)(y - (float)hi[t][i]);
         } else {
           hi[t][i] = (_Float16)e;
+          if constexpr (kLow) lo[t][i] = (_Float16)(e - (float)hi[t][i]);
         }
       }
       if constexpr (!kTwo) {
         const kv8_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-        const kv8_f4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi[t], kv8_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        kv8_f4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi[t], kv8_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        if constexpr (kLow) r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo[t], r, 0, 0, 0);
         sum[t] += r[0];
         all = r[0];
       }
@@ -288,7 +308,7 @@ struct Kv8Rows {
       for (int t = 0; t < N; t++) {
         o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hi[t], o[t][2 * p], 0, 0, 0);
         o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hi[t], o[t][2 * p + 1], 0, 0, 0);
-        if constexpr (kTwo) {
+        if constexpr (kLow) {
           o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo[t], o[t][2 * p], 0, 0, 0);
           o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo[t], o[t][2 * p + 1], 0, 0, 0);
         }
@@ -417,19 +437,20 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
   return sh.last != 0;
 }
 
-// An item of the plan and 16 N of its unit's rows of a kv head (y).  The four waves take every fourth page each and
+// An item of the plan and 16 N of its unit's rows of a kv head (y).  Waves share the pages and not the rows, as a token has
+// few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 13.7 us.  The four waves take every fourth page each and
 // add up their sums in shared memory, 16 rows at a time.  A unit in several parts: the last workgroup of each 16 parts to be
 // done adds those up, and the last of these the sums of 16, always in the order of the parts.
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,
                                          int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {
-  constexpr bool kTwo = sizeof(T) == 4;
+  constexpr bool kTwo = sizeof(T) == 4, kLow = kLowWeights<T, N>;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * (16 * N);
   const int rows = min(16 * N, it.n * G - r0);                  // of this tile
   if (rows <= 0) return;
-  Kv8Rows<HD, kTwo, N> w;
+  Kv8Rows<HD, kTwo, kLow, N> w;
   int row_last[N];
   const T* row[N];
 #pragma unroll
@@ -495,17 +516,18 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
 }
 
 // Many rows: 64 N neighbouring rows of a sequence and kv head (row r: position r / G of the step, head r % G), 16 N of each
-// wave, which passes over all the pages that they look at.
+// wave, which passes over all the pages that they look at.  So a page is fetched once for 128 rows, and from the L2 by each
+// wave: no shared memory, no barrier.  (32 rows of a wave rather than 16: the codes' fp16 forms serve both.)
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q, T* out, int64_t q_stride, int64_t out_stride,
                                          float scale, bool wide, int tile, int g) {
-  constexpr bool kTwo = sizeof(T) == 4;
+  constexpr bool kTwo = sizeof(T) == 4, kLow = kLowWeights<T, N>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const Kv8Tile it = v.tiles[tile];
   const int r0 = it.tile * kKv8TileRows + wave * (16 * N), end = it.n * G;
   if (r0 >= end) return;
-  Kv8Rows<HD, kTwo, N> w;
+  Kv8Rows<HD, kTwo, kLow, N> w;
   int last[N];
   const T* row[N];
 #pragma unroll

@@ -330,6 +330,32 @@ def test_attend_is_the_same_every_time():
     assert all(torch.equal(g, got[0]) for g in got)
 
 
+@pytest.mark.parametrize("H,KVH,hd", [(14, 2, 64), (32, 8, 128), (20, 20, 64)])
+def test_fp16_tokens_are_as_good_as_their_rounding(H, KVH, hd):
+    """Weights in one fp16 number add an error of the size of the output's own rounding where many positions count alike, which makes
+    the root of the mean square 1.4 times that of the rounding alone.  Two numbers add 2^-22 relative to the weights, and the
+    scores' fp32 rounding less than 2^-18: nothing of 2^-12.  1.1 leaves room for the 2,000 values' chance."""
+    rng = np.random.default_rng(15)
+    t = Both(H, KVH, hd, 2, 3100, 200, 4000)
+    t.plan([0, 0], [3000, 700])
+    t.fill(rng, "f16")
+    t.plan([3000, 700], [1, 1])
+    t.fill(rng, "f16")
+    w = H * hd
+    q = (0.1 * torch.randn(2, w, generator=torch.Generator().manual_seed(3))).half().cuda()
+    out = torch.zeros(2, w, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    t.kv.attend(0, q.data_ptr(), out.data_ptr(), q4hip.F16, w, w)
+    got, err, rounding = out.double().cpu().numpy().reshape(2, H, hd), 0.0, 0.0
+    for b, n in enumerate((3001, 701)):
+        K, V = (c.values(t.pool.tables[b], n) for c in t.ref[0])
+        ks, vs = (c.scale_of(t.pool.tables[b], n) for c in t.ref[0])
+        want = kv8_ref.attend(q[b:b + 1].float().cpu().numpy().reshape(1, H, hd), K, V, ks, vs, n - 1, hd ** -0.5, HALF["f16"])[0][0]
+        err += np.square(got[b] - want).sum()
+        rounding += np.square(want.astype(np.float16).astype(np.float64) - want).sum()
+    assert err < 1.1 ** 2 * rounding
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_large_and_small_values(dtype):
     """Rows and pages of very different size: scores far apart, V scales from 1e-6 to 1e6."""
