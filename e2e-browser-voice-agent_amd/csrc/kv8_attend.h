@@ -13,7 +13,7 @@
 // fp32 rows (kTwo) hold q and w as sums of two fp16 numbers and multiply twice.  Their codes become fp16 by a byte permute
 // (0x6400 | u = 1024 + u) and one packed subtraction, exactly; v is a whole number there and the scale's rest a factor
 // of w, so that 2^-v is exact.
-// 16-bit rows multiply once.  Their codes are the fp16 numbers u * 2^-24, u = code + 128: the byte permute alone.  What
+// 16-bit rows multiply once, but for the weights of fp16 tokens (kLowWeights).  Their codes are the fp16 numbers u * 2^-24, u = code + 128: the byte permute alone.  What
 // the 128 add to a score is subtracted by the product's first addend, and what they add to O in the end, from the
 // sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
 // an earlier one's: its weights may be too small for fp16 where its probabilities are not.)
@@ -108,11 +108,11 @@ struct Kv8Codes {
   }
 };
 
-// Whether weights are sums of two fp16 numbers: of fp32 rows, and of fp16 rows by 16 (tokens).  One fp16 number is off by up to
-// 2^-11.  Over 131,072 positions of similar weight that made the error of fp16 outputs 2.8e-4 where their own
-// rounding is 2.0e-4; the second number takes it back to 2.0e-4 for 1 to 5% of the time.  In a prompt, whose first
-// rows see few positions, it is 1.8 to 2.3e-4 with one number and 1.8 to 2.2e-4 with two, for 17 to 33% of the time: there it is one.  In bf16
-// outputs, rounded by 2^-8, it does not show.
+// Whether weights are sums of two fp16 numbers: of fp32 rows, and of fp16 rows by 16 (tokens).  One fp16 number is
+// off by up to 2^-11.  Over 131,072 positions of similar weight that made the error of fp16 outputs 2.8e-4 where
+// their own rounding is 2.0e-4; the second number takes it back to 2.0e-4 for 1 to 5% of the time.  In a prompt,
+// whose first rows see few positions, it is 1.8 to 2.3e-4 with one number and 1.8 to 2.2e-4 with two, for 17 to 33%
+// of the time: there it is one.  In bf16 outputs, rounded by 2^-8, it does not show.
 template <class T, int N>
 constexpr bool kLowWeights = sizeof(T) == 4 || (std::is_same_v<T, _Float16> && N == 1);
 
@@ -438,8 +438,8 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
 }
 
 // An item of the plan and 16 N of its unit's rows of a kv head (y).  Waves share the pages and not the rows, as a token has
-// few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 13.7 us.  The four waves take every fourth page each and
-// add up their sums in shared memory, 16 rows at a time.  A unit in several parts: the last workgroup of each 16 parts to be
+// few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 13.8 us.
+// The four waves take every fourth page each and add up their sums in shared memory, 16 rows at a time.  A unit in several parts: the last workgroup of each 16 parts to be
 // done adds those up, and the last of these the sums of 16, always in the order of the parts.
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,

@@ -204,8 +204,8 @@ int q4hip_batch_read_logits(q4hip_batch* bt, float* out, int64_t n);
  * Q4HIP_KV8_BLOCK positions, 2 * layers * kv_heads * (32 * head_dim + 4) bytes each -- a quarter of the fp32
  * cache's bytes, and only for positions that are held.  The calls above work on it with these differences:
  * K and V are rounded to 8 bits as q4hip_kv8_append does, and attention is q4hip_kv8_attend's (not the
- * reference's order of operations: results are close to, not equal to those of the other caches, and of a prompt cut into passes at
- * other positions); a call that needs more pages than the pool has fails with Q4HIP_ECONTEXT before anything
+ * reference's order of operations: results are close to, not equal to those of the other caches, and of a prompt
+ * cut into passes at other positions); a call that needs more pages than the pool has fails with Q4HIP_ECONTEXT before anything
  * runs; positions are written in order: `pos` (pos0 of q4hip_batch_set_kv) is at most the number of positions that the
  * sequence holds, and afterwards it ends with the call's last position (q4hip_batch_set_kv refuses one
  * before its end); any number of query heads per kv head and any ctx of the context. */
@@ -261,10 +261,10 @@ int q4hip_mv_run_noalloc(q4hip_mv* m, const float* x, float* y, void* stream);
  * Nothing is allocated after q4hip_kv8_create, and all of a step's work is enqueued on the caller's
  * stream, so that it can be captured into a HIP graph.  `stream` (a hipStream_t) NULL: the handle's own
  * stream, and the call waits for its end.  Pointers are device memory of the handle's device and are
- * checked, with the bytes behind them, before anything is launched.  Calls on one handle are serialized by the caller, also on the GPU: calls on
- * several streams, or graphs that hold them, are ordered by events or waits.  Handles are independent.  A captured
- * append or attend serves plans of up to the `rows` of the plan that it was captured after; replayed on a larger
- * one it does nothing, and q4hip_kv8_status returns Q4HIP_ESTATE. */
+ * checked, with the bytes behind them, before anything is launched.  Calls on one handle are serialized by the
+ * caller, also on the GPU: calls on several streams, or graphs that hold them, are ordered by events or waits.
+ * Handles are independent.  A captured append or attend serves plans of up to the `rows` of the plan that it was
+ * captured after; replayed on a larger one it does nothing, and q4hip_kv8_status returns Q4HIP_ESTATE. */
 typedef struct q4hip_kv8 q4hip_kv8;
 #define Q4HIP_KV8_BLOCK 32
 /* A cache of `pages` pages for `seqs` sequences of up to max_len positions; plans hold up to max_rows
@@ -292,8 +292,8 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
 int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages);
 /* K and V of the step's rows, `type` F32, F16 or BF16: row t, kv head g, column d at
  * k[t * k_stride + g * head_dim + d] (strides in elements; the buffers hold the `rows` of the plan).  Of the rows that fall
- * into one page, with the first at offset f of it, and one head: t = max|x| / 127 in fp32, or 0 where that is below 2^-100; f = 0 sets the scale to t; f > 0
- * doubles it until it reaches t, and halves the codes of the f positions before as often, to the nearest even
+ * into one page, with the first at offset f of it, and one head: t = max|x| / 127 in fp32, or 0 where that is below
+ * 2^-100; f = 0 sets the scale to t; f > 0 doubles it until it reaches t, and halves the codes of the f positions before as often, to the nearest even
  * integer.  A code is x / scale in fp32 rounded to the nearest even integer.  A value read back is off by at most
  * half of its page's scale, or by less than the whole of it if the scale has grown since.  NaN counts as 0, an infinity
  * as the largest code of its sign; neither counts for the maximum. */
