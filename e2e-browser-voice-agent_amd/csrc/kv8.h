@@ -72,6 +72,14 @@ struct Kv8Tile {
   int tile, unused[3];
 };
 
+// RoPE beside an append: the table ([positions][head_dim] cosines and sines in turn), the rows' positions, their q.
+struct Kv8Rope {
+  const float* table;
+  const int* pos;
+  float* q;
+  int64_t q_stride;
+};
+
 // The device side of a cache.
 struct Kv8View {
   uint8_t* codes;      // [layers][pages][kv_heads][K, V][32 * HD]
@@ -116,6 +124,8 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
 // heads [g0, g0 + heads) of the cache from heads 0.. of the rows
 void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
                        int64_t v_stride, int g0, int heads);
+// Rows of q|k|v that begin at multiples of 16 bytes: q turned in place, k and v into the cache, k turned on its way.
+void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos);
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
                        int64_t out_stride, float scale);
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v);

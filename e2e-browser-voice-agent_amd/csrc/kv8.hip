@@ -44,6 +44,13 @@ __device__ int doublings(float s, float t) {
   return __builtin_amdgcn_frexp_expf(t) - __builtin_amdgcn_frexp_expf(s) + (mt > ms ? 1 : 0);
 }
 
+// RoPE of 4 columns and of those half a head later (kernels.c:337-345): cs holds their cosines and sines in turn.
+__device__ inline void turn(float4& lo, float4& hi, const float4* cs) {
+  const float4 a = cs[0], b = cs[1], x = lo, y = hi;
+  lo = {x.x * a.x - y.x * a.y, x.y * a.z - y.y * a.w, x.z * b.x - y.z * b.y, x.w * b.z - y.w * b.w};
+  hi = {y.x * a.x + x.x * a.y, y.y * a.z + x.y * a.w, y.z * b.x + x.z * b.y, y.w * b.z + x.w * b.w};
+}
+
 // A run of rows (blockIdx.x) of one kv head; K for blockIdx.z = 0, else V.  The rows pass through shared memory, where
 // their 32-bit values are turned into the order of the codes; a thread forms 16 codes that lie together, so that they leave as
 // 16 bytes; one barrier, as each wave's maximum and its check for infinities cross it together.
@@ -51,14 +58,16 @@ __device__ int doublings(float s, float t) {
 // is one chain of loads, 5.6 us.  A code needs the rounded quotient, which two fused operations give (code_bits), where the
 // division's dozen instructions would bound the kernel.
 // kWide: rows whose 16 bytes can be loaded at once.
-template <int HD, class T, bool kWide>
+// kRope: K is turned by its positions first, and q (blockIdx.z = 2: the heads that read this kv head) in place; a launch less in each
+// layer of a batch's step (32 sequences at 1,024 positions, 28 layers, 2.66 -> 2.61 ms).
+template <int HD, class T, bool kWide, bool kRope>
 __global__ __launch_bounds__(2 * HD) void k_kv8_append(Kv8View v, int layer, const T* __restrict__ k, const T* __restrict__ val,
-                                                     int64_t k_stride, int64_t v_stride, int rows, int g0) {
+                                                     int64_t k_stride, int64_t v_stride, int rows, int g0, Kv8Rope rope) {
   __shared__ float tile[kKv8Block][HD + 1];
   __shared__ float most[HD / 32];
   __shared__ int odd[HD / 32];                 // of a wave's values, whether one is not finite
   const int g = g0 + blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const bool is_v = blockIdx.z != 0;
+  const bool is_v = blockIdx.z == 1;
   const Kv8Head head = *v.head;
   const Kv8Run run = v.runs[blockIdx.x];       // on its way together with the head: the grid is no larger than the list
   if (head.rows > rows) {                      // replayed on a larger plan than it was launched for
@@ -67,6 +76,19 @@ __global__ __launch_bounds__(2 * HD) void k_kv8_append(Kv8View v, int layer, con
   }
   if ((int)blockIdx.x >= head.runs) return;
   const int m = run.m, f = run.slot % kKv8Block;
+  if constexpr (kRope)
+    if (blockIdx.z == 2) {
+      const int G = v.H / v.KVH;
+      for (int i = tid; i < m * G * (HD / 8); i += 2 * HD) {
+        const int r = i / (G * (HD / 8)), e = i - r * (G * (HD / 8)), c = e % (HD / 8) * 4;
+        float4* const p = (float4*)(rope.q + (run.t + r) * rope.q_stride + (g * G + e / (HD / 8)) * HD + c);
+        float4 lo = p[0], hi = p[HD / 8];
+        turn(lo, hi, (const float4*)(rope.table + (size_t)rope.pos[run.t + r] * HD + 2 * c));
+        p[0] = lo;
+        p[HD / 8] = hi;
+      }
+      return;
+    }
   const int64_t ld = is_v ? v_stride : k_stride;
   const T* x = (is_v ? val : k) + (int64_t)run.t * ld + (int)blockIdx.y * HD;
   const size_t block = ((size_t)layer * v.pages + run.slot / kKv8Block) * v.KVH + g;
@@ -84,7 +106,20 @@ __global__ __launch_bounds__(2 * HD) void k_kv8_append(Kv8View v, int layer, con
     if (z < __builtin_inff()) a = __builtin_fmaxf(a, z);
     else strange = true;
   };
-  if constexpr (kWide) {
+  if (kRope && !is_v) {
+    for (int i = tid; i < m * (HD / 8); i += 2 * HD) {
+      const int r = i / (HD / 8), c = i % (HD / 8) * 4;
+      const float4* const p = (const float4*)(x + r * ld + c);
+      float4 lo = p[0], hi = p[HD / 8];
+      turn(lo, hi, (const float4*)(rope.table + (size_t)rope.pos[run.t + r] * HD + 2 * c));
+      const float *const y0 = (const float*)&lo, *const y1 = (const float*)&hi;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        take(r, c + j, y0[j]);
+        take(r, c + HD / 2 + j, y1[j]);
+      }
+    }
+  } else if constexpr (kWide) {
     constexpr int kVec = 16 / sizeof(T), kCols = HD / kVec;
     for (int i = tid; i < m * kCols; i += 2 * HD) {
       const int r = i / kCols, c = i % kCols * kVec;
@@ -291,19 +326,36 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
   if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
 }
 
+namespace {
+
+// runs of a sequence: its rows over 32, and two at its ends
+unsigned runs_bound(const q4hip_kv8* kv) {
+  return (unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(kv->v.B, kv->rows));
+}
+
+}  // namespace
+
 void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
                        int64_t v_stride, int g0, int heads) {
   const Kv8View& w = kv->v;
   if (!kv->rows) return;
-  // runs of a sequence: its rows over 32, and two at its ends
-  const dim3 grid((unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(w.B, kv->rows)), (unsigned)heads, 2);
+  const dim3 grid(runs_bound(kv), (unsigned)heads, 2);
   const bool wide = aligned16(k, k_stride, type) && aligned16(v, v_stride, type);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true> : k_kv8_append<64, T, false>)
-                          : (wide ? k_kv8_append<128, T, true> : k_kv8_append<128, T, false>);
-    fn<<<grid, 2 * w.HD, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0);
+    auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true, false> : k_kv8_append<64, T, false, false>)
+                          : (wide ? k_kv8_append<128, T, true, false> : k_kv8_append<128, T, false, false>);
+    fn<<<grid, 2 * w.HD, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0, Kv8Rope{});
   });
+}
+
+void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos) {
+  const Kv8View& w = kv->v;
+  if (!kv->rows) return;
+  const float *const k = qkv + w.H * w.HD, *const v = k + w.KVH * w.HD;
+  auto* fn = w.HD == 64 ? k_kv8_append<64, float, true, true> : k_kv8_append<128, float, true, true>;
+  fn<<<dim3(runs_bound(kv), (unsigned)w.KVH, 3), 2 * w.HD, 0, s>>>(w, layer, k, v, stride, stride, kv->rows, 0,
+                                                                  Kv8Rope{table, pos, qkv, stride});
 }
 
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,

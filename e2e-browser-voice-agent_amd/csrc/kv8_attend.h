@@ -13,9 +13,9 @@
 // fp32 rows (kTwo) hold q and w as sums of two fp16 numbers and multiply twice.  Their codes become fp16 by a byte permute
 // (0x6400 | u = 1024 + u) and one packed subtraction, exactly; v is a whole number there and the scale's rest a factor
 // of w, so that 2^-v is exact.
-// 16-bit rows multiply once, but for the weights of fp16 tokens (kLowWeights).  Their codes are the fp16 numbers u * 2^-24, u = code + 128: the byte permute alone.  What
-// the 128 add to a score is subtracted by the product's first addend, and what they add to O in the end, from the
-// sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
+// 16-bit rows multiply once, but for the weights of fp16 tokens (kLowWeights).  Their codes are the fp16 numbers
+// u * 2^-24, u = code + 128: the byte permute alone.  What the 128 add to a score is subtracted by the product's first
+// addend, and what they add to O in the end, from the sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
 // an earlier one's: its weights may be too small for fp16 where its probabilities are not.)
 //
 // What bounds it.  One token of a short text: the launch and one chain of loads (5.5 us at 300 positions).  Many tokens: the
@@ -439,8 +439,9 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
 
 // An item of the plan and 16 N of its unit's rows of a kv head (y).  Waves share the pages and not the rows, as a token has
 // few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 13.8 us.
-// The four waves take every fourth page each and add up their sums in shared memory, 16 rows at a time.  A unit in several parts: the last workgroup of each 16 parts to be
-// done adds those up, and the last of these the sums of 16, always in the order of the parts.
+// The four waves take every fourth page each and add up their sums in shared memory, 16 rows at a time.  A unit in
+// several parts: the last workgroup of each 16 parts to be done adds those up, and the last of these the sums of 16, always
+// in the order of the parts.
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,
                                          int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {

@@ -1160,16 +1160,6 @@ __global__ void k_rope_kv_list(float* __restrict__ qkv, int QKV, int D, int H, i
   }
 }
 
-// RoPE of token m's q and k heads at position pos[m], in place (kernels.c:337-345).  Grid (H + KVH, M), HD/2 threads.
-__global__ void k_rope_rows(float* __restrict__ qkv, int QKV, int HD, const float* __restrict__ rope, const int* __restrict__ pos) {
-  const int m = blockIdx.y, i = threadIdx.x, half = HD / 2;
-  float* v = qkv + (size_t)m * QKV + blockIdx.x * HD;
-  const float* cs = rope + (size_t)pos[m] * HD;
-  const float c = cs[2 * i], s = cs[2 * i + 1], x0 = v[i], x1 = v[i + half];
-  v[i] = x0 * c - x1 * s;
-  v[i + half] = x1 * c + x0 * s;
-}
-
 // Attention of token b over positions [0, pos[b]] of sequence b's cache (kernels.c:355-377), in
 // two launches that keep the reference's per-head operation order:
 //   k_attn_scores_list  scores s_t = (q . k_t) * 1/sqrt(head_dim) of the G = H/KVH heads of kv
@@ -3452,8 +3442,7 @@ void enqueue_kv8_layers(q4hip_batch* bt, int M, const int* pos) {
     Layer& y = h->L[l];
     launch_quant<QM_NORM>(s, M, h->x, D, D, y.attn_norm, h->eps, h->xq, h->xstride, 0, xh);
     launch_matvec<OP_BIAS>(s, y.qkv, h->xq, h->xstride, M, h->qkv, QKV, y.bqkv, xh);
-    k_rope_rows<<<dim3(h->H + h->KVH, M), HD / 2, 0, s>>>(h->qkv, QKV, HD, h->rope, pos);
-    kv8_launch_append(bt->kv8, s, l, h->qkv + D, h->qkv + D + h->KVH * HD, Q4HIP_TYPE_F32, QKV, QKV, 0, h->KVH);
+    kv8_launch_append_rope(bt->kv8, s, l, h->qkv, QKV, h->rope, pos);
     kv8_launch_attend(bt->kv8, s, l, h->qkv, h->att, Q4HIP_TYPE_F32, QKV, D, 0.0f);
     launch_quant<QM_PLAIN>(s, M, h->att, D, D, nullptr, 0.0f, h->xq, h->xstride, 0, xh);
     launch_matvec<OP_ADD>(s, y.o, h->xq, h->xstride, M, h->x, D, nullptr, xh);
