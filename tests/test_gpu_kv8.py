@@ -111,7 +111,7 @@ class Both:
 
 # ---------------------------------------------------------------------------- plan
 
-@pytest.mark.parametrize("seqs,max_len", [(1, 1), (1, 500), (3, 64), (70, 200), (1500, 130)])
+@pytest.mark.parametrize("seqs,max_len", [(1, 1), (1, 500), (3, 64), (70, 200), (700, 90), (1024, 40), (1500, 130)])
 def test_plan_follows_the_stack(seqs, max_len):
     rng = np.random.default_rng(seqs + max_len)
     W = -(-max_len // 32)
