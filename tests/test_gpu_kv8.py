@@ -356,6 +356,38 @@ def test_fp16_tokens_are_as_good_as_their_rounding(H, KVH, hd):
     assert err < 1.1 ** 2 * rounding
 
 
+@pytest.mark.parametrize("H,KVH,hd,have,add", [(20, 20, 64, 12000, 4100), (1, 1, 64, 16000, 40)])
+def test_prompts_behind_a_long_text_are_nearly_as_good_as_their_rounding(H, KVH, hd, have, add):
+    """fp16 rows whose positions all count alike, on columns of different size, where codes cancel most.  Weights in one fp16
+    number add an error of at most 2^-11 / sqrt(3) of a weight in the root of the mean square (all of them just above a power of
+    two), as the outputs' own rounding has it: with random signs sqrt(2) to sqrt(1 + 2) of the rounding alone, whose values lie
+    anywhere between two powers (ln 2 * 3 / 2 of that square).  The fp32 sums of code + 128 over 2,048 positions add
+    sqrt(64) 2^-25 * 128 * 2048 / (sqrt(2048) * 12) of a sum of codes of 12: 1.2e-4, half of the rounding.  So below
+    sqrt(3 + 1 / 4) = 1.8; the sums over all 16,000 would be 7 to 8 times the 1.2e-4."""
+    rng = np.random.default_rng(16)
+    t = Both(H, KVH, hd, 1, have + add, 520, have + add)
+    cols = np.exp(0.5 * rng.standard_normal((1, KVH, hd))).astype(np.float32)
+    for plan in (([0], [have]), ([have], [add])):
+        t.plan(*plan)
+        shape = (len(t.slots), KVH, hd)
+        t.append(rng.standard_normal(shape).astype(np.float32), rng.standard_normal(shape).astype(np.float32) * cols, "f16")
+    w = H * hd
+    q = (0.03 * torch.randn(add, w, generator=torch.Generator().manual_seed(3))).half().cuda()
+    out = torch.zeros(add, w, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    t.kv.attend(0, q.data_ptr(), out.data_ptr(), q4hip.F16, w, w)
+    K, V = (c.values(t.pool.tables[0], have + add) for c in t.ref[0])
+    ks, vs = (c.scale_of(t.pool.tables[0], have + add) for c in t.ref[0])
+    rows, err, rounding = np.linspace(0, add - 1, 40).astype(int), 0.0, 0.0
+    y, got = q.float().cpu().numpy().reshape(add, H, hd), out.double().cpu().numpy().reshape(add, H, hd)
+    for r in rows:
+        n = have + r
+        want = kv8_ref.attend(y[r:r + 1], K[:n + 1], V[:n + 1], ks[:n + 1], vs[:n + 1], n, hd ** -0.5, HALF["f16"])[0][0]
+        err += np.square(got[r] - want).sum()
+        rounding += np.square(want.astype(np.float16).astype(np.float64) - want).sum()
+    assert err < 1.8 ** 2 * rounding
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_large_and_small_values(dtype):
     """Rows and pages of very different size: scores far apart, V scales from 1e-6 to 1e6."""
