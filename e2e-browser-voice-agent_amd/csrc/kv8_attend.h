@@ -112,7 +112,8 @@ struct Kv8Codes {
 // off by up to 2^-11.  Over 131,072 positions of similar weight that made the error of fp16 outputs 2.8e-4 where
 // their own rounding is 2.0e-4; the second number takes it back to 2.0e-4 for 1 to 5% of the time.  In a prompt,
 // whose first rows see few positions, it is 1.8 to 2.3e-4 with one number and 1.8 to 2.2e-4 with two, for 17 to 33%
-// of the time: there it is one.  In bf16 outputs, rounded by 2^-8, it does not show.
+// of the time; behind a longer text 2.6 to 3.0e-4 with one and 2.1e-4 with two, for 25 to 35%: prompts take one.  In bf16
+// outputs, rounded by 2^-8, it does not show.
 template <class T, int N>
 constexpr bool kLowWeights = sizeof(T) == 4 || (std::is_same_v<T, _Float16> && N == 1);
 
