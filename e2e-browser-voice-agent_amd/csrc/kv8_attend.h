@@ -10,13 +10,20 @@
 // row's largest contribution and no page needs a product of its own.  The tile of scores leaves the matrix cores
 // with the positions where the second product wants them (kv8.h: the order of V), so no weight changes lanes.
 //
-// fp32 rows (kTwo) hold q and w as sums of two fp16 numbers and multiply twice.  Their codes become fp16 by a byte permute
-// (0x6400 | u = 1024 + u) and one packed subtraction, exactly; v is a whole number there and the scale's rest a factor
+// w is the sum of two fp16 numbers, 22 bits, and is multiplied twice.  One number, off by up to 2^-11, adds an error of the
+// size of fp16 outputs' own rounding where many positions count alike: 3,900 fp16 rows behind 4,000 positions 3.0e-4,
+// with two 2.07e-4, which is the rounding alone (bf16 rows behind 60,000 1.69e-3 and 1.67e-3).
+// V's codes become fp16 by a byte permute (0x6400 | u = 1024 + u, u = code + 128) and one packed subtraction, exactly.  The
+// permute alone gives u * 2^-24, whose 128 the weights' sum could take back.  But the matrix instruction keeps no more of a
+// product than the largest summand's 24 bits (32 products of 2^-25 leave 1 as it is), and what is left of sums
+// of positive products after that is not exact enough: a token over 131,072 positions, columns of different size, was off by 2.7e-4 so
+// (2.8e-4 where they were taken back at every page), 2.2e-4 now, the rounding alone.
+// fp32 rows (kTwo) hold q, too, as the sum of two fp16 numbers; v is a whole number there and the scale's rest a factor
 // of w, so that 2^-v is exact.
-// 16-bit rows multiply once, but for the weights of fp16 tokens (kLowWeights).  Their codes are the fp16 numbers
-// u * 2^-24, u = code + 128: the byte permute alone.  What the 128 add to a score is subtracted by the product's first
-// addend, and what they add to O every 64 pages, by the sum of the weights, a product with a row of ones, which also gives l.  (Not of a page whose V scale is under 2^-12 of
-// an earlier one's: its weights may be too small for fp16 where its probabilities are not.)
+// 16-bit rows hold q as given.  K's codes are u * 2^-24 for them, and the product's first addend takes the 128 from the scores: the
+// same outputs' errors as with exact codes in all of the cases above, and 771 us against 818 for the 8,192 rows below.  l is the
+// sum of the fp16 weights, a product with a row of ones.  (Not of a page whose V scale is under 2^-12 of an earlier one's: its
+// weights may be too small for fp16 where its probabilities are not.)
 //
 // What bounds it.  One token of a short text: the launch and one chain of loads (5.5 us at 300 positions).  Many tokens: the
 // cache's bytes, 1.12 GB in 212 us, 5.3 TB/s (64 sequences of up to 16,000 positions, 8 kv heads of 128 columns); a 1 GiB copy
@@ -26,19 +33,18 @@
 // Not kept: raised priority around the matrix instructions (0 to 8% slower); a page's scores formed beside the weights of the page
 // before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7% slower).
 #pragma once
-#include <type_traits>
-
 #include "kv8.h"
 
 namespace q4 {
 
 using kv8_h2 = _Float16 __attribute__((ext_vector_type(2)));
+using kv8_f2 = float __attribute__((ext_vector_type(2)));
 using kv8_h8 = _Float16 __attribute__((ext_vector_type(8)));
 using kv8_f4 = float __attribute__((ext_vector_type(4)));
 
 constexpr float kKv8Lowest = -3.402823466e38f;
 
-// 8 codes (two words) as fp16: code - 128 + 128 = u as u * 2^-24, or exactly code.
+// 8 codes (two words) as fp16: u = code + 128 as u * 2^-24, or exactly code.
 template <bool kExact>
 __device__ inline kv8_h8 kv8_halves(uint32_t lo, uint32_t hi) {
   constexpr uint32_t kHigh = kExact ? 0x64646464u : 0u;
@@ -108,15 +114,6 @@ struct Kv8Codes {
   }
 };
 
-// Whether weights are sums of two fp16 numbers: of fp32 rows, and of fp16 rows by 16 (tokens).  One fp16 number is
-// off by up to 2^-11.  Over 131,072 positions of similar weight that made the error of fp16 outputs 2.8e-4 where
-// their own rounding is 2.0e-4; the second number takes it back to 2.0e-4 for 1 to 5% of the time.  In a prompt,
-// whose first rows see few positions, it is 1.8 to 2.3e-4 with one number and 1.8 to 2.2e-4 with two, for 17 to 33%
-// of the time; behind a longer text 2.6 to 3.0e-4 with one and 2.1e-4 with two, for 25 to 35%: prompts take one.  In bf16
-// outputs, rounded by 2^-8, it does not show.
-template <class T, int N>
-constexpr bool kLowWeights = sizeof(T) == 4 || (std::is_same_v<T, _Float16> && N == 1);
-
 // What the softmax needs of a page's scales.
 struct Kv8Scale {
   float k, v, iv, mant;      // K scale; v, 2^-v; the V scale over 2^v
@@ -134,12 +131,12 @@ __device__ inline Kv8Scale kv8_scale(float2 s) {
 }
 
 // 16 N rows of a wave.  Lane l: rows l % 16 of each 16, quarter l / 16 of every contraction.
-template <int HD, bool kTwo, bool kLow, int N>
+template <int HD, bool kTwo, int N>
 struct Kv8Rows {
   kv8_h8 q[N][kTwo ? 2 : 1][HD / 32];
   kv8_f4 o[N][HD / 16];
   kv8_f4 first[kTwo ? 1 : N];                     // what the 128 add to the scores, negative
-  float m[N], l[N], c[N], sum[kTwo ? 1 : N];      // c: attention scale, log2 e and the power of two that q was divided by
+  float m[N], l[N], c[N];                         // c: attention scale, log2 e and the power of two that q was divided by
 
   // The rows at row[t]; wide: 16 bytes of a row can be loaded at once.  All loads before any use: they wait for one another
   // otherwise.
@@ -196,7 +193,6 @@ struct Kv8Rows {
     if constexpr (!kTwo) {
       all = kv8_sum_quarters(all) * -0x1p-17f;                  // 128 * 2^-24
       first[t] = kv8_f4{all, all, all, all};
-      sum[t] = 0.0f;
     }
     m[t] = kKv8Lowest;
     l[t] = 0.0f;
@@ -261,7 +257,6 @@ struct Kv8Rows {
         const float m2 = __builtin_fmaxf(kv8_max_quarters(most[t]) - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
         m[t] = m2;
         l[t] *= f;
-        if constexpr (!kTwo) sum[t] *= f;
 #pragma unroll
         for (auto& y : o[t]) y *= f;
       }
@@ -274,73 +269,56 @@ struct Kv8Rows {
         l[t] = __builtin_fmaf(kv8_sum_quarters(all), sc.iv, l[t]);
       }
     const float l_scale = faint ? 0.0f : sc.iv;
-    kv8_h8 hi[N], lo[kLow ? N : 1];
+    float minus = -1.0f;
+    asm("" : "+s"(minus));        // not known to the compiler: the difference below stays one fused operation that rounds to fp16
+    kv8_h8 hi[N], lo[N];
 #pragma unroll
     for (int t = 0; t < N; t++) {
       const float v = sc.v - m[t];
       float all = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], ks[t], v));
+      for (int i = 0; i < 8; i += 2) {
+        kv8_f2 y;
+#pragma unroll
+        for (int k = 0; k < 2; k++) y[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][(i & 3) + k], ks[t], v));
         if constexpr (kTwo) {
-          all += e;
-          float y = e * sc.mant;
+          all += y[0];
+          all += y[1];
+          y *= sc.mant;
           asm("" : "+v"(y));      // rounded to fp32 here: else one of its two uses takes the product rounded to fp16 at once
-          hi[t][i] = (_Float16)y;
-          lo[t][i] = (_Float16)(y - (float)hi[t][i]);
-        } else {
-          hi[t][i] = (_Float16)e;
-          if constexpr (kLow) lo[t][i] = (_Float16)(e - (float)hi[t][i]);
+        }
+        kv8_h2 h = __builtin_convertvector(y, kv8_h2);
+        asm("" : "+v"(h));        // both by one conversion, not again one by one
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          hi[t][i + k] = h[k];
+          lo[t][i + k] = (_Float16)__builtin_fmaf((float)h[k], minus, y[k]);
         }
       }
       if constexpr (!kTwo) {
         const kv8_h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
         kv8_f4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi[t], kv8_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-        if constexpr (kLow) r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo[t], r, 0, 0, 0);
-        sum[t] += r[0];
+        r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo[t], r, 0, 0, 0);
         all = r[0];
       }
       l[t] = __builtin_fmaf(all, l_scale, l[t]);
     }
 #pragma unroll
     for (int p = 0; p < HD / 32; p++) {
-      const kv8_h8 a0 = kv8_halves<kTwo>(w.v[p].x, w.v[p].y), a1 = kv8_halves<kTwo>(w.v[p].z, w.v[p].w);
+      const kv8_h8 a0 = kv8_halves<true>(w.v[p].x, w.v[p].y), a1 = kv8_halves<true>(w.v[p].z, w.v[p].w);
 #pragma unroll
       for (int t = 0; t < N; t++) {
         o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, hi[t], o[t][2 * p], 0, 0, 0);
         o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, hi[t], o[t][2 * p + 1], 0, 0, 0);
-        if constexpr (kLow) {
-          o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo[t], o[t][2 * p], 0, 0, 0);
-          o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo[t], o[t][2 * p + 1], 0, 0, 0);
-        }
+        o[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, lo[t], o[t][2 * p], 0, 0, 0);
+        o[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, lo[t], o[t][2 * p + 1], 0, 0, 0);
       }
     }
   }
 
-  // Takes what the 128 of the codes added to o back, after at most 64 pages: o's roundings are relative to what it holds,
-  // and the 128 add up where the codes' signs cancel.  (bf16 rows at 60,000 to 80,000 positions of similar weight, error of
-  // the outputs: 2.3 to 3.8e-3 when it was taken back at the end, 1.66e-3 so, their own rounding 1.64e-3; same time.)
-  __device__ __forceinline__ void settle() {
-    if constexpr (!kTwo)
-#pragma unroll
-      for (int t = 0; t < N; t++) {
-        const float f = -0x1p-17f * sum[t];                       // 128 * 2^-24
-        sum[t] = 0.0f;
-#pragma unroll
-        for (auto& x : o[t])
-#pragma unroll
-          for (int i = 0; i < 4; i++) x[i] += f;
-      }
-  }
-
-  // The sums of the pages seen: o becomes sum w code, l the sum of all quarters.
+  // The sums of the pages seen: l becomes that of all quarters.
   __device__ void finish(int t) {
-    if constexpr (kTwo) {
-      l[t] = kv8_sum_quarters(l[t]);
-    } else {
-#pragma unroll
-      for (auto& x : o[t]) x *= 0x1p24f;
-    }
+    if constexpr (kTwo) l[t] = kv8_sum_quarters(l[t]);
   }
 
   // Pages first, first + step, ... (count of them) of a sequence's table, whose first row of this wave lies at
@@ -383,7 +361,6 @@ struct Kv8Rows {
         w.load_v(next, lane);
         top = __builtin_fmaxf(top, y.v);
       }
-      settle();
     }
   }
 };
@@ -460,13 +437,13 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,
                                          int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {
-  constexpr bool kTwo = sizeof(T) == 4, kLow = kLowWeights<T, N>;
+  constexpr bool kTwo = sizeof(T) == 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * (16 * N);
   const int rows = min(16 * N, it.n * G - r0);                  // of this tile
   if (rows <= 0) return;
-  Kv8Rows<HD, kTwo, kLow, N> w;
+  Kv8Rows<HD, kTwo, N> w;
   int row_last[N];
   const T* row[N];
 #pragma unroll
@@ -537,13 +514,13 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
 template <int HD, class T, int N>
 __device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q, T* out, int64_t q_stride, int64_t out_stride,
                                          float scale, bool wide, int tile, int g) {
-  constexpr bool kTwo = sizeof(T) == 4, kLow = kLowWeights<T, N>;
+  constexpr bool kTwo = sizeof(T) == 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const Kv8Tile it = v.tiles[tile];
   const int r0 = it.tile * kKv8TileRows + wave * (16 * N), end = it.n * G;
   if (r0 >= end) return;
-  Kv8Rows<HD, kTwo, kLow, N> w;
+  Kv8Rows<HD, kTwo, N> w;
   int last[N];
   const T* row[N];
 #pragma unroll

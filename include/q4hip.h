@@ -304,7 +304,8 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
 int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int n, float* k, float* v, void* stream);
 /* out = softmax(scale * q . K) V of the step's rows, each over the positions of its sequence up to its own: row t, head h,
  * column d at q[t * q_stride + h * head_dim + d], `out` alike; head h reads kv head h / (heads / kv_heads).
- * Scores, the softmax and the sums are fp32; `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
+ * Scores, the softmax and the sums are fp32, whatever the type and the number of rows; the matrix products take the weights, and q
+ * of F32, as sums of two fp16 numbers (22 bits); `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
  * the step's are left as they were.  q and out may be columns of the same rows, but not the same ones. */
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
