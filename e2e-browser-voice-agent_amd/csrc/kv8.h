@@ -95,8 +95,8 @@ struct Kv8View {
   Kv8Run* runs;
   Kv8Item* items;
   Kv8Tile* tiles;
-  float* part_o;       // [slots][kv_heads * row tiles][32][HD] sums of a part, relative to 2^part_ml.x
-  float2* part_ml;     // [slots][kv_heads * row tiles][32] reference exponent, sum of the probabilities
+  float* part_o;       // [slots][kv_heads * row tiles][32][HD] averages of V of a part
+  float2* part_ml;     // [slots][kv_heads * row tiles][32] reference exponent, sum of the probabilities relative to it
   int* arrived;        // [slots][kv_heads * row tiles] parts of a unit that are done (at its first slot)
   int layers, H, KVH, HD, B, W, pages, max_len;
   uint32_t g_magic;    // 2^32 / G rounded up (0 for G = 1): r / G = r * g_magic >> 32 while r * G < 2^32

@@ -5,10 +5,14 @@
 //   w   = 2^(S c + v - m)      c: K scale, attention scale, log2 e; v: log2 of the page's V scale; m: the row's
 //                    largest such sum so far, less 14
 //   O^T = V^T w      16 columns x 16 rows a tile, over the 32 positions of a page
-//   l   = sum w 2^-v
+//   l   = sum w 2^(m - v - r)
+//                    r: the row's largest score in powers of two, less 14 and at most 1 more, so that m - r is a whole number
 // The scale of V goes into the exponent, so that the weights that the matrix cores take in fp16 are relative to the
 // row's largest contribution and no page needs a product of its own.  The tile of scores leaves the matrix cores
 // with the positions where the second product wants them (kv8.h: the order of V), so no weight changes lanes.
+// l has a reference of its own, as the V scales of a sequence's pages may lie 2^221 apart: relative to 2^m, the probabilities of
+// zeros (which count as kKv8MinScale) would pass fp32 after 16,384 positions, or vanish beside a large V.  A part of a
+// sequence travels as its own average of V, which fp32 holds, with l and r.
 //
 // w is the sum of two fp16 numbers, 22 bits, and is multiplied twice.  One number, off by up to 2^-11, adds an error of the
 // size of fp16 outputs' own rounding where many positions count alike: 3,900 fp16 rows behind 4,000 positions 3.0e-4,
@@ -22,8 +26,8 @@
 // of w, so that 2^-v is exact.
 // 16-bit rows hold q as given.  K's codes are u * 2^-24 for them, and the product's first addend takes the 128 from the scores: the
 // same outputs' errors as with exact codes in all of the cases above, and 771 us against 818 for the 8,192 rows below.  l is the
-// sum of the fp16 weights, a product with a row of ones.  (Not of a page whose V scale is under 2^-12 of an earlier one's: its
-// weights may be too small for fp16 where its probabilities are not.)
+// sum of the fp16 weights, a product with a row of ones.  (Not of a faint page, whose V scale is under 2^-12 of an earlier one's, 2^-40
+// for fp32 rows: its weights may be too small where its probabilities are not.)
 //
 // What bounds it.  One token of a short text: the launch and one chain of loads (5.5 us at 300 positions).  Many tokens: the
 // cache's bytes, 1.12 GB in 212 us, 5.3 TB/s (64 sequences of up to 16,000 positions, 8 kv heads of 128 columns); a 1 GiB copy
@@ -137,6 +141,8 @@ struct Kv8Rows {
   kv8_f4 o[N][HD / 16];
   kv8_f4 first[kTwo ? 1 : N];                     // what the 128 add to the scores, negative
   float m[N], l[N], c[N];                         // c: attention scale, log2 e and the power of two that q was divided by
+  float high[N];                                  // the largest score, less 14
+  int d[N];                                       // m - r
 
   // The rows at row[t]; wide: 16 bytes of a row can be loaded at once.  All loads before any use: they wait for one another
   // otherwise.
@@ -196,6 +202,8 @@ struct Kv8Rows {
     }
     m[t] = kKv8Lowest;
     l[t] = 0.0f;
+    high[t] = kKv8Lowest;
+    d[t] = 0;
 #pragma unroll
     for (auto& x : o[t]) x = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -233,15 +241,25 @@ struct Kv8Rows {
     }
   }
 
+  // m becomes m2, after scores of up to `most`.
+  __device__ __forceinline__ void move(int t, float m2, float most) {
+    high[t] = __builtin_fmaxf(high[t], most - 14.0f);
+    const int d2 = (int)__builtin_floorf(__builtin_fminf(__builtin_fmaxf(m2 - high[t], -256.0f), 256.0f));
+    l[t] *= __builtin_amdgcn_exp2f((m[t] - m2) + (float)(d2 - d[t]));
+    m[t] = m2;
+    d[t] = d2;
+  }
+
   // One page from its scores: the number of its positions that this lane's rows look at (masked: not all rows look at
-  // all 32); faint: its weights may be too small for fp16, so that its share of l is formed in fp32.
+  // all 32); faint: its share of l is formed of its scores alone.
   __device__ __forceinline__ void page(kv8_f4 (&s)[N][2], const Kv8Codes<HD>& w, Kv8Scale sc, int quarter, bool masked,
                                        const int (&seen)[N], bool faint) {
     float ks[N], most[N];
 #pragma unroll
     for (int t = 0; t < N; t++) ks[t] = sc.k * c[t];
-    if (masked) mask(s, ks, quarter, seen);
-    bool move = false;
+    // the branches that few pages take lie behind the loop (8,192 fp32 rows 284 us, within it 287)
+    if (__builtin_expect(masked, 0)) mask(s, ks, quarter, seen);
+    bool up = false;
 #pragma unroll
     for (int t = 0; t < N; t++) {
       most[t] = s[t][0][0];
@@ -249,24 +267,24 @@ struct Kv8Rows {
       for (int i = 1; i < 8; i++) most[t] = __builtin_fmaxf(most[t], s[t][i >> 2][i & 3]);
       most[t] = __builtin_fmaf(most[t], ks[t], sc.v);
       // weights of up to 2^14, or 2^15.5 before m is moved again
-      move = move || most[t] - (kTwo ? 14.0f : 15.5f) > m[t];
+      up = up || most[t] - (kTwo ? 14.0f : 15.5f) > m[t];
     }
-    if (__builtin_amdgcn_ballot_w64(move) != 0)
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(up) != 0, 0))
 #pragma unroll
       for (int t = 0; t < N; t++) {
-        const float m2 = __builtin_fmaxf(kv8_max_quarters(most[t]) - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
-        m[t] = m2;
-        l[t] *= f;
+        const float x = kv8_max_quarters(most[t]), m2 = __builtin_fmaxf(x - 14.0f, m[t]), f = __builtin_amdgcn_exp2f(m[t] - m2);
+        move(t, m2, x - sc.v);
 #pragma unroll
         for (auto& y : o[t]) y *= f;
       }
-    if (faint)
+    if (__builtin_expect(faint, 0))
 #pragma unroll
       for (int t = 0; t < N; t++) {
+        move(t, m[t], kv8_max_quarters(most[t]) - sc.v);
         float all = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) all += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], ks[t], sc.v - m[t]));
-        l[t] = __builtin_fmaf(kv8_sum_quarters(all), sc.iv, l[t]);
+        for (int i = 0; i < 8; i++) all += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], ks[t], (float)d[t] - m[t]));
+        l[t] += kTwo ? all : kv8_sum_quarters(all);
       }
     const float l_scale = faint ? 0.0f : sc.iv;
     float minus = -1.0f;
@@ -301,7 +319,7 @@ struct Kv8Rows {
         r = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo[t], r, 0, 0, 0);
         all = r[0];
       }
-      l[t] = __builtin_fmaf(all, l_scale, l[t]);
+      l[t] = __builtin_fmaf(all, __builtin_ldexpf(l_scale, d[t]), l[t]);
     }
 #pragma unroll
     for (int p = 0; p < HD / 32; p++) {
@@ -316,10 +334,11 @@ struct Kv8Rows {
     }
   }
 
-  // The sums of the pages seen: l becomes that of all quarters.
+  // The pages seen: l becomes the sum of all quarters.
   __device__ void finish(int t) {
     if constexpr (kTwo) l[t] = kv8_sum_quarters(l[t]);
   }
+  __device__ float reference(int t) const { return m[t] - (float)d[t]; }
 
   // Pages first, first + step, ... (count of them) of a sequence's table, whose first row of this wave lies at
   // position `from`; lane's row t looks at positions up to last[t].  A page's K is loaded when the scores of the page
@@ -357,7 +376,7 @@ struct Kv8Rows {
         int seen[N];
 #pragma unroll
         for (int t = 0; t < N; t++) seen[t] = last[t] + 1 - p0;
-        page(s, w, y, quarter, p0 + kKv8Block - 1 > from, seen, !kTwo && y.v < top - 12.0f);
+        page(s, w, y, quarter, p0 + kKv8Block - 1 > from, seen, y.v < top - (kTwo ? 40.0f : 12.0f));
         w.load_v(next, lane);
         top = __builtin_fmaxf(top, y.v);
       }
@@ -365,7 +384,7 @@ struct Kv8Rows {
   }
 };
 
-// 4 columns of a row of the sums of `parts` parts at `slot`, `slot + step`, ...: o, l relative to 2^m.
+// 4 columns of a row of the average of `parts` parts at `slot`, `slot + step`, ...: o; l relative to 2^m.
 template <int HD>
 __device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int parts, int row, int d, kv8_f4& o, float& m, float& l) {
   const float* const ml = (const float*)(v.part_ml + slot * 32 + row);
@@ -385,14 +404,19 @@ __device__ inline void kv8_join(const Kv8View& v, size_t slot, size_t step, int 
     }
 #pragma unroll
     for (int k = 0; k < 8; k++) m2 = __builtin_fmaxf(m2, a[k].x);
-    const float f0 = __builtin_amdgcn_exp2f(m - m2);
-    l *= f0;
-    o *= f0;
+    const float l0 = l * __builtin_amdgcn_exp2f(m - m2);
+    l = l0;
     m = m2;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      const float f = k0 + k < parts ? __builtin_amdgcn_exp2f(a[k].x - m) : 0.0f;
-      l = __builtin_fmaf(a[k].y, f, l);
+      a[k].y *= k0 + k < parts ? __builtin_amdgcn_exp2f(a[k].x - m) : 0.0f;
+      l += a[k].y;
+    }
+    const float il = l == 0.0f ? 0.0f : 1.0f / l;
+    o *= l0 * il;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float f = a[k].y * il;
       o[0] = __builtin_fmaf(x[k][0].x, f, o[0]);
       o[1] = __builtin_fmaf(x[k][0].y, f, o[1]);
       o[2] = __builtin_fmaf(x[k][1].x, f, o[2]);
@@ -412,7 +436,7 @@ __device__ inline void kv8_send_part(const Kv8View& v, size_t slot, int row, int
 template <int HD>
 struct Kv8Shared {
   float o[4][16][HD + 4];
-  float m[4][16], l[4][16];
+  float m[4][16], r[4][16], l[4][16];
   int last;
 };
 
@@ -456,32 +480,32 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
   w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
   const int ys = v.KVH * v.row_tiles;
   const size_t slot = (size_t)max(it.slot, 0) * ys + y;         // of the unit's first part
-  auto write = [&](int row, int d, kv8_f4 o, float l) {
+  auto write = [&](int row, int d, const kv8_f4& o) {
     const int r = r0 + row, tok = kv8_div_g(v, r);
-    o *= l == 0.0f ? 0.0f : 1.0f / l;
     kv8_put4(out + (int64_t)(it.t + tok) * out_stride + (g * G + r - tok * G) * HD + d, wide, o);
   };
 #pragma unroll
   for (int t = 0; t < N; t++) {
     w.finish(t);
     __syncthreads();                         // the shared sums before have been read
-    if (quarter == 0) { sh.m[wave][n] = w.m[t]; sh.l[wave][n] = w.l[t]; }
+    if (quarter == 0) { sh.m[wave][n] = w.m[t]; sh.r[wave][n] = w.reference(t); sh.l[wave][n] = w.l[t]; }
 #pragma unroll
     for (int d = 0; d < HD / 16; d++) *(kv8_f4*)&sh.o[wave][n][d * 16 + quarter * 4] = w.o[t][d];
     __syncthreads();
     for (int e = tid; e < min(16, rows - t * 16) * (HD / 4); e += 256) {
       const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-      const float m = __builtin_fmaxf(__builtin_fmaxf(sh.m[0][row], sh.m[1][row]), __builtin_fmaxf(sh.m[2][row], sh.m[3][row]));
-      kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float r = __builtin_fmaxf(__builtin_fmaxf(sh.r[0][row], sh.r[1][row]), __builtin_fmaxf(sh.r[2][row], sh.r[3][row]));
       float l = 0.0f;
+      for (int k = 0; k < 4; k++) l = __builtin_fmaf(sh.l[k][row], __builtin_amdgcn_exp2f(sh.r[k][row] - r), l);
+      const float il = l == 0.0f ? 0.0f : 1.0f / l;
+      kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int k = 0; k < 4; k++) {
-        const float f = __builtin_amdgcn_exp2f(sh.m[k][row] - m);
-        l = __builtin_fmaf(sh.l[k][row], f, l);
+        const float f = __builtin_amdgcn_exp2f(sh.m[k][row] - r);          // f * il may be too small
         const kv8_f4 x = *(const kv8_f4*)&sh.o[k][row][d];
-        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c] * il, f, o[c]);
       }
-      if (it.parts == 1) write(t * 16 + row, d, o, l);
-      else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, m, l);
+      if (it.parts == 1) write(t * 16 + row, d, o);
+      else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, r, l);
     }
   }
   if (it.parts > 1) {
@@ -493,7 +517,7 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
         kv8_f4 o;
         float m, l;
         kv8_join<HD>(v, own, ys, mine, row, d, o, m, l);
-        if (sixteens == 1) write(row, d, o, l);
+        if (sixteens == 1) write(row, d, o);
         else kv8_send_part<HD>(v, own, row, d, o, m, l);        // over the first part: a row's threads are of one wave
       }
       if (sixteens > 1 && kv8_last(sh, v.arrived + slot + ys, sixteens))      // counted at the second part
@@ -502,7 +526,7 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
           kv8_f4 o;
           float m, l;
           kv8_join<HD>(v, slot, (size_t)16 * ys, sixteens, row, d, o, m, l);
-          write(row, d, o, l);
+          write(row, d, o);
         }
     }
   }
@@ -538,9 +562,9 @@ __device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q
     const int r = r0 + t * 16 + n, tok = kv8_div_g(v, r);
     if (r >= end) continue;
     T* const p = out + (int64_t)(it.t + tok) * out_stride + (g * G + r - tok * G) * HD + quarter * 4;
-    const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t];
+    const float il = w.l[t] == 0.0f ? 0.0f : 1.0f / w.l[t], f = __builtin_ldexpf(1.0f, w.d[t]);
 #pragma unroll
-    for (int d = 0; d < HD / 16; d++) kv8_put4(p + d * 16, wide, w.o[t][d] * il);
+    for (int d = 0; d < HD / 16; d++) kv8_put4(p + d * 16, wide, w.o[t][d] * il * f);
   }
 }
 
