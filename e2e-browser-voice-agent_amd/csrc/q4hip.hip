@@ -3390,13 +3390,14 @@ struct q4hip_batch {
   float* sc = nullptr;       // attention scores [B][heads][ctx]
   int *am_i = nullptr, *tok = nullptr, *pos = nullptr, *out = nullptr;
   int out_cap = 0;           // ints of `out`
-  int* pin = nullptr;        // pinned staging: B tokens, B positions
+  int* pin = nullptr;        // pinned staging: B tokens, B positions; B have, B add
   // a batch on the paged 8-bit cache (kc, vc and sc are null)
   q4hip_kv8* kv8 = nullptr;
   std::vector<int> len;      // positions of a sequence in the cache
   int pages = 0;
   int *have = nullptr, *add = nullptr;   // [B] positions and rows of a step; `ones`: a row of each
   int* ones = nullptr;
+  float* some = nullptr;     // [B][V] logits of a call that not all sequences take part in
   int* at = nullptr;         // [2][MT] sequences and positions to read back
 };
 
@@ -3408,6 +3409,11 @@ __global__ void k_step_of(int* have, int* add, int B, int seq, int pos, int rows
     if (b == seq) have[b] = pos;
     add[b] = b == seq ? rows : 0;
   }
+}
+
+// The next step of those that add rows.
+__global__ void k_step_on(int* have, const int* add, int B) {
+  for (int b = threadIdx.x; b < B; b += blockDim.x) have[b] += add[b];
 }
 
 // n positions from pos0 on of sequence seq.
@@ -3458,16 +3464,19 @@ void enqueue_kv8_layers(q4hip_batch* bt, int M, const int* pos) {
   }
 }
 
-// One decode step of all B sequences: tokens bt->tok at positions bt->pos; the greedy tokens go to
-// bt->tok (and out[0..B) when given) and every position advances by one, within sp.
-void enqueue_batch_step(q4hip_batch* bt, int* out, AttnSpan sp) {
+// One decode step of the B sequences that take part, all but for the 8-bit cache (whose `have` and `add` say which): tokens bt->tok
+// at positions bt->pos; the greedy tokens go to bt->tok (and out[0..B) when given) and every position advances by one, within sp.
+void enqueue_batch_step(q4hip_batch* bt, int B, int* out, AttnSpan sp) {
   q4hip* h = bt->h;
-  const int B = bt->B, D = h->D, F = h->F, HD = h->HD, QKV = h->QKV;
+  const int D = h->D, F = h->F, HD = h->HD, QKV = h->QKV;
+  const bool all = B == bt->B;
+  float* const logits = all ? bt->logits : bt->some;
   hipStream_t s = h->stream;
   uint4* xh = B > 1 ? h->xh : nullptr;
   k_embed_list<<<B, 256, 0, s>>>(h->embd, D, bt->tok, h->x);
   if (bt->kv8) {
-    kv8_launch_plan(bt->kv8, s, bt->pos, bt->ones, B, nullptr, nullptr, nullptr, nullptr);
+    kv8_launch_plan(bt->kv8, s, all ? bt->pos : bt->have, all ? bt->ones : bt->add, B, nullptr, nullptr, nullptr, nullptr);
+    if (!all) k_step_on<<<1, 256, 0, s>>>(bt->have, bt->add, bt->B);
     enqueue_kv8_layers(bt, B, bt->pos);
   }
   for (int l = 0; !bt->kv8 && l < h->NL; l++) {
@@ -3505,20 +3514,20 @@ void enqueue_batch_step(q4hip_batch* bt, int* out, AttnSpan sp) {
     const Mat& W = h->head;
     const unsigned gx = (unsigned)((W.Np + 127) / 128);
     if (B <= 4)
-      k_head_q8_rows<4><<<dim3(gx, 1), 256, (size_t)4 * W.nb * 64, s>>>(W.view(), h->xq, h->xstride, B, bt->logits, h->V);
+      k_head_q8_rows<4><<<dim3(gx, 1), 256, (size_t)4 * W.nb * 64, s>>>(W.view(), h->xq, h->xstride, B, logits, h->V);
     else if (B <= 8)
-      k_head_q8_rows<8><<<dim3(gx, 1), 256, (size_t)8 * W.nb * 64, s>>>(W.view(), h->xq, h->xstride, B, bt->logits, h->V);
+      k_head_q8_rows<8><<<dim3(gx, 1), 256, (size_t)8 * W.nb * 64, s>>>(W.view(), h->xq, h->xstride, B, logits, h->V);
     else
       k_head_q8_rows<16><<<dim3(gx, (unsigned)((B + 15) / 16)), 256, (size_t)16 * W.nb * 64, s>>>(W.view(), h->xq, h->xstride,
-                                                                                                  B, bt->logits, h->V);
+                                                                                                  B, logits, h->V);
   } else if (h->head.fmt == Q4HIP_TYPE_Q8_0) {
     for (int b = 0; b < B; b++)
       k_matvec_q8<<<(unsigned)(h->head.Np / 16), 64, (size_t)h->head.nb * 64, s>>>(
-          h->head.view(), h->xq + (size_t)b * h->xstride * 4, bt->logits + (size_t)b * h->V);
+          h->head.view(), h->xq + (size_t)b * h->xstride * 4, logits + (size_t)b * h->V);
   } else {
-    launch_matvec<OP_STORE>(s, h->head, h->xq, h->xstride, B, bt->logits, h->V, nullptr, xh);
+    launch_matvec<OP_STORE>(s, h->head, h->xq, h->xstride, B, logits, h->V, nullptr, xh);
   }
-  k_argmax_rows1<<<dim3(bt->P, B), 256, 0, s>>>(bt->logits, h->V, bt->am_v, bt->am_i, bt->P);
+  k_argmax_rows1<<<dim3(bt->P, B), 256, 0, s>>>(logits, h->V, bt->am_v, bt->am_i, bt->P);
   k_argmax_rows2<<<B, 256, 0, s>>>(bt->am_v, bt->am_i, bt->P, bt->tok, bt->pos, out);
 }
 
@@ -3530,7 +3539,7 @@ void q4hip_batch_destroy(q4hip_batch* bt) {
   (void)hipStreamSynchronize(bt->h->stream);
   q4hip_kv8_destroy(bt->kv8);
   void* bufs[] = {bt->kc, bt->vc, bt->logits, bt->am_v, bt->am_i, bt->tok, bt->pos, bt->out, bt->sc, bt->have, bt->add, bt->ones,
-                  bt->at};
+                  bt->at, bt->some};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (bt->pin) (void)hipHostFree(bt->pin);
   delete bt;
@@ -3580,7 +3589,7 @@ static int create_batch(q4hip_batch** out, q4hip* h, int B, int pages) {
     if (e == hipSuccess) e = hipMemsetAsync(bt->have, 0, (size_t)B * 4, h->stream);
     if (e == hipSuccess) e = hipMemsetD32Async((hipDeviceptr_t)bt->ones, 1, B, h->stream);
   }
-  if (e == hipSuccess) e = hipHostMalloc((void**)&bt->pin, (size_t)2 * B * 4, hipHostMallocDefault);
+  if (e == hipSuccess) e = hipHostMalloc((void**)&bt->pin, (size_t)4 * B * 4, hipHostMallocDefault);
   if (e == hipSuccess) e = hipStreamSynchronize(h->stream);   // caches zeroed before q4hip_batch_set_kv
   if (e != hipSuccess) {
     const int rc = fail(Q4HIP_EHIP, "batch of %d: %s", B, hipGetErrorString(e));
@@ -3764,20 +3773,33 @@ static int run_batch(q4hip_batch* bt, const int* first, const int* pos, int step
   q4hip* h = bt->h;
   const int B = bt->B;
   if (steps <= 0) return fail(Q4HIP_EINVAL, "steps must be positive");
+  const auto idle = [&](int b) { return bt->kv8 && pos[b] == -1; };
   for (int b = 0; b < B; b++)
-    if (pos[b] < 0 || (int64_t)pos[b] + steps >= h->ctx) return fail(Q4HIP_ECONTEXT, "context full (sequence %d)", b);
+    if (!idle(b) && (pos[b] < 0 || (int64_t)pos[b] + steps >= h->ctx)) return fail(Q4HIP_ECONTEXT, "context full (sequence %d)", b);
   int rc = check_ready(h);
   if (rc) return rc;
-  rc = check_ids(h, first, B);
+  for (int b = 0; b < B && !rc; b++)
+    if (!idle(b)) rc = check_ids(h, first + b, 1);
   if (rc) return rc;
   if (bt->kv8) {
     int64_t need = 0;
     for (int b = 0; b < B; b++) {
-      if (pos[b] > bt->len[b]) return fail(Q4HIP_EINVAL, "position %d: sequence %d holds %d", pos[b], b, bt->len[b]);
-      need += pages_of(pos[b] + steps);
+      if (!idle(b) && pos[b] > bt->len[b]) return fail(Q4HIP_EINVAL, "position %d: sequence %d holds %d", pos[b], b, bt->len[b]);
+      need += pages_of(idle(b) ? bt->len[b] : pos[b] + steps);
     }
     if (need > bt->pages) return fail(Q4HIP_ECONTEXT, "cache full: %lld pages needed, the pool has %d", (long long)need, bt->pages);
   }
+  // tokens and positions of those that take part, one after the other
+  int A = 0;
+  for (int b = 0; b < B; b++) {
+    if (!idle(b)) {
+      bt->pin[A] = first[b];
+      bt->pin[B + A++] = pos[b];
+    }
+    bt->pin[2 * B + b] = idle(b) ? bt->len[b] : pos[b];
+    bt->pin[3 * B + b] = idle(b) ? 0 : 1;
+  }
+  if (!A) return fail(Q4HIP_EINVAL, "no sequence takes part");
   HIPCHK(hipSetDevice(h->device));
   if ((int64_t)steps * B > bt->out_cap) {
     if (bt->out) HIPCHK(hipFree(bt->out));
@@ -3786,30 +3808,44 @@ static int run_batch(q4hip_batch* bt, const int* first, const int* pos, int step
     HIPCHK(hipMalloc(&bt->out, (size_t)steps * B * 4));
     bt->out_cap = steps * B;
   }
-  memcpy(bt->pin, first, (size_t)B * 4);
-  memcpy(bt->pin + B, pos, (size_t)B * 4);
-  HIPCHK(hipMemcpyAsync(bt->tok, bt->pin, (size_t)B * 4, hipMemcpyHostToDevice, h->stream));
-  HIPCHK(hipMemcpyAsync(bt->pos, bt->pin + B, (size_t)B * 4, hipMemcpyHostToDevice, h->stream));
+  if (A < B && !bt->some) HIPCHK(hipMalloc(&bt->some, (size_t)B * h->V * 4));
+  HIPCHK(hipMemcpyAsync(bt->tok, bt->pin, (size_t)A * 4, hipMemcpyHostToDevice, h->stream));
+  HIPCHK(hipMemcpyAsync(bt->pos, bt->pin + B, (size_t)A * 4, hipMemcpyHostToDevice, h->stream));
+  if (A < B) {
+    HIPCHK(hipMemcpyAsync(bt->have, bt->pin + 2 * B, (size_t)B * 4, hipMemcpyHostToDevice, h->stream));
+    HIPCHK(hipMemcpyAsync(bt->add, bt->pin + 3 * B, (size_t)B * 4, hipMemcpyHostToDevice, h->stream));
+  }
   hipEvent_t e0 = nullptr, e1 = nullptr;
   if (ms) {
     HIPCHK(hipEventCreate(&e0));
     HIPCHK(hipEventCreate(&e1));
     HIPCHK(hipEventRecord(e0, h->stream));
   }
-  const AttnSpan sp = batch_span(pos, B, h->KVH, steps);
-  for (int i = 0; i < steps; i++) enqueue_batch_step(bt, bt->out + (size_t)i * B, sp);
+  const AttnSpan sp = batch_span(bt->pin + B, A, h->KVH, steps);
+  for (int i = 0; i < steps; i++) enqueue_batch_step(bt, A, bt->out + (size_t)i * A, sp);
   if (ms) HIPCHK(hipEventRecord(e1, h->stream));
-  if (bt->kv8) HIPCHK(hipMemcpyAsync(bt->have, bt->pos, (size_t)B * 4, hipMemcpyDeviceToDevice, h->stream));
+  if (A < B) {
+    for (int b = 0, a = 0; b < B; b++)
+      if (!idle(b))
+        HIPCHK(hipMemcpyAsync(bt->logits + (size_t)b * h->V, bt->some + (size_t)a++ * h->V, (size_t)h->V * 4, hipMemcpyDeviceToDevice,
+                              h->stream));
+  } else if (bt->kv8) {
+    HIPCHK(hipMemcpyAsync(bt->have, bt->pos, (size_t)B * 4, hipMemcpyDeviceToDevice, h->stream));
+  }
   HIPCHK(hipGetLastError());
   HIPCHK(hipStreamSynchronize(h->stream));
   if (bt->kv8)
-    for (int b = 0; b < B; b++) bt->len[b] = pos[b] + steps;
+    for (int b = 0; b < B; b++)
+      if (!idle(b)) bt->len[b] = pos[b] + steps;
   if (ms) {
     HIPCHK(hipEventElapsedTime(ms, e0, e1));
     (void)hipEventDestroy(e0);
     (void)hipEventDestroy(e1);
   }
-  HIPCHK(hipMemcpy(out, bt->out, (size_t)steps * B * 4, hipMemcpyDeviceToHost));
+  HIPCHK(hipMemcpy(out, bt->out, (size_t)steps * A * 4, hipMemcpyDeviceToHost));
+  if (A < B)                                  // from the last entry on, as none moves forward
+    for (int i = steps - 1; i >= 0; i--)
+      for (int b = B - 1, a = A - 1; b >= 0; b--) out[(size_t)i * B + b] = idle(b) ? -1 : out[(size_t)i * A + a--];
   return Q4HIP_OK;
 }
 

@@ -86,6 +86,7 @@ const DECODE_NAMES = { 0: null, 1: "graph", 2: "persistent" };
 // (q4hip_batch_create_kv8 in include/q4hip.h says what differs):
 //   release(seq)   gives the sequence's pages back
 //   freePages()    pages that no sequence holds
+//   generate       a sequence with pos[b] -1 sits out, with an empty array of tokens
 // Calls on a batch and on its backend share the backend's buffers and run one at a time.
 function makeBatch(a, h, B, vocab, ctx, kv8Pages) {
   const bt = kv8Pages === undefined ? a.batchCreate(h, B) : a.batchCreate(h, B, kv8Pages);
@@ -106,8 +107,8 @@ function makeBatch(a, h, B, vocab, ctx, kv8Pages) {
       a.batchGenerate(bt, ints(first, "first"), ints(pos, "pos"), o);
       const per = [];
       for (let b = 0; b < B; b++) {
-        const t = new Array(steps);
-        for (let i = 0; i < steps; i++) t[i] = o[i * B + b];
+        const t = new Array(pos[b] === -1 ? 0 : steps);
+        for (let i = 0; i < t.length; i++) t[i] = o[i * B + b];
         per.push(t);
       }
       return per;

@@ -342,7 +342,8 @@ class Batch:
         return f, p
 
     def generate(self, first, pos, steps: int) -> np.ndarray:
-        """[steps][B] greedy tokens: row i holds every sequence's token at its position pos[b]+1+i."""
+        """[steps][B] greedy tokens: row i holds every sequence's token at its position pos[b]+1+i (-1 of one that sits out, with
+        pos[b] -1 on an 8-bit cache)."""
         f, p = self._args(first, pos)
         out = np.empty((steps, self.B), dtype=np.int32)
         _check(lib().q4hip_batch_generate(self.h, _ptr(f), _ptr(p), steps, _ptr(out)))
