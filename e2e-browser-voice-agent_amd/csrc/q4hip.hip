@@ -3616,7 +3616,8 @@ int q4hip_batch_create_kv8(q4hip_batch** out, q4hip* h, int B, int pages) {
   return create_batch(out, h, B, pages);
 }
 
-// K and V rows of positions from pos0 on of one kv head.
+// K and V rows of positions from pos0 on of one kv head.  Positions that the sequence did not hold are zeros in the other layers
+// and heads until they are written, as in the other caches (a page may come from another sequence).
 static int set_kv8(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, int n, const float* k, const float* v) {
   q4hip* h = bt->h;
   const int HD = h->HD;
@@ -3629,10 +3630,17 @@ static int set_kv8(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, i
   // all at once: a step that ended before the sequence does would give its last pages back
   float* rows = nullptr;
   const size_t bytes = (size_t)n * HD * 4;
-  HIPCHK(hipMalloc(&rows, 2 * bytes));
+  const int fresh = pos0 + n - bt->len[seq];
+  HIPCHK(hipMalloc(&rows, 2 * bytes + (size_t)h->KVH * HD * 4));
+  float* const zeros = rows + (size_t)2 * n * HD;
   hipError_t e = hipMemcpyAsync(rows, k, bytes, hipMemcpyHostToDevice, h->stream);
   if (e == hipSuccess) e = hipMemcpyAsync(rows + (size_t)n * HD, v, bytes, hipMemcpyHostToDevice, h->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(zeros, 0, (size_t)h->KVH * HD * 4, h->stream);
   if (e == hipSuccess) {
+    if (fresh) {
+      plan_of(bt, seq, bt->len[seq], fresh);
+      for (int l = 0; l < h->NL; l++) kv8_launch_append(bt->kv8, h->stream, l, zeros, zeros, Q4HIP_TYPE_F32, 0, 0, 0, h->KVH);
+    }
     plan_of(bt, seq, pos0, n);
     kv8_launch_append(bt->kv8, h->stream, layer, rows, rows + (size_t)n * HD, Q4HIP_TYPE_F32, HD, HD, kv_head, 1);
     k_step_of<<<1, 256, 0, h->stream>>>(bt->have, bt->add, bt->B, seq, pos0 + n, 0);

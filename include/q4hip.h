@@ -208,7 +208,7 @@ int q4hip_batch_read_logits(q4hip_batch* bt, float* out, int64_t n);
  * cut into passes at other positions); a call that needs more pages than the pool has fails with Q4HIP_ECONTEXT before anything
  * runs; positions are written in order: `pos` (pos0 of q4hip_batch_set_kv) is at most the number of positions that the
  * sequence holds, and afterwards it ends with the call's last position (q4hip_batch_set_kv refuses one
- * before its end); a sequence whose pos[b] is -1 sits q4hip_batch_generate and q4hip_batch_time_generate out: first[b] is not looked
+ * before its end, and positions that it adds are zeros in the other layers and kv heads until they are set, too); a sequence whose pos[b] is -1 sits q4hip_batch_generate and q4hip_batch_time_generate out: first[b] is not looked
  * at, its cache and logits stay as they are, and its tokens in `out` are -1 (Q4HIP_EINVAL if all of them do); any number of query
  * heads per kv head and any ctx of the context. */
 int q4hip_batch_create_kv8(q4hip_batch** out, q4hip* h, int B, int pages);

@@ -141,3 +141,43 @@ def test_through_napi(tmp_path):
     assert out == {"first": first, "tokens": [[], bt.generate([first], [9], 8)[:, 0].tolist()], "free": 3}
     bt.close()
     g.close()
+
+
+@pytest.mark.parametrize("first,then", [(70, 40), (64, 3), (5, 1)])
+def test_positions_that_no_row_has_reached_are_zeros(first, then):
+    """set_kv of one layer and head on pages that another sequence has held: zeros in all others, until they are set; what the
+    head itself holds is as without them."""
+    import kv8_ref
+    shape, t, g = model("small", 3, 150)
+    rng = np.random.default_rng(4)
+    n = first + then
+    K, V = rng.standard_normal((2, n, shape.head_dim), dtype=np.float32)
+    bt = q4hip.Batch(g, 2, kv8_pages=-(-n // 32))
+    try:
+        bt.prefill(0, rng.integers(0, shape.vocab, n).astype(np.int32), 0)
+        bt.release(0)
+        last, head = shape.layers - 1, shape.kv_heads - 1
+        ref = [kv8_ref.Cache(-(-n // 32), 1, shape.head_dim) for _ in range(2)]
+        table = list(range(-(-n // 32)))
+        for a, b in ((0, first), (first, n)):
+            bt.set_kv(1, last, head, a, K[a:b], V[a:b])
+            for l in range(shape.layers):
+                for h in range(shape.kv_heads):
+                    k, v = bt.get_kv(1, l, h, 0, b)
+                    if (l, h) != (last, head):
+                        assert (k == 0).all() and (v == 0).all(), (l, h)
+            for c, x in zip(ref, (K, V)):
+                c.append(x[a:b, None], np.arange(a, b))
+            k, v = bt.get_kv(1, last, head, 0, b)
+            assert np.array_equal(k, ref[0].values(table, b)[:, 0]) and np.array_equal(v, ref[1].values(table, b)[:, 0])
+        # the others afterwards, up to the end
+        bt.set_kv(1, 0, 0, first, K[first:], V[first:])
+        k, _ = bt.get_kv(1, 0, 0, 0, n)
+        assert (k[:first] == 0).all()
+        step = np.abs(K[first:]).max() / 127
+        assert (np.abs(k[first:] - K[first:]) <= step).all()
+        k, _ = bt.get_kv(1, last, head, 0, n)
+        assert np.array_equal(k, ref[0].values(table, n)[:, 0])
+    finally:
+        bt.close()
+        g.close()
