@@ -295,10 +295,10 @@ class Batch:
     kv8_pages pages of an 8-bit one (q4hip_batch_create_kv8).
     Holds a reference to the model; close the batch before closing the model explicitly."""
 
-    def __init__(self, model: Model, B: int, kv8_pages: int = 0):
+    def __init__(self, model: Model, B: int, kv8_pages: int | None = None):
         self.model, self.B = model, B
         h = ctypes.c_void_p()
-        if kv8_pages:
+        if kv8_pages is not None:
             _check(lib().q4hip_batch_create_kv8(ctypes.byref(h), model.h, B, kv8_pages))
         else:
             _check(lib().q4hip_batch_create(ctypes.byref(h), model.h, B))

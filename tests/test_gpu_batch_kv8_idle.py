@@ -181,3 +181,17 @@ def test_positions_that_no_row_has_reached_are_zeros(first, then):
     finally:
         bt.close()
         g.close()
+
+
+def test_a_pool_of_no_pages_is_refused():
+    shape, t, g = model("tiny", 4, 96)
+    try:
+        with pytest.raises(q4hip.Q4Error) as e:
+            q4hip.Batch(g, 1, kv8_pages=0)
+        assert e.value.code == q4hip.EINVAL
+        bt = q4hip.Batch(g, 1, kv8_pages=None)
+        with pytest.raises(q4hip.Q4Error):
+            bt.free_pages()
+        bt.close()
+    finally:
+        g.close()
