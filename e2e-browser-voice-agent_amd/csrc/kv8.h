@@ -111,23 +111,26 @@ struct Kv8View {
 struct q4hip_kv8 {
   q4::Kv8View v{};
   int device = 0, max_rows = 0;
-  int rows = 0;                // rows the last plan was called for
+  int rows = 0;                // rows the last plan was called for, outside of captures
+  unsigned long long capture = 0;   // the last capture of a plan, and the rows of that
+  int capture_rows = 0;
   hipStream_t stream = nullptr;
   q4::Kv8Head* pin = nullptr;  // pinned copy of v.head
 };
 
 namespace q4 {
 
-// The operators' launches without the checks of their arguments (include/q4hip.h); q and out, k and v of `type`.
+// The operators' launches without the checks of their arguments (include/q4hip.h); q and out, k and v of `type`; rows: of the plan.
 void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
                      int* tables);
 // heads [g0, g0 + heads) of the cache from heads 0.. of the rows
 void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
-                       int64_t v_stride, int g0, int heads);
+                       int64_t v_stride, int g0, int heads, int rows);
 // Rows of q|k|v that begin at multiples of 16 bytes: q turned in place, k and v into the cache, k turned on its way.
-void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos);
+void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos,
+                            int rows);
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
-                       int64_t out_stride, float scale);
+                       int64_t out_stride, float scale, int rows);
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v);
 
 }  // namespace q4

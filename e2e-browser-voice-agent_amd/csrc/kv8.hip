@@ -288,9 +288,25 @@ int plan_error(const q4hip_kv8* kv, int status) {
     case KV8_TOO_LONG: return fail(Q4HIP_ECONTEXT, "plan: a sequence longer than %d positions", kv->v.max_len);
     case KV8_STALE:
       return fail(Q4HIP_ESTATE, "append or attend replayed on a plan of more rows than they were captured for");
-    case KV8_ROWS: return fail(Q4HIP_EINVAL, "plan: more rows than the %d it was called for", kv->rows);
+    case KV8_ROWS: return fail(Q4HIP_EINVAL, "plan: more rows than it was called for");
     default: return fail(Q4HIP_ECONTEXT, "plan: more than the pool's %d pages", kv->v.pages);
   }
+}
+
+// The capture that `s` is in, 0 for none.
+int capture_of(hipStream_t s, unsigned long long* id) {
+  hipStreamCaptureStatus st;
+  HIPCHK(hipStreamGetCaptureInfo(s, &st, id));
+  if (st == hipStreamCaptureStatusNone) *id = 0;
+  return Q4HIP_OK;
+}
+
+// Rows of the plan that a call on `s` follows: the one captured before it in the same capture, else the last one outside of any.
+int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
+  unsigned long long id;
+  const int rc = capture_of(s, &id);
+  *rows = id && id == kv->capture ? kv->capture_rows : kv->rows;
+  return rc;
 }
 
 int read_head(q4hip_kv8* kv, hipStream_t s) {
@@ -311,7 +327,6 @@ void by_type(int type, F f) {
 void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
                      int* tables) {
   const Kv8View& v = kv->v;
-  kv->rows = rows;
   // What the lists hold in all: in the same launch if the one workgroup is through with it in a few rounds, which takes less
   // than a second launch does.
   const size_t items = rows + std::min<size_t>(kKv8MoreItems * v.items_aim, rows ? (size_t)v.pages * rows / kKv8MinPart : 0);
@@ -329,52 +344,53 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
 namespace {
 
 // runs of a sequence: its rows over 32, and two at its ends
-unsigned runs_bound(const q4hip_kv8* kv) {
-  return (unsigned)std::min<int64_t>(kv->rows, kv->rows / kKv8Block + 2 * (int64_t)std::min(kv->v.B, kv->rows));
+unsigned runs_bound(const Kv8View& v, int rows) {
+  return (unsigned)std::min<int64_t>(rows, rows / kKv8Block + 2 * (int64_t)std::min(v.B, rows));
 }
 
 }  // namespace
 
 void kv8_launch_append(q4hip_kv8* kv, hipStream_t s, int layer, const void* k, const void* v, int type, int64_t k_stride,
-                       int64_t v_stride, int g0, int heads) {
+                       int64_t v_stride, int g0, int heads, int rows) {
   const Kv8View& w = kv->v;
-  if (!kv->rows) return;
-  const dim3 grid(runs_bound(kv), (unsigned)heads, 2);
+  if (!rows) return;
+  const dim3 grid(runs_bound(w, rows), (unsigned)heads, 2);
   const bool wide = aligned16(k, k_stride, type) && aligned16(v, v_stride, type);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     auto* fn = w.HD == 64 ? (wide ? k_kv8_append<64, T, true, false> : k_kv8_append<64, T, false, false>)
                           : (wide ? k_kv8_append<128, T, true, false> : k_kv8_append<128, T, false, false>);
-    fn<<<grid, 2 * w.HD, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, kv->rows, g0, Kv8Rope{});
+    fn<<<grid, 2 * w.HD, 0, s>>>(w, layer, (const T*)k, (const T*)v, k_stride, v_stride, rows, g0, Kv8Rope{});
   });
 }
 
-void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos) {
+void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv, int64_t stride, const float* table, const int* pos,
+                            int rows) {
   const Kv8View& w = kv->v;
-  if (!kv->rows) return;
+  if (!rows) return;
   const float *const k = qkv + w.H * w.HD, *const v = k + w.KVH * w.HD;
   auto* fn = w.HD == 64 ? k_kv8_append<64, float, true, true> : k_kv8_append<128, float, true, true>;
-  fn<<<dim3(runs_bound(kv), (unsigned)w.KVH, 3), 2 * w.HD, 0, s>>>(w, layer, k, v, stride, stride, kv->rows, 0,
+  fn<<<dim3(runs_bound(w, rows), (unsigned)w.KVH, 3), 2 * w.HD, 0, s>>>(w, layer, k, v, stride, stride, rows, 0,
                                                                   Kv8Rope{table, pos, qkv, stride});
 }
 
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
-                       int64_t out_stride, float scale) {
+                       int64_t out_stride, float scale, int rows) {
   const Kv8View& w = kv->v;
-  if (!kv->rows) return;
+  if (!rows) return;
   // the softmax's exponentials are powers of two
   const float log2_scale = (float)((scale == 0.0f ? 1.0 / std::sqrt((double)w.HD) : (double)scale) * 1.4426950408889634);
-  const int units = (int)std::min<int64_t>(kv->rows, kv->rows / w.unit_rows + (int64_t)std::min(w.B, kv->rows));
+  const int units = (int)std::min<int64_t>(rows, rows / w.unit_rows + (int64_t)std::min(w.B, rows));
   const int64_t items = units + std::min<int64_t>(kKv8MoreItems * w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
   const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
-  const bool few = kv->rows <= w.unit_rows;    // neither wide units nor tiles
-  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, kv->rows) * w.KVH);
+  const bool few = rows <= w.unit_rows;    // neither wide units nor tiles
+  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, rows) * w.KVH);
   const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
                           : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, kv->rows, wide);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide);
   });
 }
 
@@ -493,10 +509,19 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
     if (rc) return rc;
   }
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  unsigned long long id;
+  int rc = capture_of(s, &id);
+  if (rc) return rc;
   kv8_launch_plan(kv, s, have, add, rows, starts, positions, slots, tables);
   HIPCHK(hipGetLastError());
+  if (id) {
+    kv->capture = id;
+    kv->capture_rows = rows;
+  } else {
+    kv->rows = rows;
+  }
   if (stream) return Q4HIP_OK;
-  const int rc = read_head(kv, s);
+  rc = read_head(kv, s);
   return rc ? rc : plan_error(kv, kv->pin->status);
 }
 
@@ -515,14 +540,16 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   if (!kv || !k || !v) return fail(Q4HIP_EINVAL, "null argument");
   int rc = check_layer(kv, layer, type);
   if (rc) return rc;
-  if (!kv->rows) return Q4HIP_OK;
   HIPCHK(hipSetDevice(kv->device));
-  const Kv8View& w = kv->v;
-  rc = check_rows(kv, k, kv->rows, w.KVH * w.HD, k_stride, type, "k");
-  if (!rc) rc = check_rows(kv, v, kv->rows, w.KVH * w.HD, v_stride, type, "v");
-  if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  kv8_launch_append(kv, s, layer, k, v, type, k_stride, v_stride, 0, w.KVH);
+  int rows;
+  rc = rows_on(kv, s, &rows);
+  if (rc || !rows) return rc;
+  const Kv8View& w = kv->v;
+  rc = check_rows(kv, k, rows, w.KVH * w.HD, k_stride, type, "k");
+  if (!rc) rc = check_rows(kv, v, rows, w.KVH * w.HD, v_stride, type, "v");
+  if (rc) return rc;
+  kv8_launch_append(kv, s, layer, k, v, type, k_stride, v_stride, 0, w.KVH, rows);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;
@@ -555,15 +582,17 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   int rc = check_layer(kv, layer, type);
   if (rc) return rc;
   if (!std::isfinite(scale) || scale < 0.0f) return fail(Q4HIP_EINVAL, "scale %g", (double)scale);
-  if (!kv->rows) return Q4HIP_OK;
   HIPCHK(hipSetDevice(kv->device));
-  const Kv8View& w = kv->v;
-  rc = check_rows(kv, q, kv->rows, w.H * w.HD, q_stride, type, "q");
-  if (!rc) rc = check_rows(kv, out, kv->rows, w.H * w.HD, out_stride, type, "out");
-  if (!rc) rc = check_apart(q, q_stride, out, out_stride, kv->rows, w.H * w.HD, type);
-  if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
-  kv8_launch_attend(kv, s, layer, q, out, type, q_stride, out_stride, scale);
+  int rows;
+  rc = rows_on(kv, s, &rows);
+  if (rc || !rows) return rc;
+  const Kv8View& w = kv->v;
+  rc = check_rows(kv, q, rows, w.H * w.HD, q_stride, type, "q");
+  if (!rc) rc = check_rows(kv, out, rows, w.H * w.HD, out_stride, type, "out");
+  if (!rc) rc = check_apart(q, q_stride, out, out_stride, rows, w.H * w.HD, type);
+  if (rc) return rc;
+  kv8_launch_attend(kv, s, layer, q, out, type, q_stride, out_stride, scale, rows);
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;

@@ -3448,8 +3448,8 @@ void enqueue_kv8_layers(q4hip_batch* bt, int M, const int* pos) {
     Layer& y = h->L[l];
     launch_quant<QM_NORM>(s, M, h->x, D, D, y.attn_norm, h->eps, h->xq, h->xstride, 0, xh);
     launch_matvec<OP_BIAS>(s, y.qkv, h->xq, h->xstride, M, h->qkv, QKV, y.bqkv, xh);
-    kv8_launch_append_rope(bt->kv8, s, l, h->qkv, QKV, h->rope, pos);
-    kv8_launch_attend(bt->kv8, s, l, h->qkv, h->att, Q4HIP_TYPE_F32, QKV, D, 0.0f);
+    kv8_launch_append_rope(bt->kv8, s, l, h->qkv, QKV, h->rope, pos, M);
+    kv8_launch_attend(bt->kv8, s, l, h->qkv, h->att, Q4HIP_TYPE_F32, QKV, D, 0.0f, M);
     launch_quant<QM_PLAIN>(s, M, h->att, D, D, nullptr, 0.0f, h->xq, h->xstride, 0, xh);
     launch_matvec<OP_ADD>(s, y.o, h->xq, h->xstride, M, h->x, D, nullptr, xh);
     launch_quant<QM_NORM>(s, M, h->x, D, D, y.ffn_norm, h->eps, h->xq, h->xstride, 0, xh);
@@ -3639,10 +3639,10 @@ static int set_kv8(q4hip_batch* bt, int seq, int layer, int kv_head, int pos0, i
   if (e == hipSuccess) {
     if (fresh) {
       plan_of(bt, seq, bt->len[seq], fresh);
-      for (int l = 0; l < h->NL; l++) kv8_launch_append(bt->kv8, h->stream, l, zeros, zeros, Q4HIP_TYPE_F32, 0, 0, 0, h->KVH);
+      for (int l = 0; l < h->NL; l++) kv8_launch_append(bt->kv8, h->stream, l, zeros, zeros, Q4HIP_TYPE_F32, 0, 0, 0, h->KVH, fresh);
     }
     plan_of(bt, seq, pos0, n);
-    kv8_launch_append(bt->kv8, h->stream, layer, rows, rows + (size_t)n * HD, Q4HIP_TYPE_F32, HD, HD, kv_head, 1);
+    kv8_launch_append(bt->kv8, h->stream, layer, rows, rows + (size_t)n * HD, Q4HIP_TYPE_F32, HD, HD, kv_head, 1, n);
     k_step_of<<<1, 256, 0, h->stream>>>(bt->have, bt->add, bt->B, seq, pos0 + n, 0);
     e = hipGetLastError();
   }

@@ -266,7 +266,9 @@ int q4hip_mv_run_noalloc(q4hip_mv* m, const float* x, float* y, void* stream);
  * checked, with the bytes behind them, before anything is launched.  Calls on one handle are serialized by the
  * caller, also on the GPU: calls on several streams, or graphs that hold them, are ordered by events or waits.
  * Handles are independent.  A captured append or attend serves plans of up to the `rows` of the plan that it was
- * captured after; replayed on a larger one it does nothing, and q4hip_kv8_status returns Q4HIP_ESTATE. */
+ * captured after, the one in the same capture or, if there is none, the last one outside of any; replayed on a larger one it does
+ * nothing, and q4hip_kv8_status returns Q4HIP_ESTATE.  One that is not captured follows the last plan that was not
+ * (after a replay of a graph with a plan of more rows, plan again). */
 typedef struct q4hip_kv8 q4hip_kv8;
 #define Q4HIP_KV8_BLOCK 32
 /* A cache of `pages` pages for `seqs` sequences of up to max_len positions; plans hold up to max_rows
