@@ -19,14 +19,14 @@ namespace q4 {
 constexpr int kKv8Block = 32;
 // A unit of more than kKv8Whole pages is shared among several workgroups, in parts of at least kKv8MinPart pages and, while
 // that leaves no more than kKv8MoreItems times the items aimed at, at most kKv8MaxPart.  One token (14 heads, 2 kv heads of
-// 64 columns): 300 positions whole 6.0 us, in parts 7.2; 1,000 positions whole 8.4, in parts of 8 pages 7.4.  64
-// sequences of up to 16,000 positions: parts of at most 128 pages 196 us, as long as the aim asks 209.
+// 64 columns): 300 positions whole 6.0 us, in parts 7.4; 1,000 positions whole 8.7, in parts of 8 pages 7.6.  64
+// sequences of up to 16,000 positions: parts of at most 128 pages 225 us, as long as the aim asks 245.
 constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups; else in units, whose pages can be shared.  Tiles and units, us: 2,048 rows of 14 heads (fp32)
-// 57 and 42, 8,192 rows 288 and 372; of 32 heads (bf16) 65 and 72, 546 and 626; of 8 heads of one kv head (bf16) 51 and 26, 189
-// and 175; a step of 4 prompts and 44 tokens, 20 kv heads, 52 and 59.
+// 57 and 42, 8,192 rows 283 and 370; of 32 heads (bf16) 83 and 84, 773 and 860; of 8 heads of one kv head (bf16) 65 and 32, 262
+// and 237; a step of 4 prompts and 44 tokens, 20 kv heads, 78 and 87.
 constexpr int kKv8MinTiles = 640;
 constexpr float kKv8MinScale = 0x1p-100f;     // a smaller scale is 0, and so are the values
 

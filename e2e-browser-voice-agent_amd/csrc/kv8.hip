@@ -18,8 +18,8 @@ constexpr int kItemsAim = 256;
 // launch against two: 200 sequences with tables, 6,400 entries, 9.0 us and 11.1; 48 with 2,171 rows 7.2 and 8.4) and in
 // global memory (6,000 sequences 63 us and 38).
 constexpr size_t kFillInPlan = 8192, kFillInPlanGlobal = 2048;
-// Workgroups of attention at most; each takes every so-manieth tile or item.  (1,024 to 8,192: the same times; 512: up to 20%
-// more, as the tiles of a step differ in length.)
+// Workgroups of attention at most; each takes every so-manieth tile or item.  (1,024: up to 9% more time, 512: up to 35%, as the
+// tiles of a step differ in length.)
 constexpr int64_t kMostWorkgroups = 8192;
 
 // The quotient x / s rounded to fp32, from r = 1 / s rounded: one correction of x * r by its residual gives it

@@ -20,22 +20,25 @@
 // V's codes become fp16 by a byte permute (0x6400 | u = 1024 + u, u = code + 128) and one packed subtraction, exactly.  The
 // permute alone gives u * 2^-24, whose 128 the weights' sum could take back.  But the matrix instruction keeps no more of a
 // product than the largest summand's 24 bits (32 products of 2^-25 leave 1 as it is), and what is left of sums
-// of positive products after that is not exact enough: a token over 131,072 positions, columns of different size, was off by 2.7e-4 so
-// (2.8e-4 where they were taken back at every page), 2.2e-4 now, the rounding alone.
+// of positive products after that is not exact enough: a token over 131,072 positions, columns of different size, was off by
+// 2.7e-4 so (2.8e-4 where they were taken back at every page), 2.2e-4 now, the rounding alone.
 // fp32 rows (kTwo) hold q, too, as the sum of two fp16 numbers; v is a whole number there and the scale's rest a factor
 // of w, so that 2^-v is exact.
 // 16-bit rows hold q as given.  K's codes are u * 2^-24 for them, and the product's first addend takes the 128 from the scores: the
-// same outputs' errors as with exact codes in all of the cases above, and 771 us against 818 for the 8,192 rows below.  l is the
-// sum of the fp16 weights, a product with a row of ones.  (Not of a faint page, whose V scale is under 2^-12 of an earlier one's, 2^-40
-// for fp32 rows: its weights may be too small where its probabilities are not.)
+// same outputs' errors as with exact codes in all of the cases above, and 775 us against 821 for the 8,192 rows below, 79 and
+// 91 for a step of 4 prompts and 44 tokens (20 kv heads of 64; 32 tokens at 1,024 positions, though, 23 and 19).  l is the sum of the
+// fp16 weights, a product with a row of ones.  (Not of a faint page, whose V scale is under 2^-12 of an earlier one's, 2^-40 for
+// fp32 rows: its weights may be too small where its probabilities are not.)
 //
-// What bounds it.  One token of a short text: the launch and one chain of loads (5.5 us at 300 positions).  Many tokens: the
-// cache's bytes, 1.12 GB in 212 us, 5.3 TB/s (64 sequences of up to 16,000 positions, 8 kv heads of 128 columns); a 1 GiB copy
-// moves 5.15.  Prompts: the vector instructions that turn codes into fp16 (64 of some 150 for a page and 32 rows), form the
-// exponentials (16, at a quarter of the rate) and find the largest, 67% of the issue slots, beside matrix instructions that are
-// busy 45% of the time: 8,192 bf16 rows, 32 heads of 128, in 577 us, 953 TFLOP/s; a large bf16 product reaches 1,221.
-// Not kept: raised priority around the matrix instructions (0 to 8% slower); a page's scores formed beside the weights of the page
-// before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7% slower).
+// What bounds it.  One token of a short text: the launch and one chain of loads (5.8 us at 300 positions).  Many tokens: the
+// cache's bytes, 1.12 GB in 216 us, 5.2 TB/s (64 sequences of up to 16,000 positions, 8 kv heads of 128 columns); a 1 GiB copy
+// moves 5.15.  Prompts: the vector instructions that turn codes into fp16 (96 of some 220 for a page and 32 rows), split the
+// weights (24), form the exponentials (16, at a quarter of the rate) and find the largest, 68% of the issue slots, beside matrix
+// instructions that are busy 51% of the time: 8,192 bf16 rows, 32 heads of 128, in 772 us, 712 TFLOP/s; a large bf16 product
+// reaches 1,221.
+// Not kept, while weights were one fp16 number: raised priority around the matrix instructions (0 to 8% slower); a page's scores
+// formed beside the weights of the page before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7%
+// slower).
 #pragma once
 #include "kv8.h"
 
@@ -454,7 +457,7 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
 }
 
 // An item of the plan and 16 N of its unit's rows of a kv head (y).  Waves share the pages and not the rows, as a token has
-// few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 13.8 us.
+// few rows and the loads of four waves are in flight at once; 131,072 positions of one sequence, in parts, 14.5 us.
 // The four waves take every fourth page each and add up their sums in shared memory, 16 rows at a time.  A unit in
 // several parts: the last workgroup of each 16 parts to be done adds those up, and the last of these the sums of 16, always
 // in the order of the parts.

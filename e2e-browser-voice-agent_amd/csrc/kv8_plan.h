@@ -5,7 +5,9 @@
 // long sequence alone, and the lists can be spread over the GPU where there is much of them.
 // Nothing but latency bounds it: a chain of loads, sums and bisections, and the fetches of code that runs once.  So
 // the code is short (a thread forms its sequence's numbers, then a wave takes each sum), sums over a wave stay in
-// registers, those over up to kPlanShared sequences in shared memory, and all lists are filled in one loop.  A launch with
+// registers, those over up to kPlanShared sequences in shared memory, and all lists are filled in one loop.  (Which of the ten
+// arrays a wave takes is chosen as it runs: the compiler keeps their addresses in 88 bytes of scratch memory a lane, and
+// reaches the arrays by flat accesses.)  A launch with
 // all of the caller's arrays: 32 sequences 6.6 us, 48 with 2,171 rows 9.8, 1,024 with 15,454 rows 15.6 (two launches); with
 // every sum unrolled through shared memory 7.7, 15.8 and 24.
 #pragma once

@@ -207,10 +207,11 @@ int q4hip_batch_read_logits(q4hip_batch* bt, float* out, int64_t n);
  * reference's order of operations: results are close to, not equal to those of the other caches, and of a prompt
  * cut into passes at other positions); a call that needs more pages than the pool has fails with Q4HIP_ECONTEXT before anything
  * runs; positions are written in order: `pos` (pos0 of q4hip_batch_set_kv) is at most the number of positions that the
- * sequence holds, and afterwards it ends with the call's last position (q4hip_batch_set_kv refuses one
- * before its end, and positions that it adds are zeros in the other layers and kv heads until they are set, too); a sequence whose pos[b] is -1 sits q4hip_batch_generate and q4hip_batch_time_generate out: first[b] is not looked
- * at, its cache and logits stay as they are, and its tokens in `out` are -1 (Q4HIP_EINVAL if all of them do); any number of query
- * heads per kv head and any ctx of the context. */
+ * sequence holds, and afterwards it ends with the call's last position (q4hip_batch_set_kv refuses one before its end, and
+ * positions that it adds are zeros in the other layers and kv heads until they are set, too); a sequence whose pos[b] is -1
+ * sits q4hip_batch_generate and q4hip_batch_time_generate out: first[b] is not looked at, its cache and logits stay as they
+ * are, and its tokens in `out` are -1 (Q4HIP_EINVAL if all of them do); any number of query heads per kv head and any ctx of
+ * the context. */
 int q4hip_batch_create_kv8(q4hip_batch** out, q4hip* h, int B, int pages);
 /* Give a sequence's pages back (8-bit cache): it holds no position afterwards. */
 int q4hip_batch_release(q4hip_batch* bt, int seq);
@@ -280,7 +281,8 @@ void q4hip_kv8_destroy(q4hip_kv8* kv);
  * Afterwards every sequence has exactly the ceil((have + add) / 32) pages that it needs: one that needs
  * fewer than it had gives the rest back (0 and 0: all of them), then those that lack some take them from
  * the pool.  Positions from have[b] on are written by the step; have[b] may be less than the sequence held
- * (a chat cut back).  The same plan again changes nothing.  `rows` is at least the sum of add; the
+ * (a chat cut back).  What a page held for another sequence, or a longer one, stays in it until it is written: a step
+ * appends its rows in every layer that reads them.  The same plan again changes nothing.  `rows` is at least the sum of add; the
  * rows of the step lie one sequence after the other.  Device arrays that are not NULL receive
  *   starts[seqs + 1]   the first row of each sequence, and the number of rows
  *   positions[rows]    a row's position in its sequence
