@@ -16,7 +16,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "lib")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-SOURCES = ["q4hip.hip", "kv8.hip"]
+SOURCES = ["q4hip.hip", "kv8.hip", "rope.hip", "logits.hip"]
 NODE_INCLUDE = os.environ.get("NODE_INCLUDE", "/usr/include/node")
 
 # -ffp-contract=off: no multiply-add fusion, so every binary32 operation rounds once as on the CPU.

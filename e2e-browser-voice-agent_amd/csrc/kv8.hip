@@ -8,6 +8,7 @@
 #include "host.h"
 #include "kv8_attend.h"
 #include "kv8_plan.h"
+#include "rows.h"
 
 namespace q4 {
 namespace {
@@ -237,48 +238,9 @@ size_t tiles_bound(const Kv8View& v, int rows) {
   return (size_t)((int64_t)rows * (v.H / v.KVH) / kKv8TileRows + std::min(v.B, rows / (v.unit_rows + 1)) + 1);
 }
 
-int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
-
-// Whether 16 bytes of any row can be loaded at once.
-bool aligned16(const void* p, int64_t stride, int type) {
-  return ((uintptr_t)p | (uintptr_t)(stride * elem_size(type))) % 16 == 0;
-}
-
 int check_layer(const q4hip_kv8* kv, int layer, int type) {
   if (layer < 0 || layer >= kv->v.layers) return fail(Q4HIP_EINVAL, "layer %d of %d", layer, kv->v.layers);
-  if (type != Q4HIP_TYPE_F32 && type != Q4HIP_TYPE_F16 && type != Q4HIP_TYPE_BF16)
-    return fail(Q4HIP_ETYPE, "type %d: expected F32, F16 or BF16", type);
-  return Q4HIP_OK;
-}
-
-// `rows` rows of `width` elements, `stride` elements apart.
-int check_rows(const q4hip_kv8* kv, const void* p, int rows, int width, int64_t stride, int type, const char* what) {
-  const int es = elem_size(type);
-  if ((uintptr_t)p % es) return fail(Q4HIP_EINVAL, "%s: not aligned to its type", what);
-  if (stride < width) return fail(Q4HIP_EINVAL, "%s: rows of %d values, %lld apart", what, width, (long long)stride);
-  if (stride > ((int64_t)1 << 31)) return fail(Q4HIP_EINVAL, "%s: rows %lld values apart", what, (long long)stride);
-  return check_device_span(p, ((size_t)(rows - 1) * stride + width) * es, kv->device, what);
-}
-
-// Rows that one call reads and another buffer's that it writes must not share a byte.  Neighbouring columns of the same
-// rows may: where the strides differ, the whole spans count.
-int check_apart(const void* p, int64_t p_stride, const void* out, int64_t out_stride, int rows, int width, int type) {
-  const int es = elem_size(type);
-  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)out, w = (uintptr_t)width * es;
-  const uintptr_t a_end = a + (uintptr_t)(rows - 1) * p_stride * es + w, b_end = b + (uintptr_t)(rows - 1) * out_stride * es + w;
-  if (a_end <= b || b_end <= a) return Q4HIP_OK;
-  if (p_stride == out_stride) {
-    const uintptr_t s = (uintptr_t)p_stride * es, d = b >= a ? (b - a) % s : (s - (a - b) % s) % s;
-    if (d >= w && s - d >= w) return Q4HIP_OK;
-  }
-  return fail(Q4HIP_EINVAL, "q and out overlap");
-}
-
-// int32 arrays of n elements; NULL or an empty one is not looked at.
-int check_ints(const q4hip_kv8* kv, const void* p, size_t n, const char* what) {
-  if (!p || !n) return Q4HIP_OK;
-  if ((uintptr_t)p % 4) return fail(Q4HIP_EINVAL, "%s: not aligned to its type", what);
-  return check_device_span(p, n * 4, kv->device, what);
+  return check_type(type);
 }
 
 int plan_error(const q4hip_kv8* kv, int status) {
@@ -313,13 +275,6 @@ int read_head(q4hip_kv8* kv, hipStream_t s) {
   HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
   HIPCHK(hipStreamSynchronize(s));
   return Q4HIP_OK;
-}
-
-template <class F>
-void by_type(int type, F f) {
-  if (type == Q4HIP_TYPE_F32) f(float());
-  else if (type == Q4HIP_TYPE_F16) f(_Float16());
-  else f(__bf16());
 }
 
 }  // namespace
@@ -505,7 +460,7 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
       {have, (size_t)v.B, "have"}, {add, (size_t)v.B, "add"}, {starts, (size_t)v.B + 1, "starts"},
       {positions, (size_t)rows, "positions"}, {slots, (size_t)rows, "slots"}, {tables, (size_t)v.B * v.W, "tables"}};
   for (const auto& a : spans) {
-    const int rc = check_ints(kv, a.p, a.n, a.what);
+    const int rc = check_ints(kv->device, a.p, a.n, a.what);
     if (rc) return rc;
   }
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
@@ -546,8 +501,8 @@ int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int
   rc = rows_on(kv, s, &rows);
   if (rc || !rows) return rc;
   const Kv8View& w = kv->v;
-  rc = check_rows(kv, k, rows, w.KVH * w.HD, k_stride, type, "k");
-  if (!rc) rc = check_rows(kv, v, rows, w.KVH * w.HD, v_stride, type, "v");
+  rc = check_rows(kv->device, k, rows, w.KVH * w.HD, k_stride, type, "k");
+  if (!rc) rc = check_rows(kv->device, v, rows, w.KVH * w.HD, v_stride, type, "v");
   if (rc) return rc;
   kv8_launch_append(kv, s, layer, k, v, type, k_stride, v_stride, 0, w.KVH, rows);
   HIPCHK(hipGetLastError());
@@ -564,10 +519,10 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
   HIPCHK(hipSetDevice(kv->device));
   const Kv8View& w = kv->v;
   const size_t row = (size_t)w.KVH * w.HD;
-  rc = check_ints(kv, seq, n, "seq");
-  if (!rc) rc = check_ints(kv, pos, n, "pos");
-  if (!rc) rc = check_rows(kv, k, n, (int)row, row, Q4HIP_TYPE_F32, "k");
-  if (!rc) rc = check_rows(kv, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
+  rc = check_ints(kv->device, seq, n, "seq");
+  if (!rc) rc = check_ints(kv->device, pos, n, "pos");
+  if (!rc) rc = check_rows(kv->device, k, n, (int)row, row, Q4HIP_TYPE_F32, "k");
+  if (!rc) rc = check_rows(kv->device, v, n, (int)row, row, Q4HIP_TYPE_F32, "v");
   if (rc) return rc;
   hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
   kv8_launch_read(kv, s, layer, seq, pos, n, k, v);
@@ -588,9 +543,9 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
   rc = rows_on(kv, s, &rows);
   if (rc || !rows) return rc;
   const Kv8View& w = kv->v;
-  rc = check_rows(kv, q, rows, w.H * w.HD, q_stride, type, "q");
-  if (!rc) rc = check_rows(kv, out, rows, w.H * w.HD, out_stride, type, "out");
-  if (!rc) rc = check_apart(q, q_stride, out, out_stride, rows, w.H * w.HD, type);
+  rc = check_rows(kv->device, q, rows, w.H * w.HD, q_stride, type, "q");
+  if (!rc) rc = check_rows(kv->device, out, rows, w.H * w.HD, out_stride, type, "out");
+  if (!rc) rc = check_apart(q, q_stride, out, out_stride, rows, w.H * w.HD, type, "q and out");
   if (rc) return rc;
   kv8_launch_attend(kv, s, layer, q, out, type, q_stride, out_stride, scale, rows);
   HIPCHK(hipGetLastError());

@@ -22,6 +22,8 @@ DECODE_AUTO, DECODE_GRAPH, DECODE_PERSISTENT = 0, 1, 2
 KV_F32, KV_F16 = 0, 1
 F32, F16, BF16 = 0, 1, 30      # element types of an 8-bit cache's rows (GGML numbers)
 KV8_BLOCK = 32                 # positions of its pages
+ROPE_ORDERS = {"halves": 0, "pairs": 1}
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "bands": 2, "yarn": 3}
 NOALLOC_MAX_K = 65536          # include/q4hip.h Q4HIP_NOALLOC_MAX_K
 PROF_NAMES = ["embed", "norm+quantize", "matvec qkv", "rope+kv", "attention", "quantize", "matvec o",
               "matvec gate+up", "swiglu+quantize", "matvec down", "matvec output", "sample"]
@@ -37,6 +39,8 @@ EXPORTS = [
     "q4hip_attn_ring_rows", "q4hip_check_ordered_sum", "q4hip_kv8_create", "q4hip_kv8_destroy", "q4hip_kv8_plan",
     "q4hip_batch_create_kv8", "q4hip_batch_release", "q4hip_batch_free_pages", "q4hip_batch_get_kv",
     "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend",
+    "q4hip_rope_frequencies", "q4hip_rope_create", "q4hip_rope_run", "q4hip_rope_destroy",
+    "q4hip_logits_create", "q4hip_logits_run", "q4hip_logits_destroy",
 ]
 
 _lib = None
@@ -55,7 +59,7 @@ def lib() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f"{LIB_PATH} is not built: run __graft_entry__.build() first")
     L = ctypes.CDLL(LIB_PATH)
-    P, I, I64, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+    P, I, I64, F, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
     sig = {
         "q4hip_last_error": (ctypes.c_char_p, []),
         "q4hip_device_count": (I, [ctypes.POINTER(I)]),
@@ -100,6 +104,13 @@ def lib() -> ctypes.CDLL:
         "q4hip_kv8_append": (I, [P, I, P, P, I, I64, I64, P]),
         "q4hip_kv8_read": (I, [P, I, P, P, I, P, P, P]),
         "q4hip_kv8_attend": (I, [P, I, P, P, I, I64, I64, F, P]),
+        "q4hip_rope_frequencies": (I, [I, D, I, D, D, D, D, P, ctypes.POINTER(F)]),
+        "q4hip_rope_create": (I, [ctypes.POINTER(P), I, I, I, P, F, I]),
+        "q4hip_rope_run": (I, [P, P, P, I, I, I64, I64, P, I, P, P]),
+        "q4hip_rope_destroy": (None, [P]),
+        "q4hip_logits_create": (I, [ctypes.POINTER(P), I, I, I]),
+        "q4hip_logits_run": (I, [P, P, P, I, I64, I64, I, P, P, I64, P, I64, P, I, P, P]),
+        "q4hip_logits_destroy": (None, [P]),
         "q4hip_attn_ring_rows": (I, [I, I, I, I, I, I, ctypes.POINTER(I), ctypes.POINTER(I), ctypes.POINTER(I)]),
     }
     for name, (res, args) in sig.items():
@@ -459,6 +470,79 @@ class Kv8:
     def close(self) -> None:
         if self.h:
             lib().q4hip_kv8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rope_frequencies(rot: int, theta: float, scaling: str = "plain", factor: float = 1.0, original: float = 0.0, low: float = 0.0,
+                     high: float = 0.0) -> tuple:
+    """(radians a position of the rot / 2 pairs in 64 bits, amplitude): include/q4hip.h, Q4HIP_ROPE_PLAIN to Q4HIP_ROPE_YARN."""
+    freq, amplitude = np.zeros(max(rot, 2) // 2), ctypes.c_float(0)
+    _check(lib().q4hip_rope_frequencies(rot, theta, ROPE_SCALINGS[scaling], factor, original, low, high, _ptr(freq),
+                                        ctypes.byref(amplitude)))
+    return freq, amplitude.value
+
+
+class Rope:
+    """Rotary positions of rows on device buffers given by address (include/q4hip.h, q4hip_rope_*).  A call waits for its end
+    unless a stream is given."""
+
+    def __init__(self, head_dim: int, rot: int, order: str, freq, amplitude: float = 1.0, device: int = 0):
+        freq = np.ascontiguousarray(freq, np.float64)
+        if freq.shape != (rot // 2,):
+            raise ValueError(f"{rot // 2} frequencies expected")
+        h = ctypes.c_void_p()
+        _check(lib().q4hip_rope_create(ctypes.byref(h), head_dim, rot, ROPE_ORDERS[order], _ptr(freq), amplitude, device))
+        self.h = h
+
+    def run(self, x: int, y: int, heads: int, dtype: int, x_stride: int, y_stride: int, pos: int, rows: int, count: int = 0,
+            stream: int = 0) -> None:
+        """Rows x turned by their positions into y (which may be x); count: address of the number of rows that there are."""
+        _check(lib().q4hip_rope_run(self.h, x or None, y or None, heads, dtype, x_stride, y_stride, pos or None, rows, count or None,
+                                    stream or None))
+
+    def close(self) -> None:
+        if self.h:
+            lib().q4hip_rope_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# A row's rules (q4hip_logits_row) and a bias (q4hip_logits_bias), to be filled and copied to the device.
+LOGITS_ROW = np.dtype([("repetition", np.float32), ("presence", np.float32), ("frequency", np.float32), ("history_begin", np.int32),
+                       ("history_end", np.int32), ("bias_begin", np.int32), ("bias_end", np.int32), ("mask", np.int32)])
+LOGITS_BIAS = np.dtype([("token", np.int32), ("value", np.float32)])
+
+
+class Logits:
+    """Penalties, biases and masks on rows of logits, and each row's best token, on device buffers given by address
+    (include/q4hip.h, q4hip_logits_*).  A call waits for its end unless a stream is given."""
+
+    def __init__(self, vocab: int, max_rows: int, device: int = 0):
+        h = ctypes.c_void_p()
+        _check(lib().q4hip_logits_create(ctypes.byref(h), vocab, max_rows, device))
+        self.h = h
+
+    def run(self, x: int, y: int, dtype: int, x_stride: int, y_stride: int, rows: int, params: int, history: int = 0,
+            history_n: int = 0, biases: int = 0, biases_n: int = 0, mask: int = 0, mask_rows: int = 0, best: int = 0,
+            stream: int = 0) -> None:
+        """Rows x by the rules params[rows] (LOGITS_ROW) into y (which may be x); best: int32 [rows]."""
+        _check(lib().q4hip_logits_run(self.h, x or None, y or None, dtype, x_stride, y_stride, rows, params or None, history or None,
+                                      history_n, biases or None, biases_n, mask or None, mask_rows, best or None, stream or None))
+
+    def close(self) -> None:
+        if self.h:
+            lib().q4hip_logits_destroy(self.h)
             self.h = None
 
     def __del__(self):

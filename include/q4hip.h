@@ -316,6 +316,73 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
 
+/* ---- rotary positions ---------------------------------------------------------------------------
+ * For callers that bring their own rows (between q4hip_kv8_plan, which gives the rows' positions, and q4hip_kv8_append):
+ * the pairs (x, y) of the first `rot` columns of a head become, at position p,
+ *   amplitude * (x cos a - y sin a,  y cos a + x sin a),   a = p * freq[i] for the i-th pair
+ * and the columns behind them stay as they are.  (The engine's own passes turn q and k from a table, engine/kernels.c:337-345;
+ * the other orders, parts of heads and stretched contexts have no counterpart there.)  The angle is exact to 2^-32 of
+ * a turn at every position of 32 bits; sines, cosines and the sums are fp32, rounded once to the rows' type. */
+typedef struct q4hip_rope q4hip_rope;
+#define Q4HIP_ROPE_MAX_DIM 512
+/* Order of a pair's columns: rot / 2 apart, or neighbours. */
+#define Q4HIP_ROPE_HALVES 0
+#define Q4HIP_ROPE_PAIRS 1
+/* Frequencies: theta^(-2 i / rot) as they are; all divided by `factor`; divided by it in part, by the turns t that a pair makes
+ * in the `original` context (t <= low: whole, t >= high: not, between them in proportion to t); the same in proportion to i, between the
+ * pairs that make `high` turns (rounded down) and `low` turns (rounded up), with amplitude 0.1 ln(factor) + 1. */
+#define Q4HIP_ROPE_PLAIN 0
+#define Q4HIP_ROPE_LINEAR 1
+#define Q4HIP_ROPE_BANDS 2
+#define Q4HIP_ROPE_YARN 3
+/* Writes the rot / 2 frequencies, in radians a position, and the amplitude (host only, no GPU); arguments that a scaling does not name
+ * are not looked at. */
+int q4hip_rope_frequencies(int rot, double theta, int scaling, double factor, double original, double low, double high, double* freq,
+                           float* amplitude);
+/* freq[rot / 2] is host memory, of q4hip_rope_frequencies or the caller's own. */
+int q4hip_rope_create(q4hip_rope** out, int head_dim, int rot, int order, const double* freq, float amplitude, int device);
+/* Row t, head h, column d at x[t * x_stride + h * head_dim + d] (`type` F32, F16 or BF16, strides in elements), y alike; pos[t] is the
+ * row's position.  q and k of fused rows are one call with the heads of both.  y is x (the same pointer and stride), or
+ * shares no byte with the rows of x.  `count` (one int32 in device memory, or NULL): only the first min(rows, *count) rows are
+ * turned, the others left as they were (starts + seqs of a captured plan).  Pointers are device memory of the handle's device and are
+ * checked, with the bytes behind them, before anything is launched; nothing is allocated.  `stream` NULL: the handle's own, and the
+ * call waits for its end. */
+int q4hip_rope_run(q4hip_rope* r, const void* x, void* y, int heads, int type, int64_t x_stride, int64_t y_stride, const int* pos,
+                   int rows, const int* count, void* stream);
+void q4hip_rope_destroy(q4hip_rope* r);
+
+/* ---- logits: penalties, biases, masks, the best token ------------------------------------------------
+ * For callers that pick tokens by rules (the engine picks the first maximum, engine/cpu-worker.js:154-158; no counterpart
+ * there).  Of a row's token v with logit x, in fp32 and in this order:
+ *   c > 0 occurrences in the row's history:  x = x > 0 ? x / repetition : x * repetition;  x = x - (frequency * c + presence)
+ *   biases of the row with this token:       x = x + value of the last one
+ *   bit v % 32 of word v / 32 of the row's mask is 0:  x = -infinity
+ * rounded once to the rows' type.  Entries of lists that name no token of the vocabulary count for nothing. */
+typedef struct q4hip_logits q4hip_logits;
+typedef struct {
+  float repetition, presence, frequency;   /* 1, 0 and 0 change nothing */
+  int history_begin, history_end;          /* its entries of the history (cut to the list; none where begin >= end) */
+  int bias_begin, bias_end;                /* its entries of the biases, alike */
+  int mask;                                /* its mask; none outside of 0..mask_rows-1 */
+} q4hip_logits_row;
+typedef struct {
+  int token;
+  float value;
+} q4hip_logits_bias;
+/* For rows of `vocab` logits, up to max_rows of them in a call. */
+int q4hip_logits_create(q4hip_logits** out, int vocab, int max_rows, int device);
+/* Row t at x[t * x_stride], its results at y[t * y_stride] (`type` F32, F16 or BF16, strides in elements); y is x (the same pointer
+ * and stride) or shares no byte with the rows of x.  params[rows], history[history_n], biases[biases_n] and mask[mask_rows][ceil(vocab /
+ * 32)] (lists of no entries may be NULL).  best (NULL, or int32 [rows]): the lowest token of the row's largest value, as it was before
+ * it was rounded to the type; NaN and -infinity do not count, -1 where nothing else is left.  All of them are device memory of the
+ * handle's device and are checked, with the bytes behind them, before anything is launched; nothing is allocated.  `stream` NULL: the
+ * handle's own, and the call waits for its end.  Calls with `best` on one handle are serialized by the caller, also on the GPU (graphs
+ * that hold them, too). */
+int q4hip_logits_run(q4hip_logits* lg, const void* x, void* y, int type, int64_t x_stride, int64_t y_stride, int rows,
+                     const q4hip_logits_row* params, const int* history, int64_t history_n, const q4hip_logits_bias* biases,
+                     int64_t biases_n, const uint32_t* mask, int mask_rows, int* best, void* stream);
+void q4hip_logits_destroy(q4hip_logits* lg);
+
 /* ---- self-check of the quotient forms ------------------------------------------------------
  * The kernels compute the reference's IEEE binary32 divisions (engine/kernels.c:84, 98-99, 395)
  * by reciprocal products with fused corrections on verified domains.  This runs every input of
