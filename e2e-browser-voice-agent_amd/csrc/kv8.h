@@ -23,6 +23,7 @@ constexpr int kKv8Block = 32;
 // sequences of up to 16,000 positions: parts of at most 128 pages 225 us, as long as the aim asks 245.
 constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
+constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups; else in units, whose pages can be shared.  Tiles and units, us: 2,048 rows of 14 heads (fp32)
 // 57 and 42, 8,192 rows 283 and 370; of 32 heads (bf16) 83 and 84, 773 and 860; of 8 heads of one kv head (bf16) 65 and 32, 262
@@ -46,8 +47,16 @@ struct Kv8Head {
   int free_pages;
   int runs, items, tiles;
   int parts_of;    // pages from which on a unit's pages are shared among several items, and in parts of how many
+  int shared;      // whether any page belongs to several sequences (else `refs` means nothing)
 };
-enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE };
+enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE, KV8_SHARED, KV8_FORK_SOURCE, KV8_FORK_PAGES };
+
+// What the launches of a fork tell one another.
+struct Kv8Fork {
+  int bad;         // an argument that cannot be, 0 between calls
+  int status, copies;
+  uint64_t entries;    // of all tables, afterwards
+};
 
 // A run: rows t.. that lie in one page from `slot` on, m of them.
 struct Kv8Run {
@@ -86,7 +95,7 @@ struct Kv8View {
   float2* scales;      // [layers][pages][kv_heads] of K, V
   int* table;          // [seqs][blocks] pages, -1 past those a sequence holds
   int* held;           // [seqs] pages of a sequence
-  int* stack;          // [pages] free pages, the next one to take last
+  int* stack;          // [4][pages]: free pages, the next one to take last; refs(), count(), first()
   Kv8Head* head;
   int *base, *lens;    // [seqs] positions before and after the step
   int* starts;         // [seqs + 1] first row of a sequence in the step
@@ -104,12 +113,25 @@ struct Kv8View {
   int row_tiles;       // of a unit: 16 rows (32 of a wide one, which has no more of them)
   int items_aim;       // items that fill the GPU
   double aim_inverse;  // 1 / items_aim, not rounded down
+  // Behind the stack and not pointers of their own: every launch takes this struct along, and 56 more bytes cost 0.2 us.
+  __device__ int* refs() const { return stack + pages; }                 // sequences that hold a page, while any page has several
+  __device__ int* count() const { return stack + 2 * (size_t)pages; }    // scratch of plan and fork, 0 between calls
+  __device__ int* first() const { return stack + 3 * (size_t)pages; }    // alike, INT_MAX between calls
+};
+
+// The scratch memory of a fork.
+struct Kv8ForkView {
+  int* next;           // [seqs][blocks] the tables afterwards
+  int2* copies;        // [seqs] a sequence whose last page is copied, and the page
+  int* chunk;          // [pages / kKv8Chunk] free pages
+  Kv8Fork* fork;
 };
 
 }  // namespace q4
 
 struct q4hip_kv8 {
   q4::Kv8View v{};
+  q4::Kv8ForkView f{};
   int device = 0, max_rows = 0;
   int rows = 0;                // rows the last plan was called for, outside of captures
   unsigned long long capture = 0;   // the last capture of a plan, and the rows of that
@@ -131,6 +153,7 @@ void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv,
                             int rows);
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
                        int64_t out_stride, float scale, int rows);
+void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables);
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v);
 
 }  // namespace q4

@@ -7,6 +7,7 @@
 
 #include "host.h"
 #include "kv8_attend.h"
+#include "kv8_fork.h"
 #include "kv8_plan.h"
 #include "rows.h"
 
@@ -22,6 +23,9 @@ constexpr size_t kFillInPlan = 8192, kFillInPlanGlobal = 2048;
 // Workgroups of attention at most; each takes every so-manieth tile or item.  (1,024: up to 9% more time, 512: up to 35%, as the
 // tiles of a step differ in length.)
 constexpr int64_t kMostWorkgroups = 8192;
+
+// Workgroups of a fork's copies at most.
+constexpr int64_t kForkGrid = 4096;
 
 // The quotient x / s rounded to fp32, from r = 1 / s rounded: one correction of x * r by its residual gives it
 // (P. Markstein, IBM J. Res. Dev. 34(1), 1990) where the residual is exact, which |x / s| >= 1/4 and s >= 2^-100 make
@@ -222,15 +226,22 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8View v, int layer, const in
 }
 
 // The free pages in the order in which they are taken, and a table without pages.
-__global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v) {
+__global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v, Kv8ForkView f) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i < (size_t)v.B * v.W) v.table[i] = -1;
-  if (i < (size_t)v.pages) v.stack[i] = v.pages - 1 - (int)i;
+  if (i < (size_t)v.pages) {
+    v.stack[i] = v.pages - 1 - (int)i;
+    v.count()[i] = 0;
+    v.first()[i] = INT32_MAX;
+  }
   if (i <= (size_t)v.B) {
     v.starts[i] = 0;
     if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
   }
-  if (i == 0) *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1};
+  if (i == 0) {
+    *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0};
+    *f.fork = Kv8Fork{};
+  }
 }
 
 // At most so many tiles have `rows` rows: of full ones, and of a last one of each sequence.
@@ -246,11 +257,15 @@ int check_layer(const q4hip_kv8* kv, int layer, int type) {
 int plan_error(const q4hip_kv8* kv, int status) {
   switch (status) {
     case KV8_OK: return Q4HIP_OK;
-    case KV8_BAD_LENGTH: return fail(Q4HIP_EINVAL, "plan: a negative length");
+    case KV8_BAD_LENGTH: return fail(Q4HIP_EINVAL, "plan or fork: a negative length");
     case KV8_TOO_LONG: return fail(Q4HIP_ECONTEXT, "plan: a sequence longer than %d positions", kv->v.max_len);
     case KV8_STALE:
       return fail(Q4HIP_ESTATE, "append or attend replayed on a plan of more rows than they were captured for");
     case KV8_ROWS: return fail(Q4HIP_EINVAL, "plan: more rows than it was called for");
+    case KV8_SHARED:
+      return fail(Q4HIP_EINVAL, "plan: rows into a page that another sequence holds, too: cut the sequence back by a fork first");
+    case KV8_FORK_SOURCE: return fail(Q4HIP_EINVAL, "fork: a sequence that there is not, or more positions than it holds");
+    case KV8_FORK_PAGES: return fail(Q4HIP_ECONTEXT, "fork: more than the pool's %d pages", kv->v.pages);
     default: return fail(Q4HIP_ECONTEXT, "plan: more than the pool's %d pages", kv->v.pages);
   }
 }
@@ -349,6 +364,18 @@ void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, v
   });
 }
 
+void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables) {
+  const Kv8View& v = kv->v;
+  const unsigned chunks = (unsigned)((v.pages + kKv8Chunk - 1) / kKv8Chunk), all = (unsigned)kForkGrid;
+  const size_t entries = (size_t)v.B * v.W;
+  k_kv8_fork_count<<<dim3((unsigned)std::min((v.W + kForkThreads - 1) / kForkThreads, 64), (unsigned)std::min(v.B, 65535)), kForkThreads,
+                     0, s>>>(v, kv->f, from, keep);
+  k_kv8_fork_weigh<<<chunks + 1, kKv8Chunk, 0, s>>>(v, kv->f, keep);
+  k_kv8_fork_commit<<<std::max(chunks, (unsigned)std::min<size_t>((entries + kKv8Chunk - 1) / kKv8Chunk, 512)), kKv8Chunk, 0, s>>>(
+      v, kv->f, keep, tables);
+  k_kv8_fork_copy<<<(unsigned)std::min<int64_t>((int64_t)v.B * v.layers * v.KVH, all), kForkThreads, 0, s>>>(v, kv->f, keep, tables);
+}
+
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v) {
   const Kv8View& w = kv->v;
   const int per = 1024 / w.HD;                 // rows of a workgroup
@@ -369,7 +396,7 @@ void q4hip_kv8_destroy(q4hip_kv8* kv) {
   if (kv->stream) (void)hipStreamSynchronize(kv->stream);
   Kv8View& v = kv->v;
   void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
-                  v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived};
+                  kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (kv->pin) (void)hipHostFree(kv->pin);
   if (kv->stream) (void)hipStreamDestroy(kv->stream);
@@ -417,7 +444,11 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.scales, blocks);
   al(&v.table, (size_t)seqs * v.W);
   al(&v.held, seqs);
-  al(&v.stack, pages);
+  al(&v.stack, (size_t)4 * pages);
+  al(&kv->f.next, (size_t)seqs * v.W);
+  al(&kv->f.copies, seqs);
+  al(&kv->f.chunk, (pages + kKv8Chunk - 1) / kKv8Chunk);
+  al(&kv->f.fork, 1);
   al(&v.head, 1);
   al(&v.base, seqs);
   al(&v.lens, seqs);
@@ -437,7 +468,7 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   if (e == hipSuccess) e = hipMemsetAsync(v.arrived, 0, parts * sizeof(int), kv->stream);
   if (e == hipSuccess) {
     const size_t n = std::max({(size_t)seqs * v.W, (size_t)pages, (size_t)seqs + 1});
-    k_kv8_reset<<<(unsigned)((n + 255) / 256), 256, 0, kv->stream>>>(v);
+    k_kv8_reset<<<(unsigned)((n + 255) / 256), 256, 0, kv->stream>>>(v, kv->f);
     e = hipGetLastError();
   }
   if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
@@ -474,6 +505,35 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
     kv->capture_rows = rows;
   } else {
     kv->rows = rows;
+  }
+  if (stream) return Q4HIP_OK;
+  rc = read_head(kv, s);
+  return rc ? rc : plan_error(kv, kv->pin->status);
+}
+
+int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables, void* stream) {
+  if (!kv || !from || !keep) return fail(Q4HIP_EINVAL, "null argument");
+  const Kv8View& v = kv->v;
+  HIPCHK(hipSetDevice(kv->device));
+  int rc = check_ints(kv->device, from, v.B, "from");
+  if (!rc) rc = check_ints(kv->device, keep, v.B, "keep");
+  if (!rc) rc = check_ints(kv->device, tables, (size_t)v.B * v.W, "tables");
+  const size_t n = (size_t)v.B * 4;
+  if (!rc && tables && (overlap(tables, n * v.W, from, n) || overlap(tables, n * v.W, keep, n)))
+    rc = fail(Q4HIP_EINVAL, "tables overlaps from or keep");
+  if (rc) return rc;
+  hipStream_t s = stream ? (hipStream_t)stream : kv->stream;
+  unsigned long long id;
+  rc = capture_of(s, &id);
+  if (rc) return rc;
+  kv8_launch_fork(kv, s, from, keep, tables);
+  HIPCHK(hipGetLastError());
+  // the step is over: nothing is left to append or attend
+  if (id) {
+    kv->capture = id;
+    kv->capture_rows = 0;
+  } else {
+    kv->rows = 0;
   }
   if (stream) return Q4HIP_OK;
   rc = read_head(kv, s);

@@ -38,7 +38,7 @@ EXPORTS = [
     "q4hip_batch_read_logits", "q4hip_mv_time_cold", "q4hip_check_division", "q4hip_mv_run_noalloc",
     "q4hip_attn_ring_rows", "q4hip_check_ordered_sum", "q4hip_kv8_create", "q4hip_kv8_destroy", "q4hip_kv8_plan",
     "q4hip_batch_create_kv8", "q4hip_batch_release", "q4hip_batch_free_pages", "q4hip_batch_get_kv",
-    "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend",
+    "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend", "q4hip_kv8_fork",
     "q4hip_rope_frequencies", "q4hip_rope_create", "q4hip_rope_run", "q4hip_rope_destroy",
     "q4hip_logits_create", "q4hip_logits_run", "q4hip_logits_destroy",
 ]
@@ -100,6 +100,7 @@ def lib() -> ctypes.CDLL:
         "q4hip_kv8_create": (I, [ctypes.POINTER(P), I, I, I, I, I, I, I, I, I]),
         "q4hip_kv8_destroy": (None, [P]),
         "q4hip_kv8_plan": (I, [P, P, P, I, P, P, P, P, P]),
+        "q4hip_kv8_fork": (I, [P, P, P, P, P]),
         "q4hip_kv8_status": (I, [P, P, ctypes.POINTER(I), ctypes.POINTER(I)]),
         "q4hip_kv8_append": (I, [P, I, P, P, I, I64, I64, P]),
         "q4hip_kv8_read": (I, [P, I, P, P, I, P, P, P]),
@@ -448,8 +449,12 @@ class Kv8:
         _check(lib().q4hip_kv8_plan(self.h, have or None, add or None, rows, starts or None, positions or None, slots or None,
                                     tables or None, stream or None))
 
+    def fork(self, from_: int, keep: int, tables: int = 0, stream: int = 0) -> None:
+        """Sequence b becomes the first keep[b] positions of sequence from_[b], all at once; whole pages are shared."""
+        _check(lib().q4hip_kv8_fork(self.h, from_ or None, keep or None, tables or None, stream or None))
+
     def status(self, stream: int = 0) -> tuple:
-        """(rows of the last plan, free pages); raises the plan's error."""
+        """(rows of the last plan, free pages); raises the plan's or fork's error."""
         rows, free = ctypes.c_int(0), ctypes.c_int(0)
         _check(lib().q4hip_kv8_status(self.h, stream or None, ctypes.byref(rows), ctypes.byref(free)))
         return rows.value, free.value

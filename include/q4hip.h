@@ -294,7 +294,20 @@ void q4hip_kv8_destroy(q4hip_kv8* kv);
  * returns that error; otherwise q4hip_kv8_status does. */
 int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,
                    int* tables, void* stream);
-/* Waits for `stream` (NULL: the handle's) and returns the last plan's error, its rows and the pages left. */
+/* Sequences become the beginnings of others, all at once: afterwards sequence b holds the first keep[b] positions that sequence from[b]
+ * held (int32 device arrays of `seqs`; from[b] = b keeps or cuts back, keep[b] = 0 empties and looks at no from[b]), in all layers.
+ * Pages of 32 positions that are whole are shared, and belong to all who hold them until the last one gives them back.  A
+ * last page that is not whole stays with the first sequence whose last page it is, if it is nobody's whole page; the others get
+ * copies of it, in the order of the sequences, in the free pages of the lowest numbers.  Pages that nobody holds any more are free, and
+ * all free pages are taken from then on in the order of their numbers.  `tables` (NULL, or device memory): as of a plan.  The step
+ * is over: append and attend do nothing until the next plan.  Arguments that do not fit (a sequence that there is not, more positions than
+ * it holds) or too few free pages for the copies make the call fail as a whole, as a plan does: nothing changes hands, and with
+ * `stream` NULL the call returns the error, otherwise q4hip_kv8_status does.
+ * A plan whose rows would lie in a page that another sequence holds afterwards, too, fails (Q4HIP_EINVAL): only whole pages are shared,
+ * so this takes a chat that was cut back to within one, and a fork that cuts it back there (from[b] = b, keep[b] = have[b])
+ * makes that page its own. */
+int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables, void* stream);
+/* Waits for `stream` (NULL: the handle's) and returns the last plan's or fork's error, its rows and the pages left. */
 int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages);
 /* K and V of the step's rows, `type` F32, F16 or BF16: row t, kv head g, column d at
  * k[t * k_stride + g * head_dim + d] (strides in elements; the buffers hold the `rows` of the plan).  Of the rows that fall
