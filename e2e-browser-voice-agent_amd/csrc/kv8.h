@@ -23,6 +23,8 @@ constexpr int kKv8Block = 32;
 // sequences of up to 16,000 positions: parts of at most 128 pages 225 us, as long as the aim asks 245.
 constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
+// Joints of a step at most, which is 16,384 rows of attention: their sums take 32 * head_dim * 8 bytes a kv head each.
+constexpr int kKv8Joints = 512;
 constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups; else in units, whose pages can be shared.  Tiles and units, us: 2,048 rows of 14 heads (fp32)
@@ -47,7 +49,8 @@ struct Kv8Head {
   int free_pages;
   int runs, items, tiles;
   int parts_of;    // pages from which on a unit's pages are shared among several items, and in parts of how many
-  int shared;      // whether any page belongs to several sequences (else `refs` means nothing)
+  int shared;      // whether any page belongs to several sequences (else refs() means nothing)
+  int joint_items, joints; // items of the list with joints and joints, 0 where there is no such list
 };
 enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE, KV8_SHARED, KV8_FORK_SOURCE, KV8_FORK_PAGES };
 
@@ -71,7 +74,21 @@ struct Kv8Item {
   int pos;               // position of the first row
   int page0, pages;      // of the sequence's table
   int part, slot;        // slot: of the unit's first part in the workspace, -1 for a unit in one part
-  int parts, wide, unused[2];
+  int parts, wide;
+  // of a list with joints: the joint (counted from 1) of an item over a joint's pages, whose n are its rows of attention; -1
+  // for a unit with rows in joints, the first of which is `row`; 0 for any other
+  int joint, row;
+};
+
+// A joint: up to 32 rows of attention, neighbours among the rows of units whose sequences begin with the same pages.  One pass over those
+// pages serves them all; a row is the sum of that and of its unit's pass over the pages behind.
+struct Kv8Joint {
+  int slot, parts;       // where its sums lie in the workspace
+};
+struct Kv8JointRow {
+  int t, h;              // the row of the step (-1: none), the head of the kv head's
+  int slot, parts, row;  // where its unit's sums lie
+  int unused[3];
 };
 
 // A tile: kKv8TileRows rows of attention (positions x G) of a sequence with many rows.
@@ -119,6 +136,15 @@ struct Kv8View {
   __device__ int* first() const { return stack + 3 * (size_t)pages; }    // alike, INT_MAX between calls
 };
 
+// The lists with joints, which a step of a cache with shared pages has beside its own.
+struct Kv8JointView {
+  Kv8Item* items;
+  Kv8Joint* joints;    // [most]
+  Kv8JointRow* rows;   // [most][32]
+  int most;            // joints of a step.  The workspace's slots 0..most-1 are of joints in one part, rows of units in one part lie
+                       // in the slots most..2 most-1 (32 each, as in the joints), other slots begin behind them
+};
+
 // The scratch memory of a fork.
 struct Kv8ForkView {
   int* next;           // [seqs][blocks] the tables afterwards
@@ -132,6 +158,9 @@ struct Kv8ForkView {
 struct q4hip_kv8 {
   q4::Kv8View v{};
   q4::Kv8ForkView f{};
+  q4::Kv8JointView j{};
+  int* joint_scratch = nullptr;
+  bool forked = false;         // whether pages may be shared: a plan makes lists with joints, too
   int device = 0, max_rows = 0;
   int rows = 0;                // rows the last plan was called for, outside of captures
   unsigned long long capture = 0;   // the last capture of a plan, and the rows of that

@@ -8,6 +8,7 @@
 #include "host.h"
 #include "kv8_attend.h"
 #include "kv8_fork.h"
+#include "kv8_joint.h"
 #include "kv8_plan.h"
 #include "rows.h"
 
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v, Kv8ForkView f) {
     if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
   }
   if (i == 0) {
-    *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0};
+    *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0, 0, 0};
     *f.fork = Kv8Fork{};
   }
 }
@@ -286,6 +287,9 @@ int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
   return rc;
 }
 
+// Whether a step's units may be joined: more than 16 rows of a kv head fill the matrix cores by themselves.
+bool joined(const q4hip_kv8* kv, int rows) { return kv->forked && kv->v.H / kv->v.KVH <= 16 && rows > 1 && kv->v.B > 1; }
+
 int read_head(q4hip_kv8* kv, hipStream_t s) {
   HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
   HIPCHK(hipStreamSynchronize(s));
@@ -309,6 +313,9 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
     k_kv8_plan<false><<<1, kPlanThreads, 0, s>>>(v, have, add, rows, starts, positions, slots, tables, fill);
   }
   if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
+  if (!joined(kv, rows)) return;
+  if (shared) k_kv8_joints<true><<<1, kJointThreads, 0, s>>>(v, kv->j, have, add, nullptr);
+  else k_kv8_joints<false><<<1, kJointThreads, 0, s>>>(v, kv->j, have, add, kv->joint_scratch);
 }
 
 namespace {
@@ -354,18 +361,30 @@ void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, v
   const int64_t items = units + std::min<int64_t>(kKv8MoreItems * w.items_aim, (int64_t)units * (w.pages / kKv8MinPart));
   const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
   const bool few = rows <= w.unit_rows;    // neither wide units nor tiles
-  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, rows) * w.KVH);
+  const bool joint = joined(kv, rows);
+  const int64_t work = (items + (joint ? std::min(units, kv->j.most) : 0)) * w.KVH * w.row_tiles +
+                       (few && !joint ? 0 : (int64_t)tiles_bound(w, rows) * w.KVH);
   const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
-    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
-                          : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide);
+    if (joint) {
+      auto* fn = w.HD == 64 ? k_kv8_attend<64, T, 2, true> : k_kv8_attend<128, T, 2, true>;
+      fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide, kv->j);
+      // rows of joints, or less
+      const int64_t most = std::min<int64_t>(32 * (int64_t)kv->j.most, (int64_t)rows * (w.H / w.KVH) + 31 * (rows / 2));
+      auto* sum = w.HD == 64 ? k_kv8_gather<64, T> : k_kv8_gather<128, T>;
+      sum<<<(unsigned)std::min(most * w.KVH, kMostWorkgroups), 256, 0, s>>>(w, kv->j, (T*)out, out_stride, rows, wide);
+      return;
+    }
+    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0, false> : k_kv8_attend<64, T, 2, false>)
+                          : (few ? k_kv8_attend<128, T, 0, false> : k_kv8_attend<128, T, 2, false>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide, Kv8NoJoints{});
   });
 }
 
 void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables) {
   const Kv8View& v = kv->v;
+  kv->forked = true;
   const unsigned chunks = (unsigned)((v.pages + kKv8Chunk - 1) / kKv8Chunk), all = (unsigned)kForkGrid;
   const size_t entries = (size_t)v.B * v.W;
   k_kv8_fork_count<<<dim3((unsigned)std::min((v.W + kForkThreads - 1) / kForkThreads, 64), (unsigned)std::min(v.B, 65535)), kForkThreads,
@@ -396,7 +415,8 @@ void q4hip_kv8_destroy(q4hip_kv8* kv) {
   if (kv->stream) (void)hipStreamSynchronize(kv->stream);
   Kv8View& v = kv->v;
   void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
-                  kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived};
+                  kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived,
+                  kv->j.items, kv->j.joints, kv->j.rows, kv->joint_scratch};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (kv->pin) (void)hipHostFree(kv->pin);
   if (kv->stream) (void)hipStreamDestroy(kv->stream);
@@ -457,8 +477,16 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   const size_t most_items = (size_t)kKv8MoreItems * v.items_aim;      // beyond one for each unit
   al(&v.items, max_rows + most_items);
   al(&v.tiles, tiles_bound(v, max_rows));
+  if (seqs > 1 && G <= 16) {
+    // the rows of groups of two and more, in whole joints
+    kv->j.most = (int)std::min<int64_t>(((int64_t)seqs * v.unit_rows * G + 31) / 32 + seqs / 2, kKv8Joints);
+    al(&kv->j.items, max_rows + most_items + kv->j.most);
+    al(&kv->j.joints, kv->j.most);
+    al(&kv->j.rows, (size_t)32 * kv->j.most);
+    if (seqs > kPlanShared) al(&kv->joint_scratch, (size_t)kJointArrays * seqs);
+  }
   // units in several parts: each has more pages than a part, so that the last one's part at most doubles them
-  const size_t parts = 2 * most_items * kv_heads * v.row_tiles;
+  const size_t parts = (2 * most_items + 2 * (size_t)kv->j.most) * kv_heads * v.row_tiles;
   al(&v.part_o, parts * 32 * head_dim);
   al(&v.part_ml, parts * 32);
   al(&v.arrived, parts);

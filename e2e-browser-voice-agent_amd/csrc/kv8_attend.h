@@ -40,6 +40,8 @@
 // formed beside the weights of the page before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7%
 // slower).
 #pragma once
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace q4 {
@@ -436,6 +438,8 @@ __device__ inline void kv8_send_part(const Kv8View& v, size_t slot, int row, int
   if (d == 0) kv8_send((float*)(v.part_ml + slot * 32 + row), m, l);
 }
 
+struct Kv8NoJoints {};
+
 template <int HD>
 struct Kv8Shared {
   float o[4][16][HD + 4];
@@ -461,14 +465,16 @@ __device__ inline bool kv8_last(S& sh, int* counter, int count) {
 // The four waves take every fourth page each and add up their sums in shared memory, 16 rows at a time.  A unit in
 // several parts: the last workgroup of each 16 parts to be done adds those up, and the last of these the sums of 16, always
 // in the order of the parts.
-template <int HD, class T, int N>
-__device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv8Shared<HD>& sh, int layer, const T* q, T* out,
-                                         int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {
+// kJoint: the item may be of a joint.  Then its sums stay in the workspace, for kv8_gather.
+template <int HD, class T, int N, bool kJoint>
+__device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8JointView& jv, const Kv8Item& it, Kv8Shared<HD>& sh, int layer,
+                                         const T* q, T* out, int64_t q_stride, int64_t out_stride, float scale, bool wide, int y) {
   constexpr bool kTwo = sizeof(T) == 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, quarter = lane >> 4, G = v.H / v.KVH;
   const int g = y / v.row_tiles, r0 = (y % v.row_tiles) * (16 * N);
-  const int rows = min(16 * N, it.n * G - r0);                  // of this tile
+  const bool joint = kJoint && it.joint, common = joint && it.joint > 0;
+  const int rows = min(16 * N, common ? it.n : it.n * G - r0);                  // of this tile
   if (rows <= 0) return;
   Kv8Rows<HD, kTwo, N> w;
   int row_last[N];
@@ -476,11 +482,18 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
 #pragma unroll
   for (int t = 0; t < N; t++) {
     const int r = r0 + min(t * 16 + n, rows - 1), tok = kv8_div_g(v, r);      // rows behind the end: as the last one, not written
+    if (common) {
+      const Kv8JointRow* const jr = jv.rows + (size_t)(it.joint - 1) * 32 + r;
+      row[t] = q + (int64_t)jr->t * q_stride + (g * G + jr->h) * HD;
+      row_last[t] = INT32_MAX - 1;             // all of the pages
+      continue;
+    }
     row[t] = q + (int64_t)(it.t + tok) * q_stride + (g * G + r - tok * G) * HD;
     row_last[t] = it.pos + tok;
   }
   w.init(row, quarter, wide, scale);
-  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, it.pos, row_last);
+  w.run(v, layer, g, v.table + (size_t)it.seq * v.W, it.page0 + wave, 4, (it.pages - wave + 3) >> 2, common ? INT32_MAX : it.pos,
+        row_last);
   const int ys = v.KVH * v.row_tiles;
   const size_t slot = (size_t)max(it.slot, 0) * ys + y;         // of the unit's first part
   auto write = [&](int row, int d, const kv8_f4& o) {
@@ -507,11 +520,14 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8Item& it, Kv
         const kv8_f4 x = *(const kv8_f4*)&sh.o[k][row][d];
         for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c] * il, f, o[c]);
       }
-      if (it.parts == 1) write(t * 16 + row, d, o);
+      if (joint && !common && it.parts == 1) {
+        const int at = it.row + row;
+        kv8_send_part<HD>(v, (size_t)(jv.most + (at >> 5)) * ys + y, at & 31, d, o, r, l);
+      } else if (it.parts == 1 && !joint) write(t * 16 + row, d, o);
       else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, r, l);
     }
   }
-  if (it.parts > 1) {
+  if (it.parts > 1 && !joint) {
     const int first = it.part & ~15, mine = min(16, it.parts - first), sixteens = (it.parts + 15) >> 4;
     const size_t own = slot + (size_t)first * ys;
     if (kv8_last(sh, v.arrived + own, mine)) {
@@ -572,10 +588,11 @@ __device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q
 }
 
 // A step's tiles, the longest first, then its items.  The kv heads are neighbours in the grid, so that the tiles of one
-// meet on the same XCDs and find its pages in their L2.
-template <int HD, class T, int N>
+// meet on the same XCDs and find its pages in their L2.  kJoint: of the list with joints, if the plan has made one.
+template <int HD, class T, int N, bool kJoint>
 __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                    int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide) {
+                                                    int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide,
+                                                    std::conditional_t<kJoint, Kv8JointView, Kv8NoJoints> jv) {
   __shared__ Kv8Shared<HD> sh;
   const int ys = v.KVH * v.row_tiles;
   const Kv8Head head = *v.head;
@@ -585,7 +602,14 @@ __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, con
     if (threadIdx.x == 0) v.head->status = KV8_STALE;
     return;
   }
-  const int tiles = N ? head.tiles * v.KVH : 0, all = tiles + head.items * ys;
+  const Kv8Item* items = v.items;
+  int n = head.items;
+  Kv8JointView j = {};
+  if constexpr (kJoint) {
+    j = jv;
+    if (head.joint_items) { items = jv.items; n = head.joint_items; }
+  }
+  const int tiles = N ? head.tiles * v.KVH : 0, all = tiles + n * ys;
   for (int i = blockIdx.x; i < all; i += gridDim.x) {
     if constexpr (N > 0)
       if (i < tiles) {
@@ -593,13 +617,84 @@ __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, con
         continue;
       }
     const int k = i - tiles, y = k % ys;
-    if (N > 0 || i != (int)blockIdx.x) it = v.items[k / ys];
+    if (N > 0 || i != (int)blockIdx.x) it = items[k / ys];
     if constexpr (N > 0)
       if (it.wide) {
-        kv8_item<HD, T, N>(v, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+        kv8_item<HD, T, N, kJoint>(v, j, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
         continue;
       }
-    kv8_item<HD, T, 1>(v, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+    kv8_item<HD, T, 1, kJoint>(v, j, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+  }
+}
+
+// The rows of joints: a workgroup adds up a row's parts, of its joint and of its unit, a group of threads every so-manieth one.
+// (The last workgroup to be done could, too, as it does for units: but it alone then reads up to 128 parts of 32 rows.  8 sequences
+// behind 131,072 positions: 41.3 us so, 25.2 now.)
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_kv8_gather(Kv8View v, Kv8JointView jv, T* __restrict__ out, int64_t out_stride, int rows,
+                                                    bool wide) {
+  constexpr int kCols = HD / 4, kGroups = 256 / kCols;
+  __shared__ kv8_f4 so[kGroups][kCols];
+  __shared__ float2 sml[kGroups];
+  const Kv8Head head = *v.head;
+  if (head.rows > rows) return;
+  const int tid = threadIdx.x, col = tid % kCols, group = tid / kCols, d = col * 4, G = v.H / v.KVH, ys = v.KVH;
+  for (int i = blockIdx.x; i < head.joints * 32 * ys; i += gridDim.x) {
+    const int at = i / ys, y = i - at * ys;
+    const Kv8JointRow r = jv.rows[at];
+    if (r.t < 0) continue;
+    const Kv8Joint j = jv.joints[at >> 5];
+    const int parts = j.parts + r.parts;
+    float m = kKv8Lowest, l = 0.0f;
+    kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};       // an average, as in kv8_join
+    for (int k0 = group; k0 < parts; k0 += 4 * kGroups) {
+      float2 a[4];
+      kv8_f4 x[4];
+      float m2 = m;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int p = min(k0 + k * kGroups, parts - 1);
+        const bool common = p < j.parts;
+        const size_t e = ((size_t)(common ? j.slot + p : r.slot + p - j.parts) * ys + y) * 32 + (common ? at & 31 : r.row);
+        a[k] = v.part_ml[e];
+        x[k] = *(const kv8_f4*)(v.part_o + e * HD + d);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if (k0 + k * kGroups >= parts) a[k] = {kKv8Lowest, 0.0f};
+        m2 = __builtin_fmaxf(m2, a[k].x);
+      }
+      const float l0 = l * __builtin_amdgcn_exp2f(m - m2);
+      m = m2;
+      l = l0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        a[k].y *= __builtin_amdgcn_exp2f(a[k].x - m);
+        l += a[k].y;
+      }
+      const float il = l == 0.0f ? 0.0f : 1.0f / l;
+      o *= l0 * il;
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[k][c], a[k].y * il, o[c]);
+    }
+    __syncthreads();                           // the row before has been read
+    so[group][col] = o;
+    if (col == 0) sml[group] = {m, l};
+    __syncthreads();
+    if (group) continue;
+    const int used = min(parts, kGroups);
+    for (int k = 0; k < used; k++) m = __builtin_fmaxf(m, sml[k].x);
+    l = 0.0f;
+    o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < used; k++) l = __builtin_fmaf(sml[k].y, __builtin_amdgcn_exp2f(sml[k].x - m), l);
+    const float il = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int k = 0; k < used; k++) {
+      const float f = sml[k].y * il * __builtin_amdgcn_exp2f(sml[k].x - m);
+      const kv8_f4 x = so[k][col];
+      for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+    }
+    kv8_put4(out + (int64_t)r.t * out_stride + (y * G + r.h) * HD + d, wide, o);
   }
 }
 

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kKv8Chunk) void k_kv8_fork_commit(Kv8View v, Kv8For
   if (c == 0 && tid == 0) {
     Kv8Head h = *v.head;
     h.status = status;
-    h.rows = h.runs = h.items = h.tiles = 0;
+    h.rows = h.runs = h.items = h.tiles = h.joint_items = h.joints = 0;
     if (!status) {
       h.free_pages = free - w.copies;
       h.shared = w.entries > (uint64_t)(v.pages - h.free_pages);

@@ -298,6 +298,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   __syncthreads();
   const int free0 = head.free_pages;
   const uint64_t bad = sums[5];
+  head.joint_items = head.joints = 0;
   head.status = bad >> 32 ? KV8_TOO_LONG : bad ? KV8_BAD_LENGTH : sums[0] > (uint64_t)rows ? KV8_ROWS
                 : sums[1] > (uint64_t)v.pages && !head.shared ? KV8_PAGES : KV8_OK;
   int freed = total[0];
