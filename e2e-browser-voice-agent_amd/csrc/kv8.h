@@ -23,6 +23,11 @@ constexpr int kKv8Block = 32;
 // sequences of up to 16,000 positions: parts of at most 128 pages 225 us, as long as the aim asks 245.
 constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
+// Sequences are attended to together where that saves passes over so many pages of a kv head.  Together and one by one, us:
+// 64 sequences behind 300 positions (32 heads of 8 x 128, 4,000 pages saved) 19.6 and 15.0, behind 1,000 (13,900) 21.0 and 21.8, behind
+// 4,000 (56,000) 33.1 and 54.6; 32 of one to two rows behind 4,100 (12 of 2 x 128, 5,900) 19.1 and 23.0; 8 behind 131,072 (8 of 1 x 128,
+// 24,600) 26.2 and 55; 8 behind 4,000 (14 of 2 x 64, 1,500) 12.7 and 10.2.
+constexpr int kKv8JointSaves = 5500;
 // Joints of a step at most, which is 16,384 rows of attention: their sums take 32 * head_dim * 8 bytes a kv head each.
 constexpr int kKv8Joints = 512;
 constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
@@ -51,6 +56,7 @@ struct Kv8Head {
   int parts_of;    // pages from which on a unit's pages are shared among several items, and in parts of how many
   int shared;      // whether any page belongs to several sequences (else refs() means nothing)
   int joint_items, joints; // items of the list with joints and joints, 0 where there is no such list
+  int most_parts;  // of a row in a joint
 };
 enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE, KV8_SHARED, KV8_FORK_SOURCE, KV8_FORK_PAGES };
 
@@ -141,6 +147,9 @@ struct Kv8JointView {
   Kv8Item* items;
   Kv8Joint* joints;    // [most]
   Kv8JointRow* rows;   // [most][32]
+  int workgroups;      // of attention
+  int saves;           // pages of a kv head that joints have to save
+  int* queue;          // items of attention that have been drawn, 0 between launches
   int most;            // joints of a step.  The workspace's slots 0..most-1 are of joints in one part, rows of units in one part lie
                        // in the slots most..2 most-1 (32 each, as in the joints), other slots begin behind them
 };

@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <new>
 
 #include "host.h"
@@ -25,6 +26,10 @@ constexpr size_t kFillInPlan = 8192, kFillInPlanGlobal = 2048;
 // tiles of a step differ in length.)
 constexpr int64_t kMostWorkgroups = 8192;
 
+// Workgroups of attention with joints: two for each CU, as many as its registers hold.
+constexpr int kJointWorkgroups = 512;
+// Workgroups that add a step's joints up, at most; without any they cost 2 us.
+constexpr int64_t kGatherWorkgroups = 2048;
 // Workgroups of a fork's copies at most.
 constexpr int64_t kForkGrid = 4096;
 
@@ -240,7 +245,7 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v, Kv8ForkView f) {
     if (i < (size_t)v.B) { v.held[i] = 0; v.base[i] = 0; v.lens[i] = 0; }
   }
   if (i == 0) {
-    *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0, 0, 0};
+    *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0, 0, 0, 0};
     *f.fork = Kv8Fork{};
   }
 }
@@ -287,8 +292,13 @@ int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
   return rc;
 }
 
-// Whether a step's units may be joined: more than 16 rows of a kv head fill the matrix cores by themselves.
-bool joined(const q4hip_kv8* kv, int rows) { return kv->forked && kv->v.H / kv->v.KVH <= 16 && rows > 1 && kv->v.B > 1; }
+// Whether a step's units may be joined, if the plan finds that it is worth it: then there is a launch more, which costs 2.5 us where it
+// is not (4 answers of 14 heads, 2 x 64, behind 300 positions 5.9 us without and 11.7 together, behind 32,000 13.3 and 14.1).  More than 16
+// rows of a kv head fill the matrix cores by themselves.
+bool joined(const q4hip_kv8* kv, int rows) {
+  const int G = kv->v.H / kv->v.KVH;
+  return kv->forked && kv->j.most && rows > 1 && ((int64_t)rows * G > 32 || (int64_t)rows * kv->v.H >= 256 || !kv->j.saves);
+}
 
 int read_head(q4hip_kv8* kv, hipStream_t s) {
   HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
@@ -362,23 +372,23 @@ void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, v
   const bool wide = aligned16(q, q_stride, type) && aligned16(out, out_stride, type);
   const bool few = rows <= w.unit_rows;    // neither wide units nor tiles
   const bool joint = joined(kv, rows);
-  const int64_t work = (items + (joint ? std::min(units, kv->j.most) : 0)) * w.KVH * w.row_tiles +
-                       (few && !joint ? 0 : (int64_t)tiles_bound(w, rows) * w.KVH);
+  const int64_t work = items * w.KVH * w.row_tiles + (few ? 0 : (int64_t)tiles_bound(w, rows) * w.KVH);
   const unsigned grid = (unsigned)std::min<int64_t>(work, kMostWorkgroups);
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     if (joint) {
-      auto* fn = w.HD == 64 ? k_kv8_attend<64, T, 2, true> : k_kv8_attend<128, T, 2, true>;
-      fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide, kv->j);
+      auto* fn = w.HD == 64 ? k_kv8_attend_joint<64, T> : k_kv8_attend_joint<128, T>;
+      fn<<<(unsigned)std::min<int64_t>(work + (int64_t)std::min(units, kv->j.most) * w.KVH, kv->j.workgroups), 256, 0, s>>>(
+          w, kv->j, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide);
       // rows of joints, or less
       const int64_t most = std::min<int64_t>(32 * (int64_t)kv->j.most, (int64_t)rows * (w.H / w.KVH) + 31 * (rows / 2));
       auto* sum = w.HD == 64 ? k_kv8_gather<64, T> : k_kv8_gather<128, T>;
-      sum<<<(unsigned)std::min(most * w.KVH, kMostWorkgroups), 256, 0, s>>>(w, kv->j, (T*)out, out_stride, rows, wide);
+      sum<<<(unsigned)std::min<int64_t>(most * w.KVH, kGatherWorkgroups), 256, 0, s>>>(w, kv->j, (T*)out, out_stride, rows, wide);
       return;
     }
-    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0, false> : k_kv8_attend<64, T, 2, false>)
-                          : (few ? k_kv8_attend<128, T, 0, false> : k_kv8_attend<128, T, 2, false>);
-    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide, Kv8NoJoints{});
+    auto* fn = w.HD == 64 ? (few ? k_kv8_attend<64, T, 0> : k_kv8_attend<64, T, 2>)
+                          : (few ? k_kv8_attend<128, T, 0> : k_kv8_attend<128, T, 2>);
+    fn<<<grid, 256, 0, s>>>(w, layer, (const T*)q, (T*)out, q_stride, out_stride, log2_scale, rows, wide);
   });
 }
 
@@ -416,7 +426,7 @@ void q4hip_kv8_destroy(q4hip_kv8* kv) {
   Kv8View& v = kv->v;
   void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
                   kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived,
-                  kv->j.items, kv->j.joints, kv->j.rows, kv->joint_scratch};
+                  kv->j.items, kv->j.joints, kv->j.rows, kv->j.queue, kv->joint_scratch};
   for (void* p : bufs) if (p) (void)hipFree(p);
   if (kv->pin) (void)hipHostFree(kv->pin);
   if (kv->stream) (void)hipStreamDestroy(kv->stream);
@@ -483,6 +493,11 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
     al(&kv->j.items, max_rows + most_items + kv->j.most);
     al(&kv->j.joints, kv->j.most);
     al(&kv->j.rows, (size_t)32 * kv->j.most);
+    kv->j.workgroups = kJointWorkgroups;
+    const char* saves = getenv("Q4HIP_KV8_JOINT_SAVES");
+    kv->j.saves = saves ? atoi(saves) : kKv8JointSaves;
+    al(&kv->j.queue, 1);
+    if (e == hipSuccess) e = hipMemsetAsync(kv->j.queue, 0, sizeof(int), kv->stream);
     if (seqs > kPlanShared) al(&kv->joint_scratch, (size_t)kJointArrays * seqs);
   }
   // units in several parts: each has more pages than a part, so that the last one's part at most doubles them

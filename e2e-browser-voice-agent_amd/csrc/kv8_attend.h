@@ -40,8 +40,6 @@
 // formed beside the weights of the page before (fp16 head_dim 64 5% faster, head_dim 128 out of registers and 2% slower, fp32 7%
 // slower).
 #pragma once
-#include <type_traits>
-
 #include "kv8.h"
 
 namespace q4 {
@@ -438,7 +436,12 @@ __device__ inline void kv8_send_part(const Kv8View& v, size_t slot, int row, int
   if (d == 0) kv8_send((float*)(v.part_ml + slot * 32 + row), m, l);
 }
 
-struct Kv8NoJoints {};
+// The same for the launch behind this one, which no other XCD's access needs to get past a cache for.
+template <int HD>
+__device__ inline void kv8_keep_part(const Kv8View& v, size_t slot, int row, int d, kv8_f4 o, float m, float l) {
+  *(kv8_f4*)(v.part_o + (slot * 32 + row) * HD + d) = o;
+  if (d == 0) v.part_ml[slot * 32 + row] = {m, l};
+}
 
 template <int HD>
 struct Kv8Shared {
@@ -521,9 +524,11 @@ __device__ __forceinline__ void kv8_item(const Kv8View& v, const Kv8JointView& j
         for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c] * il, f, o[c]);
       }
       if (joint && !common && it.parts == 1) {
-        const int at = it.row + row;
-        kv8_send_part<HD>(v, (size_t)(jv.most + (at >> 5)) * ys + y, at & 31, d, o, r, l);
-      } else if (it.parts == 1 && !joint) write(t * 16 + row, d, o);
+        const int at = it.row + t * 16 + row;
+        kv8_keep_part<HD>(v, (size_t)(jv.most + (at >> 5)) * ys + y, at & 31, d, o, r, l);
+      } else if (joint) {
+        kv8_keep_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, r, l);
+      } else if (it.parts == 1) write(t * 16 + row, d, o);
       else kv8_send_part<HD>(v, slot + (size_t)it.part * ys, t * 16 + row, d, o, r, l);
     }
   }
@@ -588,11 +593,10 @@ __device__ __forceinline__ void kv8_tile(const Kv8View& v, int layer, const T* q
 }
 
 // A step's tiles, the longest first, then its items.  The kv heads are neighbours in the grid, so that the tiles of one
-// meet on the same XCDs and find its pages in their L2.  kJoint: of the list with joints, if the plan has made one.
-template <int HD, class T, int N, bool kJoint>
+// meet on the same XCDs and find its pages in their L2.
+template <int HD, class T, int N>
 __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, const T* __restrict__ q, T* __restrict__ out,
-                                                    int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide,
-                                                    std::conditional_t<kJoint, Kv8JointView, Kv8NoJoints> jv) {
+                                                    int64_t q_stride, int64_t out_stride, float scale, int rows, bool wide) {
   __shared__ Kv8Shared<HD> sh;
   const int ys = v.KVH * v.row_tiles;
   const Kv8Head head = *v.head;
@@ -602,14 +606,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, con
     if (threadIdx.x == 0) v.head->status = KV8_STALE;
     return;
   }
-  const Kv8Item* items = v.items;
-  int n = head.items;
-  Kv8JointView j = {};
-  if constexpr (kJoint) {
-    j = jv;
-    if (head.joint_items) { items = jv.items; n = head.joint_items; }
-  }
-  const int tiles = N ? head.tiles * v.KVH : 0, all = tiles + n * ys;
+  const int tiles = N ? head.tiles * v.KVH : 0, all = tiles + head.items * ys;
   for (int i = blockIdx.x; i < all; i += gridDim.x) {
     if constexpr (N > 0)
       if (i < tiles) {
@@ -617,19 +614,55 @@ __global__ __launch_bounds__(256, 2) void k_kv8_attend(Kv8View v, int layer, con
         continue;
       }
     const int k = i - tiles, y = k % ys;
-    if (N > 0 || i != (int)blockIdx.x) it = items[k / ys];
+    if (N > 0 || i != (int)blockIdx.x) it = v.items[k / ys];
     if constexpr (N > 0)
       if (it.wide) {
-        kv8_item<HD, T, N, kJoint>(v, j, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+        kv8_item<HD, T, N, false>(v, {}, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
         continue;
       }
-    kv8_item<HD, T, 1, kJoint>(v, j, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
+    kv8_item<HD, T, 1, false>(v, {}, it, sh, layer, q, out, q_stride, out_stride, scale, wide, y);
   }
 }
 
-// The rows of joints: a workgroup adds up a row's parts, of its joint and of its unit, a group of threads every so-manieth one.
+// The same from the list with joints, if the plan has made one.  Its items differ in length by a factor of ten, and a grid's
+// workgroups go to the 4 shader engines of an XCD one after the other, whatever these still hold: 512 items of joints beside as many
+// short ones ran on half of the CUs.  So as many workgroups as fit stay, and draw an item when they are done with one.  (Drawn a turn
+// ahead, an item waits for its workgroup's long one beside idle ones.)
+template <int HD, class T>
+__global__ __launch_bounds__(256, 2) void k_kv8_attend_joint(Kv8View v, Kv8JointView jv, int layer, const T* __restrict__ q,
+                                                          T* __restrict__ out, int64_t q_stride, int64_t out_stride, float scale,
+                                                          int rows, bool wide) {
+  __shared__ Kv8Shared<HD> sh;
+  __shared__ int drawn;
+  const int ys = v.KVH * v.row_tiles, tid = threadIdx.x;
+  const Kv8Head head = *v.head;
+  if (head.rows > rows) {
+    if (tid == 0) v.head->status = KV8_STALE;
+    return;
+  }
+  const Kv8Item* const items = head.joint_items ? jv.items : v.items;
+  const int tiles = head.tiles * v.KVH, all = tiles + (head.joint_items ? head.joint_items : head.items) * ys;
+  for (int i = blockIdx.x; i < all;) {
+    if (i < tiles) {
+      kv8_tile<HD, T, 2>(v, layer, q, out, q_stride, out_stride, scale, wide, i / v.KVH, i % v.KVH);
+    } else {
+      const int k = i - tiles;
+      const Kv8Item it = items[k / ys];
+      if (it.wide) kv8_item<HD, T, 2, true>(v, jv, it, sh, layer, q, out, q_stride, out_stride, scale, wide, k % ys);
+      else kv8_item<HD, T, 1, true>(v, jv, it, sh, layer, q, out, q_stride, out_stride, scale, wide, k % ys);
+    }
+    if (all <= (int)gridDim.x) return;
+    __syncthreads();                           // everybody has read `drawn`
+    if (tid == 0) drawn = gridDim.x + __hip_atomic_fetch_add(jv.queue, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    i = __builtin_amdgcn_readfirstlane(drawn);
+  }
+}
+
+// The rows of joints: threads of a row take 4 columns each, of every so-manieth part of its joint and its unit, so that each has about
+// four to load; what they have is added up in shared memory.
 // (The last workgroup to be done could, too, as it does for units: but it alone then reads up to 128 parts of 32 rows.  8 sequences
-// behind 131,072 positions: 41.3 us so, 25.2 now.)
+// behind 131,072 positions: 41.3 us so, 26.2 in a launch of its own.)
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_kv8_gather(Kv8View v, Kv8JointView jv, T* __restrict__ out, int64_t out_stride, int rows,
                                                     bool wide) {
@@ -638,22 +671,25 @@ __global__ __launch_bounds__(256) void k_kv8_gather(Kv8View v, Kv8JointView jv, 
   __shared__ float2 sml[kGroups];
   const Kv8Head head = *v.head;
   if (head.rows > rows) return;
-  const int tid = threadIdx.x, col = tid % kCols, group = tid / kCols, d = col * 4, G = v.H / v.KVH, ys = v.KVH;
-  for (int i = blockIdx.x; i < head.joints * 32 * ys; i += gridDim.x) {
-    const int at = i / ys, y = i - at * ys;
+  int slices = 1;
+  while (slices < kGroups && 4 * slices < head.most_parts) slices *= 2;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *jv.queue = 0;
+  const int tid = threadIdx.x, col = tid % kCols, mine = tid / kCols, group = mine % slices, d = col * 4, G = v.H / v.KVH, ys = v.KVH;
+  const int each = kGroups / slices, all = head.joints * 32 * ys;
+  for (int i0 = blockIdx.x * each; i0 < all; i0 += gridDim.x * each) {
+    const int i = min(i0 + mine / slices, all - 1), at = i / ys, y = i - at * ys;
     const Kv8JointRow r = jv.rows[at];
-    if (r.t < 0) continue;
     const Kv8Joint j = jv.joints[at >> 5];
-    const int parts = j.parts + r.parts;
+    const int parts = r.t < 0 ? 0 : j.parts + r.parts;
     float m = kKv8Lowest, l = 0.0f;
     kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};       // an average, as in kv8_join
-    for (int k0 = group; k0 < parts; k0 += 4 * kGroups) {
+    for (int k0 = group; k0 < parts; k0 += 4 * slices) {
       float2 a[4];
       kv8_f4 x[4];
       float m2 = m;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int p = min(k0 + k * kGroups, parts - 1);
+        const int p = min(k0 + k * slices, parts - 1);
         const bool common = p < j.parts;
         const size_t e = ((size_t)(common ? j.slot + p : r.slot + p - j.parts) * ys + y) * 32 + (common ? at & 31 : r.row);
         a[k] = v.part_ml[e];
@@ -661,7 +697,7 @@ __global__ __launch_bounds__(256) void k_kv8_gather(Kv8View v, Kv8JointView jv, 
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        if (k0 + k * kGroups >= parts) a[k] = {kKv8Lowest, 0.0f};
+        if (k0 + k * slices >= parts) a[k] = {kKv8Lowest, 0.0f};
         m2 = __builtin_fmaxf(m2, a[k].x);
       }
       const float l0 = l * __builtin_amdgcn_exp2f(m - m2);
@@ -678,21 +714,25 @@ __global__ __launch_bounds__(256) void k_kv8_gather(Kv8View v, Kv8JointView jv, 
       for (int k = 0; k < 4; k++)
         for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[k][c], a[k].y * il, o[c]);
     }
-    __syncthreads();                           // the row before has been read
-    so[group][col] = o;
-    if (col == 0) sml[group] = {m, l};
-    __syncthreads();
-    if (group) continue;
-    const int used = min(parts, kGroups);
-    for (int k = 0; k < used; k++) m = __builtin_fmaxf(m, sml[k].x);
-    l = 0.0f;
-    o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < used; k++) l = __builtin_fmaf(sml[k].y, __builtin_amdgcn_exp2f(sml[k].x - m), l);
-    const float il = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int k = 0; k < used; k++) {
-      const float f = sml[k].y * il * __builtin_amdgcn_exp2f(sml[k].x - m);
-      const kv8_f4 x = so[k][col];
-      for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+    if (slices > 1) {
+      __syncthreads();                         // the rows before have been read
+      so[mine][col] = o;
+      if (col == 0) sml[mine] = {m, l};
+      __syncthreads();
+    }
+    if (group || !parts) continue;
+    if (slices > 1) {
+      const int used = min(parts, slices);
+      for (int k = 0; k < used; k++) m = __builtin_fmaxf(m, sml[mine + k].x);
+      l = 0.0f;
+      o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k = 0; k < used; k++) l = __builtin_fmaf(sml[mine + k].y, __builtin_amdgcn_exp2f(sml[mine + k].x - m), l);
+      const float il = l == 0.0f ? 0.0f : 1.0f / l;
+      for (int k = 0; k < used; k++) {
+        const float f = sml[mine + k].y * il * __builtin_amdgcn_exp2f(sml[mine + k].x - m);
+        const kv8_f4 x = so[mine + k][col];
+        for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], f, o[c]);
+      }
     }
     kv8_put4(out + (int64_t)r.t * out_stride + (y * G + r.h) * HD + d, wide, o);
   }

@@ -12,7 +12,7 @@
 namespace q4 {
 
 constexpr int kJointThreads = 1024;
-// Pages in common from which on units are joined.
+// A group has at least so many pages in common.
 constexpr int kJointPages = 8;
 
 // Sums over the threads before, and over all; `store` is shared memory.  Every thread calls it.
@@ -50,7 +50,8 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   __shared__ uint32_t store[4][kJointThreads / 64];
   __shared__ int4 chunk[kJointThreads / 4], added[kJointThreads / 4];
   __shared__ unsigned long long pages_all;
-  __shared__ int joints_all;
+  __shared__ int joints_all, most_parts, most_own;      // parts of a group's pages, of a member's own
+  __shared__ unsigned long long saved;                  // pages that the groups' members need not pass over by themselves
   const Kv8Head head = *v.head;
   if (!head.shared || !head.rows) return;
   const int tid = threadIdx.x, lane = tid & 63, G = v.H / v.KVH, B = v.B;
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
     common[b] = n;
     count[b] = total[b] = 0;
   }
-  if (tid == 0) pages_all = joints_all = 0;
+  if (tid == 0) pages_all = saved = joints_all = most_parts = most_own = 0;
   __syncthreads();
   for (int b = tid; b < B; b += kJointThreads)
     if (lead[b] == b) v.first()[page0(b)] = INT32_MAX;
@@ -132,13 +133,16 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
       joint_at[b] = (int)(sum[1] + x[1]);
       // groups that there is no room for stay as they are, and so do those behind them
       if (!n || joint_at[b] + n > jv.most) count[b] = 0;
-      else atomicMax(&joints_all, joint_at[b] + n);
+      else {
+        atomicMax(&joints_all, joint_at[b] + n);
+        atomicAdd(&saved, (unsigned long long)(in(count + b) - n) * in(common + b));
+      }
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) sum[k] += all[k];
   }
   __syncthreads();
-  if (!joints_all) return;
+  if (!joints_all || (int64_t)saved * v.KVH < jv.saves) return;
   // pages that a sequence's units do not look at themselves
   auto skipped = [&](int b) { return lead[b] >= 0 && in(count + lead[b]) ? in(common + lead[b]) : 0; };
   const bool in_tiles = head.tiles > 0;
@@ -162,8 +166,10 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
         const int parts = kv8_parts(in(common + b), parts_of);
         x[0] = joints_of(b) * parts;
         x[1] = parts > 1 ? x[0] : 0;
+        atomicMax(&most_parts, parts);
       }
       const int parts = kv8_parts(kv8_pages(have[b] + add[b]) - skipped(b), parts_of);
+      if (skipped(b)) atomicMax(&most_own, parts);
       x[2] = units_of(b) * parts;
       x[3] = parts > 1 ? x[2] : 0;
     }
@@ -179,9 +185,6 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   }
   __syncthreads();
   const int slots = 2 * jv.most, commons = (int)at[0], items = (int)(at[0] + at[2]);
-  // workgroups of the same XCD (every eighth): the joints of a group meet there over the same pages
-  int turn = 8;
-  while (turn > 1 && (turn / 2 * v.KVH) % 8 == 0) turn /= 2;
   for (int b = tid; b < B; b += kJointThreads) {
     const int a = lead[b];
     if (a < 0 || !in(count + a)) continue;
@@ -198,11 +201,29 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
       for (int r = in(total + b) * G; r < joints * 32; r++) jv.rows[joint_at[b] * 32 + r].t = -1;
     }
   }
-  for (int i = tid; i < items; i += kJointThreads) {
+  // The joints' items, which compute and are the longest, come first; and if not all of the list fits on the GPU, the units', which
+  // load, in turn with them until there are no more of one kind.  `turn`: items after which an XCD's turn comes again; a run of one
+  // kind goes over its 4 shader engines, too, which take workgroups one after the other, whatever these still hold (in turn XCD by
+  // XCD, 512 items of joints ran on half of the CUs).
+  int turn = 8;
+  while (turn > 1 && turn / 2 * v.KVH % 8 == 0) turn /= 2;
+  const int run = 4 * turn, pairs = (int64_t)items * v.KVH > jv.workgroups ? min(commons, items - commons) / run : 0;
+  for (int n = tid; n < items; n += kJointThreads) {
     Kv8Item e{};
-    if (i < commons) {
+    const int at_run = n / run;
+    bool is_common;
+    int i;                                     // the number of its kind
+    if (at_run < 2 * pairs) {
+      is_common = at_run % 2 == 0;
+      i = n - (at_run + 1) / 2 * run;
+    } else {
+      i = n - pairs * run;
+      is_common = i < commons;
+      if (!is_common) i += pairs * run - commons;
+    }
+    if (is_common) {
       const int b = find(common_at, B, i), k = i - common_at[b], joints = joints_of(b), parts = kv8_parts(in(common + b), parts_of);
-      // joint by joint, `turn` parts of each in turn
+      // `turn` parts of each one in turn: the group's joints meet on the same XCD over the same pages
       const int block = k / (turn * joints), width = min(turn, parts - block * turn), rest = k - block * turn * joints;
       const int joint = rest / width, pages_in = in(common + b), per = (pages_in + parts - 1) / parts;
       e.seq = b;
@@ -215,15 +236,15 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
       e.slot = parts > 1 ? slots + common_slot[b] + joint * parts : joint_at[b] + joint;
       e.joint = joint_at[b] + joint + 1;
     } else {
-      const int j = i - commons, b = find(item_at, B, j), k = j - item_at[b], h = have[b], n = add[b], skip = skipped(b);
-      const int parts = kv8_parts(kv8_pages(h + n) - skip, parts_of), rows = kv8_unit_rows(v, n), u = k / parts;
+      const int b = find(item_at, B, i), k = i - item_at[b], h = have[b], more = add[b], skip = skipped(b);
+      const int parts = kv8_parts(kv8_pages(h + more) - skip, parts_of), rows = kv8_unit_rows(v, more), u = k / parts;
       e.seq = b;
       e.part = k - u * parts;
       e.parts = parts;
       e.t = start[b] + u * rows;
-      e.n = min(rows, n - u * rows);
+      e.n = min(rows, more - u * rows);
       e.pos = h + u * rows;
-      e.wide = n > v.unit_rows;
+      e.wide = more > v.unit_rows;
       const int all = kv8_pages(e.pos + e.n) - skip, per = (all + parts - 1) / parts;
       e.page0 = min(e.part * per, all);
       e.pages = min(per, all - e.page0);
@@ -234,11 +255,12 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
         e.row = joint_at[lead[b]] * 32 + before_of[b] * G;
       }
     }
-    jv.items[i] = e;
+    jv.items[n] = e;
   }
   if (tid == 0) {
     v.head->joint_items = items;
     v.head->joints = joints_all;
+    v.head->most_parts = most_parts + most_own;
   }
 }
 

@@ -11,6 +11,12 @@ from test_gpu_kv8_fork import Forked
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def join_all(monkeypatch):
+    """However little it saves."""
+    monkeypatch.setenv("Q4HIP_KV8_JOINT_SAVES", "0")
+
+
 def grown(rng, H, KVH, hd, prefixes, dtype, own=40, spare=0, layers=1, max_rows=4000):
     """Groups of sequences: prefixes is [(positions, sequences)]; every sequence then adds up to `own` rows of its own."""
     B = sum(n for _, n in prefixes) + spare
@@ -190,3 +196,15 @@ def test_captured(late):
             t.plan(lens, [1] * B)
             t.attend(rng, "f32")
             lens = [n + 1 for n in lens]
+
+
+@pytest.mark.parametrize("H,KVH,hd,positions,seqs", [(20, 20, 64, 700, 40), (4, 2, 64, 300, 3)])
+def test_by_what_it_saves(monkeypatch, H, KVH, hd, positions, seqs):
+    """As a program has it: one case that is worth it, one that is not."""
+    monkeypatch.delenv("Q4HIP_KV8_JOINT_SAVES")
+    rng = np.random.default_rng(15)
+    t, lens = grown(rng, H, KVH, hd, [(positions, seqs)], "f16", max_rows=2000)
+    for _ in range(2):
+        t.grow(rng, lens, [1] * seqs, "f16")
+        t.attend(rng, "f16")
+        lens = [n + 1 for n in lens]
