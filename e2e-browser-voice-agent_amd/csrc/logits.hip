@@ -1,13 +1,16 @@
 // logits.hip -- penalties, biases and masks on rows of logits, and the best token of each (include/q4hip.h, q4hip_logits_*).
 //
-// A workgroup takes a piece of a row: kLogitsThreads * N tokens, N of them in each thread's registers.  How often the row's history
+// A workgroup takes a piece of a row: a block of threads with N tokens of each in registers.  How often the row's history
 // has each of these is counted in shared memory (whole numbers: any order of the additions gives the same), then the biases' last
-// entries are found there the same way, and a thread looks up its own tokens.  So a row's logits are read and written once,
-// no counts of the whole vocabulary lie in memory, and one launch does all of it; the history is read once for every piece, from the
+// entries are found there the same way, over the counts, and a thread looks up its own tokens.  So a row's logits are read and written
+// once, no counts of the whole vocabulary lie in memory, and one launch does all of it; the history is read once for every piece, from the
 // L2.  The best token: the largest of (value, lowest token first) as whole numbers of 64 bits, joined over the pieces by an
 // atomic maximum, which the row's last piece reads and clears.
-// One row of 151,936 fp32 logits takes 6.1 us, 64 rows (bf16) with up to 4,000 tokens of history 27.5, 256 rows (fp32) with up to
-// 16,000 115: the passes over the history beside the bytes.
+//
+// What bounds it.  One row of 151,936 fp32 logits: the launch and a chain of loads, 6.0 us.  256 rows (fp32) with 2,000 to 16,000 tokens
+// of history: bytes, 311 MB in 84.8 us, 3.7 TB/s, beside 19 passes over each history.  64 rows (bf16) with up to 4,000 tokens and 40
+// biases: 25.1 us, of which 14 are left without lists: each list is a load that waits for the row's rules, and a barrier.
+// Not kept: looking nothing up in pieces that no entry falls into (256 rows 97 us: nearly all have one).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -25,13 +28,16 @@ struct q4hip_logits {
 namespace q4 {
 namespace {
 
-// Tokens of a piece: large ones where the rows fill the GPU, as every piece reads the whole history.
+// Tokens of a piece: large ones where the rows fill the GPU, as every piece reads the whole history.  (64 rows in small pieces 45 us, in
+// 256 * 16 tokens 27.5, in 256 * 32 27.8; 256 rows in 256 * 16 106, in 256 * 32 112.)
 constexpr int kSmallThreads = 256, kSmallEach = 8, kLargeThreads = 512, kLargeEach = 16;
 constexpr int kLargeFrom = 512;         // large pieces from which on they are taken
 
-// x as a whole number in the order of the values: NaN and -inf 0, -0 as +0.
+// Entries of a list at most: counts and the biases' numbers share a word.
+constexpr int kMostEntries = 1 << 30;
+
+// x as a whole number in the order of the values, -0 as +0.
 __device__ inline uint32_t order_of(float x) {
-  if (!(x > -__builtin_inff())) return 0;
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
@@ -72,32 +78,41 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
       for (int k = 0; k < V; k++) value[s * V + k] = (float)w.e[k];
     } else {
 #pragma unroll
-      for (int k = 0; k < V; k++) value[s * V + k] = at + k < n ? (float)from[at + k] : 0.0f;
+      for (int k = 0; k < V; k++) value[s * V + k] = at + k < n ? (float)from[at + k] : -__builtin_inff();
     }
   }
-  auto fill = [&](int with) {
-    for (int i = tid; i < kPiece / 4; i += kThreads) ((int4*)table)[i] = int4{with, with, with, with};
-  };
   // entries [begin, end) of a list of `all`, none where they are not in order
   auto bounds = [](int64_t begin, int64_t end, int64_t all, int64_t& lo, int64_t& hi) {
     lo = begin < 0 ? 0 : begin;
     hi = end > all ? all : end;
   };
-  int64_t lo, hi;
-  bounds(p.history_begin, p.history_end, c.history_n, lo, hi);
-  if (lo < hi) {
-    fill(0);
-    __syncthreads();
-    for (int64_t i = lo + tid; i < hi; i += kThreads) {
-      const uint32_t at = (uint32_t)c.history[i] - (uint32_t)first;
-      if (at < (uint32_t)n) atomicAdd(&table[at], 1);
+  // f(entry, place in the piece) of a list's entries that are of the piece; four loads on their way at once
+  auto scan = [&](int64_t lo, int64_t hi, auto token, auto f) {
+    for (int64_t i = lo + tid; i < hi; i += 4 * kThreads) {
+      uint32_t at[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) at[u] = (uint32_t)token(min(i + u * kThreads, hi - 1)) - (uint32_t)first;
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (at[u] < (uint32_t)n && i + u * kThreads < hi) f(i + u * kThreads, at[u]);
     }
     __syncthreads();
+  };
+  auto entry = [&](int s, int k) { return table[(s * kThreads + tid) * V + k]; };
+  int64_t lo, hi, bias_lo, bias_hi;
+  bounds(p.history_begin, p.history_end, c.history_n, lo, hi);
+  bounds(p.bias_begin, p.bias_end, c.biases_n, bias_lo, bias_hi);
+  if (lo < hi || bias_lo < bias_hi) {
+    for (int i = tid; i < kPiece / 4; i += kThreads) ((int4*)table)[i] = int4{0, 0, 0, 0};
+    __syncthreads();
+  }
+  if (lo < hi) {
+    scan(lo, hi, [&](int64_t i) { return c.history[i]; }, [&](int64_t, uint32_t at) { atomicAdd(&table[at], 1); });
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
 #pragma unroll
       for (int k = 0; k < V; k++) {
-        const int times = table[(s * kThreads + tid) * V + k];
+        const int times = entry(s, k);
         float& v = value[s * V + k];
         if (times) {
           const float t = p.frequency * (float)times;
@@ -105,52 +120,56 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
           v = v - (t + p.presence);
         }
       }
-    __syncthreads();
+    if (bias_lo < bias_hi) __syncthreads();
   }
-  bounds(p.bias_begin, p.bias_end, c.biases_n, lo, hi);
-  if (lo < hi) {
-    fill(-1);
-    __syncthreads();
-    for (int64_t i = lo + tid; i < hi; i += kThreads) {
-      const uint32_t at = (uint32_t)c.biases[i].token - (uint32_t)first;
-      if (at < (uint32_t)n) atomicMax(&table[at], (int)(i - lo));
-    }
-    __syncthreads();
+  if (bias_lo < bias_hi) {
+    // over the counts: any bias' number is larger than these
+    scan(bias_lo, bias_hi, [&](int64_t i) { return c.biases[i].token; },
+         [&](int64_t i, uint32_t at) { atomicMax(&table[at], kMostEntries + (int)(i - bias_lo)); });
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
 #pragma unroll
       for (int k = 0; k < V; k++) {
-        const int e = table[(s * kThreads + tid) * V + k];
-        if (e >= 0) value[s * V + k] += c.biases[lo + e].value;
+        const int e = entry(s, k);
+        if (e >= kMostEntries) value[s * V + k] += c.biases[bias_lo + e - kMostEntries].value;
       }
   }
   const uint32_t* const mask = p.mask >= 0 && p.mask < c.mask_rows ? c.mask + (int64_t)p.mask * c.words : nullptr;
-  unsigned long long top = 0;
+  float most = -__builtin_inff();            // of the thread's values, the first of the largest, and its place
+  int where = 0;
 #pragma unroll
   for (int s = 0; s < kSteps; s++) {
     const int at = (s * kThreads + tid) * V;
     uint32_t bits = ~0u;
     if (mask && at < n) bits = mask[(first + at) >> 5] >> ((first + at) & 31);
-    Vec w;
 #pragma unroll
     for (int k = 0; k < V; k++) {
-      const float v = bits >> k & 1 ? value[s * V + k] : -__builtin_inff();
-      w.e[k] = (T)v;
-      if (c.best && at + k < n) {
-        const uint32_t o = order_of(v);
-        const unsigned long long here = o ? (unsigned long long)o << 32 | (uint32_t)~(first + at + k) : 0;
-        top = here > top ? here : top;
-      }
-    }
-    if (at + V <= n) {
-      *(Vec*)(to + at) = w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; k++)
-        if (at + k < n) to[at + k] = w.e[k];
+      float& v = value[s * V + k];
+      v = bits >> k & 1 ? v : -__builtin_inff();
+      if (v > most) { most = v; where = at + k; }
     }
   }
-  if (!c.best) return;
+  auto store = [&] {
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      const int at = (s * kThreads + tid) * V;
+      Vec w;
+#pragma unroll
+      for (int k = 0; k < V; k++) w.e[k] = (T)value[s * V + k];
+      if (at + V <= n) {
+        *(Vec*)(to + at) = w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k++)
+          if (at + k < n) to[at + k] = w.e[k];
+      }
+    }
+  };
+  if (!c.best) {
+    store();
+    return;
+  }
+  unsigned long long top = most > -__builtin_inff() ? (unsigned long long)order_of(most) << 32 | (uint32_t)~(first + where) : 0;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const unsigned long long other = __shfl_xor(top, d);
@@ -158,14 +177,19 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
   }
   if ((tid & 63) == 0) tops[tid >> 6] = top;
   __syncthreads();
-  if (tid) return;
+  unsigned long long before = 0;
+  if (tid == 0) {
 #pragma unroll
-  for (int i = 1; i < kThreads / 64; i++) top = tops[i] > top ? tops[i] : top;
+    for (int i = 1; i < kThreads / 64; i++) top = tops[i] > top ? tops[i] : top;
+    if (c.pieces > 1) before = __hip_atomic_fetch_max(c.top + row, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  store();                                   // the maximum is on its way meanwhile
+  if (tid) return;
   if (c.pieces > 1) {
-    // the maximum is in memory before the arrival: it has returned the one before
-    const unsigned long long before = __hip_atomic_fetch_max(c.top + row, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::"v"(before) : "memory");
-    if (__hip_atomic_fetch_add(c.arrived + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != c.pieces - 1) return;
+    // the maximum is in memory before the arrival: its value before has come back
+    int one = 1;
+    asm volatile("" : "+v"(one) : "v"(before));
+    if (__hip_atomic_fetch_add(c.arrived + row, one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != c.pieces - 1) return;
     top = __hip_atomic_exchange(c.top + row, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(c.arrived + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
@@ -230,7 +254,7 @@ int q4hip_logits_run(q4hip_logits* lg, const void* x, void* y, int type, int64_t
   if (rows < 0 || rows > lg->max_rows) return fail(Q4HIP_EINVAL, "%d rows: up to %d", rows, lg->max_rows);
   if (history_n < 0 || biases_n < 0 || mask_rows < 0 || (history_n && !history) || (biases_n && !biases) || (mask_rows && !mask))
     return fail(Q4HIP_EINVAL, "%lld tokens of history, %lld biases, %d masks", (long long)history_n, (long long)biases_n, mask_rows);
-  if (history_n > INT32_MAX || biases_n > INT32_MAX) return fail(Q4HIP_EINVAL, "lists of up to 2^31 entries");
+  if (history_n >= kMostEntries || biases_n >= kMostEntries) return fail(Q4HIP_EINVAL, "lists of less than 2^30 entries");
   if (!rows) return Q4HIP_OK;
   HIPCHK(hipSetDevice(lg->device));
   const int V = lg->vocab, words = (V + 31) / 32;
