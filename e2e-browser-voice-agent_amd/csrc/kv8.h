@@ -28,8 +28,8 @@ constexpr int kKv8TileRows = 128;
 // 4,000 (56,000) 33.1 and 54.6; 32 of one to two rows behind 4,100 (12 of 2 x 128, 5,900) 19.1 and 23.0; 8 behind 131,072 (8 of 1 x 128,
 // 24,600) 26.2 and 55; 8 behind 4,000 (14 of 2 x 64, 1,500) 12.7 and 10.2.
 constexpr int kKv8JointSaves = 5500;
-// Joints of a step at most, which is 16,384 rows of attention: their sums take 32 * head_dim * 8 bytes a kv head each.
-constexpr int kKv8Joints = 512;
+// Joints of a step at most, which is 8,192 rows of attention of a kv head: two slots of 128 * head_dim bytes a kv head for each.
+constexpr int kKv8Joints = 256;
 constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups; else in units, whose pages can be shared.  Tiles and units, us: 2,048 rows of 14 heads (fp32)

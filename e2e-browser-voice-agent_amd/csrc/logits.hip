@@ -8,8 +8,8 @@
 // atomic maximum, which the row's last piece reads and clears.
 //
 // What bounds it.  One row of 151,936 fp32 logits: the launch and a chain of loads, 6.0 us.  256 rows (fp32) with 2,000 to 16,000 tokens
-// of history: bytes, 311 MB in 84.8 us, 3.7 TB/s, beside 19 passes over each history.  64 rows (bf16) with up to 4,000 tokens and 40
-// biases: 25.1 us, of which 14 are left without lists: each list is a load that waits for the row's rules, and a barrier.
+// of history: bytes, 311 MB in 82.0 us, 3.8 TB/s, beside 19 passes over each history.  64 rows (bf16) with up to 4,000 tokens and 40
+// biases: 25.3 us, of which 14 are left without lists: 1,216 workgroups, where 1,024 fit, with up to four barriers each.
 // Not kept: looking nothing up in pieces that no entry falls into (256 rows 97 us: nearly all have one).
 #include <hip/hip_runtime.h>
 
@@ -98,10 +98,20 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
     }
     __syncthreads();
   };
+  // of the lists behind, what is waited for: the mask's words, and the first biases of each thread, on their way at once with the history
+  const uint32_t* const mask = p.mask >= 0 && p.mask < c.mask_rows ? c.mask + (int64_t)p.mask * c.words : nullptr;
+  uint32_t bits[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; s++) {
+    const int at = (s * kThreads + tid) * V;
+    bits[s] = mask && at < n ? mask[(first + at) >> 5] : ~0u;
+  }
   auto entry = [&](int s, int k) { return table[(s * kThreads + tid) * V + k]; };
   int64_t lo, hi, bias_lo, bias_hi;
   bounds(p.history_begin, p.history_end, c.history_n, lo, hi);
   bounds(p.bias_begin, p.bias_end, c.biases_n, bias_lo, bias_hi);
+  q4hip_logits_bias bias{-1, 0.0f};            // the thread's first
+  if (bias_lo + tid < bias_hi) bias = c.biases[bias_lo + tid];
   if (lo < hi || bias_lo < bias_hi) {
     for (int i = tid; i < kPiece / 4; i += kThreads) ((int4*)table)[i] = int4{0, 0, 0, 0};
     __syncthreads();
@@ -124,7 +134,9 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
   }
   if (bias_lo < bias_hi) {
     // over the counts: any bias' number is larger than these
-    scan(bias_lo, bias_hi, [&](int64_t i) { return c.biases[i].token; },
+    const uint32_t at = (uint32_t)bias.token - (uint32_t)first;
+    if (at < (uint32_t)n) atomicMax(&table[at], kMostEntries + tid);
+    scan(bias_lo + kThreads, bias_hi, [&](int64_t i) { return c.biases[i].token; },
          [&](int64_t i, uint32_t at) { atomicMax(&table[at], kMostEntries + (int)(i - bias_lo)); });
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
@@ -134,18 +146,16 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsCall c, const T* x, T
         if (e >= kMostEntries) value[s * V + k] += c.biases[bias_lo + e - kMostEntries].value;
       }
   }
-  const uint32_t* const mask = p.mask >= 0 && p.mask < c.mask_rows ? c.mask + (int64_t)p.mask * c.words : nullptr;
   float most = -__builtin_inff();            // of the thread's values, the first of the largest, and its place
   int where = 0;
 #pragma unroll
   for (int s = 0; s < kSteps; s++) {
     const int at = (s * kThreads + tid) * V;
-    uint32_t bits = ~0u;
-    if (mask && at < n) bits = mask[(first + at) >> 5] >> ((first + at) & 31);
+    const uint32_t own = bits[s] >> ((first + at) & 31);
 #pragma unroll
     for (int k = 0; k < V; k++) {
       float& v = value[s * V + k];
-      v = bits >> k & 1 ? v : -__builtin_inff();
+      v = own >> k & 1 ? v : -__builtin_inff();
       if (v > most) { most = v; where = at + k; }
     }
   }
