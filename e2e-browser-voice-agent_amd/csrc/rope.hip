@@ -14,7 +14,6 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
-#include <vector>
 
 #include "rows.h"
 
