@@ -397,11 +397,15 @@ void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* k
   kv->forked = true;
   const unsigned chunks = (unsigned)((v.pages + kKv8Chunk - 1) / kKv8Chunk), all = (unsigned)kForkGrid;
   const size_t entries = (size_t)v.B * v.W;
-  k_kv8_fork_count<<<dim3((unsigned)std::min((v.W + kForkThreads - 1) / kForkThreads, 64), (unsigned)std::min(v.B, 65535)), kForkThreads,
-                     0, s>>>(v, kv->f, from, keep);
-  k_kv8_fork_weigh<<<chunks + 1, kKv8Chunk, 0, s>>>(v, kv->f, keep);
-  k_kv8_fork_commit<<<std::max(chunks, (unsigned)std::min<size_t>((entries + kKv8Chunk - 1) / kKv8Chunk, 512)), kKv8Chunk, 0, s>>>(
-      v, kv->f, keep, tables);
+  if (v.B <= kPlanShared && v.pages <= kForkPages && entries <= (size_t)kForkEntries) {
+    k_kv8_fork_small<<<1, kPlanThreads, 0, s>>>(v, kv->f, from, keep, tables);
+  } else {
+    k_kv8_fork_count<<<dim3((unsigned)std::min((v.W + kForkThreads - 1) / kForkThreads, 64), (unsigned)std::min(v.B, 65535)), kForkThreads,
+                       0, s>>>(v, kv->f, from, keep);
+    k_kv8_fork_weigh<<<chunks + 1, kKv8Chunk, 0, s>>>(v, kv->f, keep);
+    k_kv8_fork_commit<<<std::max(chunks, (unsigned)std::min<size_t>((entries + kKv8Chunk - 1) / kKv8Chunk, 512)), kKv8Chunk, 0, s>>>(
+        v, kv->f, keep, tables);
+  }
   k_kv8_fork_copy<<<(unsigned)std::min<int64_t>((int64_t)v.B * v.layers * v.KVH, all), kForkThreads, 0, s>>>(v, kv->f, keep, tables);
 }
 

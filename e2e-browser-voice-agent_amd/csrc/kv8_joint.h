@@ -11,34 +11,9 @@
 
 namespace q4 {
 
-constexpr int kJointThreads = 1024;
+constexpr int kJointThreads = kPlanThreads;
 // A group has at least so many pages in common.
 constexpr int kJointPages = 8;
-
-// Sums over the threads before, and over all; `store` is shared memory.  Every thread calls it.
-template <int K>
-__device__ inline void kv8_block_scan(uint32_t (&x)[K], uint32_t (&all)[K], uint32_t (*store)[kJointThreads / 64]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t before[K];
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    const uint32_t y = kv8_wave_sums(x[k]);
-    if (lane == 63) store[k][wave] = y;
-    before[k] = y - x[k];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    all[k] = 0;
-    for (int w = 0; w < kJointThreads / 64; w++) {
-      const uint32_t y = store[k][w];
-      before[k] += w < wave ? y : 0;
-      all[k] += y;
-    }
-    x[k] = before[k];
-  }
-  __syncthreads();
-}
 
 constexpr int kJointArrays = 11;
 
@@ -47,7 +22,7 @@ template <bool kShared>
 __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8JointView jv, const int* __restrict__ have,
                                                               const int* __restrict__ add, int* scratch) {
   __shared__ int room[kShared ? kJointArrays : 1][kShared ? kPlanShared : 1];
-  __shared__ uint32_t store[4][kJointThreads / 64];
+  __shared__ uint32_t store[4][kPlanThreads / 64];
   __shared__ int4 chunk[kJointThreads / 4], added[kJointThreads / 4];
   __shared__ unsigned long long pages_all;
   __shared__ int joints_all, most_parts, most_own;      // parts of a group's pages, of a member's own

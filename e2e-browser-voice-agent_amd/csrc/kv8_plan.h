@@ -47,6 +47,31 @@ __device__ __forceinline__ uint64_t kv8_wave_sum(uint64_t x) {
   return all;
 }
 
+// Sums over the threads before, and over all; `store` is shared memory.  All of kPlanThreads threads call it.
+template <int K>
+__device__ inline void kv8_block_scan(uint32_t (&x)[K], uint32_t (&all)[K], uint32_t (*store)[kPlanThreads / 64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t before[K];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const uint32_t y = kv8_wave_sums(x[k]);
+    if (lane == 63) store[k][wave] = y;
+    before[k] = y - x[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    all[k] = 0;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+      const uint32_t y = store[k][w];
+      before[k] += w < wave ? y : 0;
+      all[k] += y;
+    }
+    x[k] = before[k];
+  }
+  __syncthreads();
+}
+
 // The last sequence b with at[b] <= i.
 __device__ inline int find(const int* at, int B, int i) {
   int lo = 0, hi = B;

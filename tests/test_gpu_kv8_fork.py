@@ -79,11 +79,12 @@ def test_answers_to_one_question(hd, KVH, layers, dtype, keep):
     assert len(t.pool.stack) == 40
 
 
-def test_beams_trade_places():
+@pytest.mark.parametrize("max_len,pages", [(300, 21), (50000, 21), (300, 5000)])
+def test_beams_trade_places(max_len, pages):
     """Every sequence becomes another one, at once, again and again; pages of dropped ones serve the copies."""
     rng = np.random.default_rng(3)
     B = 6
-    t = Forked(4, 2, 64, B, 300, 21, 64, 2)
+    t = Forked(4, 2, 64, B, max_len, pages, 64, 2)
     t.grow(rng, [0] * B, [50] + [0] * (B - 1))
     lens = t.fork([0] * B, [50] * B) and [50] * B
     for step in range(30):
@@ -174,16 +175,17 @@ def test_rows_into_a_shared_page():
     t.attend(rng, "f32")
 
 
+@pytest.mark.parametrize("max_len", [100, 90000])          # forked by one workgroup, and by many
 @pytest.mark.parametrize("source,keep,code", [([0, 3, 2], [5, 5, 5], q4hip.EINVAL), ([0, -1, 2], [5, 5, 0], q4hip.EINVAL),
                                               ([0, 1, 0], [5, 0, 71], q4hip.EINVAL), ([1, 1, 1], [1, 0, 0], q4hip.EINVAL),
                                               ([0, 1, 2], [-1, 0, 0], q4hip.EINVAL), ([0, 0, 2], [70, 70, 40], q4hip.ECONTEXT)])
-def test_forks_that_do_not_fit_change_nothing(source, keep, code):
+def test_forks_that_do_not_fit_change_nothing(source, keep, code, max_len):
     rng = np.random.default_rng(5)
-    t = Forked(2, 1, 64, 3, 100, 5, 110)
+    t = Forked(2, 1, 64, 3, max_len, 5, 110)
     t.grow(rng, [0, 0, 0], [70, 0, 40])
     t.pool.plan([70, 0, 40], [0, 0, 0], 0)
     assert t.pool.fork(source, keep) is None
-    f, k, out = ints(source), ints(keep), ints(np.full((3, 4), -7))
+    f, k, out = ints(source), ints(keep), ints(np.full((3, t.pool.W), -7))
     torch.cuda.synchronize()
     t.refused(lambda: t.kv.fork(f.data_ptr(), k.data_ptr(), out.data_ptr()), code)
     assert np.array_equal(out.cpu(), t.pool.table())
