@@ -31,6 +31,9 @@ constexpr int kKv8JointSaves = 5500;
 // Joints of a step at most, which is 8,192 rows of attention of a kv head: two slots of 128 * head_dim bytes a kv head for each.
 constexpr int kKv8Joints = 256;
 constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
+// Pages of all tables at most while some belong to several sequences, each counted for each: so plan's sums over the sequences fit 32
+// bits, where the pool's pages do not bound them.
+constexpr int kKv8Entries = 1 << 30;
 // Sequences that add more than one unit are taken in tiles where these and the units of the others are work for
 // kKv8MinTiles workgroups; else in units, whose pages can be shared.  Tiles and units, us: 2,048 rows of 14 heads (fp32)
 // 57 and 42, 8,192 rows 283 and 370; of 32 heads (bf16) 83 and 84, 773 and 860; of 8 heads of one kv head (bf16) 65 and 32, 262
@@ -58,7 +61,7 @@ struct Kv8Head {
   int joint_items, joints; // items of the list with joints and joints, 0 where there is no such list
   int most_parts;  // of a row in a joint
 };
-enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE, KV8_SHARED, KV8_FORK_SOURCE, KV8_FORK_PAGES };
+enum { KV8_OK, KV8_BAD_LENGTH, KV8_TOO_LONG, KV8_ROWS, KV8_PAGES, KV8_STALE, KV8_SHARED, KV8_FORK_SOURCE, KV8_FORK_PAGES, KV8_ENTRIES };
 
 // What the launches of a fork tell one another.
 struct Kv8Fork {

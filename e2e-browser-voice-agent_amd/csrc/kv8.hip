@@ -272,6 +272,8 @@ int plan_error(const q4hip_kv8* kv, int status) {
       return fail(Q4HIP_EINVAL, "plan: rows into a page that another sequence holds, too: cut the sequence back by a fork first");
     case KV8_FORK_SOURCE: return fail(Q4HIP_EINVAL, "fork: a sequence that there is not, or more positions than it holds");
     case KV8_FORK_PAGES: return fail(Q4HIP_ECONTEXT, "fork: more than the pool's %d pages", kv->v.pages);
+    case KV8_ENTRIES:
+      return fail(Q4HIP_ECONTEXT, "plan or fork: sequences of more than %d pages in all while some share any", kKv8Entries);
     default: return fail(Q4HIP_ECONTEXT, "plan: more than the pool's %d pages", kv->v.pages);
   }
 }

@@ -104,7 +104,8 @@ __global__ __launch_bounds__(kKv8Chunk) void k_kv8_fork_commit(Kv8View v, Kv8For
   }
   free = kv8_block_sum(free, store);
   before = kv8_block_sum(before, store);
-  const int status = w.status ? w.status : w.copies > free ? (int)KV8_FORK_PAGES : (int)KV8_OK;
+  const int status = w.status ? w.status : w.copies > free ? (int)KV8_FORK_PAGES
+                     : w.entries > (uint64_t)kKv8Entries ? (int)KV8_ENTRIES : (int)KV8_OK;
   if (c < chunks) {
     const int64_t page = (int64_t)c * kKv8Chunk + tid;
     const int count = page < v.pages ? v.count()[page] : 1;

@@ -325,7 +325,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   const uint64_t bad = sums[5];
   head.joint_items = head.joints = 0;
   head.status = bad >> 32 ? KV8_TOO_LONG : bad ? KV8_BAD_LENGTH : sums[0] > (uint64_t)rows ? KV8_ROWS
-                : sums[1] > (uint64_t)v.pages && !head.shared ? KV8_PAGES : KV8_OK;
+                : sums[1] <= (uint64_t)(head.shared ? kKv8Entries : v.pages) ? KV8_OK
+                : head.shared ? KV8_ENTRIES : KV8_PAGES;
   int freed = total[0];
   if (__builtin_expect(head.shared && !head.status, 0)) {
     freed = kv8_shared_gone({v.table, v.refs(), v.count(), v.first(), s.free_at, v.B, v.W, total[0]}, kShared ? s.base : have,

@@ -305,7 +305,8 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
  * `stream` NULL the call returns the error, otherwise q4hip_kv8_status does.
  * A plan whose rows would lie in a page that another sequence holds afterwards, too, fails (Q4HIP_EINVAL): only whole pages are shared,
  * so this takes a chat that was cut back to within one, and a fork that cuts it back there (from[b] = b, keep[b] = have[b])
- * makes that page its own. */
+ * makes that page its own.  While any page is shared, the sequences have up to 2^30 pages in all, each counted for each (a fork or plan of
+ * more fails with Q4HIP_ECONTEXT). */
 int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables, void* stream);
 /* Waits for `stream` (NULL: the handle's) and returns the last plan's or fork's error, its rows and the pages left. */
 int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages);
