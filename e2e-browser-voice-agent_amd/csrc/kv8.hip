@@ -326,8 +326,8 @@ void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* a
   }
   if (!fill) k_kv8_fill<<<(unsigned)std::min<size_t>((entries + 255) / 256, 1024), 256, 0, s>>>(v, positions, slots, tables);
   if (!joined(kv, rows)) return;
-  if (shared) k_kv8_joints<true><<<1, kJointThreads, 0, s>>>(v, kv->j, have, add, nullptr);
-  else k_kv8_joints<false><<<1, kJointThreads, 0, s>>>(v, kv->j, have, add, kv->joint_scratch);
+  if (shared) k_kv8_joints<true><<<1, kJointThreads, 0, s>>>(v, kv->j, nullptr);
+  else k_kv8_joints<false><<<1, kJointThreads, 0, s>>>(v, kv->j, kv->joint_scratch);
 }
 
 namespace {

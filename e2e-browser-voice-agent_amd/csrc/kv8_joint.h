@@ -19,8 +19,7 @@ constexpr int kJointArrays = 11;
 
 // kShared: v.B <= kPlanShared, and the arrays are in shared memory, else in `scratch`, [kJointArrays][B].
 template <bool kShared>
-__global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8JointView jv, const int* __restrict__ have,
-                                                              const int* __restrict__ add, int* scratch) {
+__global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8JointView jv, int* scratch) {
   __shared__ int room[kShared ? kJointArrays : 1][kShared ? kPlanShared : 1];
   __shared__ uint32_t store[4][kPlanThreads / 64];
   __shared__ int4 chunk[kJointThreads / 4], added[kJointThreads / 4];
@@ -39,9 +38,12 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   auto in = [](const int* p) { return kShared ? *p : kv8_peek(p); };
   // sums over the sequences before: items and slots of joints, of units
   int *const common_at = array(7), *const common_slot = array(8), *const item_at = array(9), *const slot_at = array(10);
+  // the step's lengths as the plan has taken them: the caller's arrays may be those that it has written to since
+  auto have = [&](int b) { return v.base[b]; };
+  auto add = [&](int b) { return v.lens[b] - v.base[b]; };
   auto page0 = [&](int b) { return v.table[(size_t)b * v.W]; };
   // what a sequence that adds a unit may have in common with others: pages before its rows
-  auto mine = [&](int b) { return add[b] > 0 && add[b] <= v.unit_rows ? have[b] / kKv8Block : 0; };
+  auto mine = [&](int b) { return add(b) > 0 && add(b) <= v.unit_rows ? have(b) / kKv8Block : 0; };
   for (int b = tid; b < B; b += kJointThreads)
     if (mine(b) >= kJointPages) atomicMin(v.first() + page0(b), b);
   __syncthreads();
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   }
   // members in the order of the sequences, 1,024 at a time
   for (int b0 = 0; b0 < B; b0 += kJointThreads) {
-    const int b = b0 + tid, a = b < B ? lead[b] : -1, n = a >= 0 ? add[b] : 0;
+    const int b = b0 + tid, a = b < B ? lead[b] : -1, n = a >= 0 ? add(b) : 0;
     ((int*)chunk)[tid] = a;
     ((int*)added)[tid] = n;
     __syncthreads();
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   uint32_t sum[2] = {};
   for (int b0 = 0; b0 < B; b0 += kJointThreads) {
     const int b = b0 + tid, n = joints_of(b);
-    uint32_t x[2] = {b < B ? (uint32_t)add[b] : 0, (uint32_t)n}, all[2];
+    uint32_t x[2] = {b < B ? (uint32_t)add(b) : 0, (uint32_t)n}, all[2];
     kv8_block_scan(x, all, store);
     if (b < B) {
       start[b] = (int)(sum[0] + x[0]);
@@ -121,10 +123,10 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   // pages that a sequence's units do not look at themselves
   auto skipped = [&](int b) { return lead[b] >= 0 && in(count + lead[b]) ? in(common + lead[b]) : 0; };
   const bool in_tiles = head.tiles > 0;
-  auto units_of = [&](int b) { return in_tiles && kv8_tiles(v, add[b]) ? 0 : kv8_units(v, add[b]); };
+  auto units_of = [&](int b) { return in_tiles && kv8_tiles(v, add(b)) ? 0 : kv8_units(v, add(b)); };
   uint64_t pages = 0;
   for (int b = tid; b < B; b += kJointThreads) {
-    pages += (uint64_t)units_of(b) * (kv8_pages(have[b] + add[b]) - skipped(b));
+    pages += (uint64_t)units_of(b) * (kv8_pages(v.lens[b]) - skipped(b));
     if (in(count + b)) pages += (uint64_t)joints_of(b) * in(common + b);
   }
   pages = kv8_wave_sum(pages);
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
         x[1] = parts > 1 ? x[0] : 0;
         atomicMax(&most_parts, parts);
       }
-      const int parts = kv8_parts(kv8_pages(have[b] + add[b]) - skipped(b), parts_of);
+      const int parts = kv8_parts(kv8_pages(v.lens[b]) - skipped(b), parts_of);
       if (skipped(b)) atomicMax(&most_own, parts);
       x[2] = units_of(b) * parts;
       x[3] = parts > 1 ? x[2] : 0;
@@ -163,8 +165,8 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   for (int b = tid; b < B; b += kJointThreads) {
     const int a = lead[b];
     if (a < 0 || !in(count + a)) continue;
-    const int n = add[b] * G, row0 = joint_at[a] * 32 + before_of[b] * G;
-    const int parts = kv8_parts(kv8_pages(have[b] + add[b]) - skipped(b), parts_of), slot = slots + (int)at[1] + slot_at[b];
+    const int n = add(b) * G, row0 = joint_at[a] * 32 + before_of[b] * G;
+    const int parts = kv8_parts(kv8_pages(v.lens[b]) - skipped(b), parts_of), slot = slots + (int)at[1] + slot_at[b];
     for (int i = 0; i < n; i++) {
       const int r = row0 + i, tok = kv8_div_g(v, i);
       jv.rows[r] = {start[b] + tok, i - tok * G, parts > 1 ? slot : jv.most + (r >> 5), parts, parts > 1 ? i : r & 31, {}};
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
       e.slot = parts > 1 ? slots + common_slot[b] + joint * parts : joint_at[b] + joint;
       e.joint = joint_at[b] + joint + 1;
     } else {
-      const int b = find(item_at, B, i), k = i - item_at[b], h = have[b], more = add[b], skip = skipped(b);
+      const int b = find(item_at, B, i), k = i - item_at[b], h = have(b), more = add(b), skip = skipped(b);
       const int parts = kv8_parts(kv8_pages(h + more) - skip, parts_of), rows = kv8_unit_rows(v, more), u = k / parts;
       e.seq = b;
       e.part = k - u * parts;

@@ -370,8 +370,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv8_plan(Kv8View v, const int*
   for (int b = tid; b < v.B; b += threads) {
     if constexpr (kShared) v.held[b] = kv8_pages(s.lens[b]);
     if (starts_out) starts_out[b] = s.starts[b];
+    if (kShared && (!fill || shared)) v.base[b] = s.base[b];       // shared: for k_kv8_joints
     if (kShared && !fill) {
-      v.base[b] = s.base[b];
       v.starts[b] = s.starts[b];
       v.run_at[b] = s.run_at[b];
       v.item_at[b] = s.item_at[b];
