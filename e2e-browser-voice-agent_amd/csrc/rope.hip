@@ -3,8 +3,9 @@
 // A pair (x, y) of a row at position p becomes a (x cos t - y sin t, y cos t + x sin t), t = p f.  A far position times a
 // frequency needs more than fp32 holds (at p = 10^6 its last bit is 0.06 rad), and a table of cosines for every position
 // would be read beside the rows.  So a frequency is held as a part of a turn in 2^-64 (as a whole number): p f mod 2^64 is the
-// angle without its full turns, exactly but for the frequency's own rounding (2^-65 p turns).  Its upper 32 bits go into sine and
-// cosine: the nearest quarter of a turn by the upper two, the rest, within an eighth, by the power series.
+// angle without its full turns, exactly but for the frequency's own rounding (2^-65 p turns, whatever the frequency).  Its upper 32
+// bits go into sine and cosine, cut off there: the nearest quarter of a turn by the upper two, the rest, within an eighth, as an fp32
+// number by the power series.
 //
 // Bytes bound it: 8,192 rows of 40 heads of 128 (bf16), 168 MB read and written, take 36.1 us, 4.65 TB/s (a 1 GiB copy moves 5.15).
 // A workgroup takes `each` rows: its threads form the cosines and sines of these in shared memory, once for all heads, while
@@ -132,6 +133,28 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_rows(RopeShape sh, const 
   }
 }
 
+// 1 / (2 pi), 64 bits a word: as many as the largest double's part of a turn is formed of.
+constexpr uint64_t kTurns[] = {
+    0x28be60db9391054a, 0x7f09d5f47d4d3770, 0x36d8a5664f10e410, 0x7f9458eaf7aef158, 0x6dc91b8e909374b8, 0x01924bba82746487,
+    0x3f877ac72c4a69cf, 0xba208d7d4baed121, 0x3a671c09ad17df90, 0x4e64758e60d4ce7d, 0x272117e2ef7e4a0e, 0xc7fe25fff7816603,
+    0xfbcbc462d6829b47, 0xdb4d9fb3c9f2c26d, 0xd3d18fd9a797fa8b, 0x5d49eeb1faf97c5e, 0xcf41ce7de294a4ba, 0x9afed7ec47e35742};
+
+// f radians without their full turns, in 2^-64 of a turn, rounded.  |f| = m 2^e, m of 53 bits: of 2^e / (2 pi) the full turns are left
+// out, which m only multiplies, and 128 bits behind the point are taken, so that what is cut off is under 2^-75.
+uint64_t turns_of(double f) {
+  int e;
+  const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(f), &e), 53);
+  e -= 53;
+  auto bits = [](int at) -> uint64_t {       // 64 of 1 / (2 pi) from the one worth 2^-(at + 1)
+    if (at < 0) return at > -64 ? kTurns[0] >> -at : 0;
+    const int w = at / 64, s = at % 64;
+    return s ? kTurns[w] << s | kTurns[w + 1] >> (64 - s) : kTurns[w];
+  };
+  const unsigned __int128 p = (unsigned __int128)bits(e + 64) * m + ((unsigned __int128)(bits(e) * m) << 64);
+  const uint64_t t = (uint64_t)(p >> 64) + ((uint64_t)p >> 63);
+  return f < 0.0 ? -t : t;
+}
+
 uint32_t magic_of(int d) { return d == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); }
 
 }  // namespace
@@ -200,12 +223,7 @@ int q4hip_rope_create(q4hip_rope** out, int head_dim, int rot, int order, const 
   r->pairs = order == Q4HIP_ROPE_PAIRS;
   r->amplitude = amplitude;
   uint64_t turns[Q4HIP_ROPE_MAX_DIM / 2];
-  for (int i = 0; i < rot / 2; i++) {
-    // long double holds the quotient's 64 bits; full turns of a whole position do not count
-    const long double t = (long double)freq[i] / 6.283185307179586476925286766559L;
-    const long double part = t - floorl(t);
-    turns[i] = (uint64_t)(__int128)(part * 18446744073709551616.0L + 0.5L);
-  }
+  for (int i = 0; i < rot / 2; i++) turns[i] = turns_of(freq[i]);
   hipError_t e = hipStreamCreateWithFlags(&r->stream, hipStreamNonBlocking);
   if (e == hipSuccess) e = hipMalloc(&r->turns, (size_t)rot / 2 * sizeof(uint64_t));
   if (e == hipSuccess) e = hipMemcpy(r->turns, turns, (size_t)rot / 2 * sizeof(uint64_t), hipMemcpyHostToDevice);

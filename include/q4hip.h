@@ -337,8 +337,9 @@ int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int typ
  * the pairs (x, y) of the first `rot` columns of a head become, at position p,
  *   amplitude * (x cos a - y sin a,  y cos a + x sin a),   a = p * freq[i] for the i-th pair
  * and the columns behind them stay as they are.  (The engine's own passes turn q and k from a table, engine/kernels.c:337-345;
- * the other orders, parts of heads and stretched contexts have no counterpart there.)  The angle is exact to 2^-32 of
- * a turn at every position of 32 bits; sines, cosines and the sums are fp32, rounded once to the rows' type. */
+ * the other orders, parts of heads and stretched contexts have no counterpart there.)  The angle without its
+ * full turns is off by less than 2^-31 of a turn at every position of 32 bits and every frequency; its distance from the nearest
+ * quarter of a turn, sines, cosines and the sums are fp32, rounded once to the rows' type. */
 typedef struct q4hip_rope q4hip_rope;
 #define Q4HIP_ROPE_MAX_DIM 512
 /* Order of a pair's columns: rot / 2 apart, or neighbours. */
