@@ -228,7 +228,6 @@ int q4hip_logits_create(q4hip_logits** out, int vocab, int max_rows, int device)
   *out = nullptr;
   if (vocab <= 0 || vocab > 1 << 30) return fail(Q4HIP_EINVAL, "a vocabulary of %d", vocab);
   if (max_rows <= 0 || max_rows > 1 << 20) return fail(Q4HIP_EINVAL, "%d rows: up to 2^20", max_rows);
-  // one launch's workgroups
   const int64_t pieces = ((int64_t)vocab + kLargeThreads * kLargeEach - 1) / (kLargeThreads * kLargeEach);
   if (pieces * max_rows > INT32_MAX / 8) return fail(Q4HIP_EINVAL, "%d rows of a vocabulary of %d", max_rows, vocab);
   int ndev = 0;
@@ -290,19 +289,18 @@ int q4hip_logits_run(q4hip_logits* lg, const void* x, void* y, int type, int64_t
   const int large = kLargeThreads * kLargeEach, small = kSmallThreads * kSmallEach;
   const bool in_large = (int64_t)rows * ((V + large - 1) / large) >= kLargeFrom;
   const int size = in_large ? large : small, pieces = (V + size - 1) / size;
-  const LogitsCall c{params, history, biases, mask, history_n, biases_n, mask_rows, V, pieces, words, x_stride, y_stride,
-                     best, lg->best, lg->arrived};
+  const int threads = in_large ? kLargeThreads : kSmallThreads;
   const bool wide = aligned16(x, x_stride, type) && aligned16(y, y_stride, type);
-  const unsigned grid = (unsigned)((int64_t)rows * pieces);
+  const int most = std::max(1, (int)(kMostThreads / threads / pieces));      // rows of a launch
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     constexpr int kVec = 16 / sizeof(T);
-    if (in_large) {
-      auto* fn = wide ? k_logits<T, kVec, kLargeThreads, kLargeEach> : k_logits<T, 1, kLargeThreads, kLargeEach>;
-      fn<<<grid, kLargeThreads, 0, s>>>(c, (const T*)x, (T*)y);
-    } else {
-      auto* fn = wide ? k_logits<T, kVec, kSmallThreads, kSmallEach> : k_logits<T, 1, kSmallThreads, kSmallEach>;
-      fn<<<grid, kSmallThreads, 0, s>>>(c, (const T*)x, (T*)y);
+    auto* fn = in_large ? (wide ? k_logits<T, kVec, kLargeThreads, kLargeEach> : k_logits<T, 1, kLargeThreads, kLargeEach>)
+                        : (wide ? k_logits<T, kVec, kSmallThreads, kSmallEach> : k_logits<T, 1, kSmallThreads, kSmallEach>);
+    for (int64_t r = 0; r < rows; r += most) {
+      const LogitsCall c{params + r, history, biases, mask, history_n, biases_n, mask_rows, V, pieces, words, x_stride, y_stride,
+                         best ? best + r : nullptr, lg->best + r, lg->arrived + r};
+      fn<<<(unsigned)(std::min<int64_t>(most, rows - r) * pieces), threads, 0, s>>>(c, (const T*)x + r * x_stride, (T*)y + r * y_stride);
     }
   });
   HIPCHK(hipGetLastError());

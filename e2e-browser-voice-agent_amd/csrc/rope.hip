@@ -65,12 +65,12 @@ __device__ inline uint32_t div_by(uint32_t i, uint32_t magic) { return magic ? _
 template <class T, bool kPairs, int V>
 __global__ __launch_bounds__(kRopeThreads) void k_rope_rows(RopeShape sh, const T* x, T* y, int64_t x_stride, int64_t y_stride,
                                                             const int* __restrict__ pos, int rows, const int* __restrict__ count,
-                                                            int each) {
+                                                            int first, int each) {
   extern __shared__ float2 cs[];             // [each][rot / 2]
   constexpr int W = kPairs && V == 1 ? 2 : V;      // columns of a turned piece (halves: of each of its two)
   struct alignas(V > 1 ? 16 : sizeof(T)) Vec { T e[W]; };
   const int tid = threadIdx.x, half = sh.rot / 2;
-  const int row0 = blockIdx.x * each;
+  const int row0 = first + blockIdx.x * each;
   if (count) rows = min(rows, *count);
   const int n = min(each, rows - row0);
   if (n <= 0) return;
@@ -274,14 +274,17 @@ int q4hip_rope_run(q4hip_rope* r, const void* x, void* y, int heads, int type, i
   sh.by_chunks = magic_of(sh.chunks);
   sh.by_heads = magic_of(heads);
   const int each = std::max(1, std::min(kRopeRows, rows / 1024));
-  const unsigned grid = (unsigned)((rows + each - 1) / each);
+  const int64_t most = (int64_t)kMostThreads / kRopeThreads * each;      // rows of a launch
   by_type(type, [&](auto zero) {
     using T = decltype(zero);
     constexpr int kVec = 16 / sizeof(T);
     auto* fn = r->pairs ? (wide ? k_rope_rows<T, true, kVec> : k_rope_rows<T, true, 1>)
                         : (wide ? k_rope_rows<T, false, kVec> : k_rope_rows<T, false, 1>);
-    fn<<<grid, kRopeThreads, (size_t)each * half * sizeof(float2), s>>>(sh, (const T*)x, (T*)y, x_stride, y_stride, pos, rows, count,
-                                                                       each);
+    for (int64_t first = 0; first < rows; first += most) {
+      const unsigned grid = (unsigned)((std::min(most, rows - first) + each - 1) / each);
+      fn<<<grid, kRopeThreads, (size_t)each * half * sizeof(float2), s>>>(sh, (const T*)x, (T*)y, x_stride, y_stride, pos, rows, count,
+                                                                         (int)first, each);
+    }
   });
   HIPCHK(hipGetLastError());
   if (!stream) HIPCHK(hipStreamSynchronize(s));

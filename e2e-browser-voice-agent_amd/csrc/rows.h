@@ -6,6 +6,9 @@
 
 namespace q4 {
 
+// Threads of a launch at most: HIP takes less than 2^32.
+constexpr uint32_t kMostThreads = 1u << 31;
+
 inline int elem_size(int type) { return type == Q4HIP_TYPE_F32 ? 4 : 2; }
 
 inline int check_type(int type) {
