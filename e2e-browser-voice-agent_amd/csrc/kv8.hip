@@ -599,6 +599,16 @@ int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages) {
   return plan_error(kv, kv->pin->status);
 }
 
+int q4hip_kv8_shared(q4hip_kv8* kv, void* stream, int* shared, int* joints) {
+  if (!kv) return fail(Q4HIP_EINVAL, "null argument");
+  HIPCHK(hipSetDevice(kv->device));
+  const int rc = read_head(kv, stream ? (hipStream_t)stream : kv->stream);
+  if (rc) return rc;
+  if (shared) *shared = kv->pin->shared != 0;
+  if (joints) *joints = kv->pin->joints;
+  return Q4HIP_OK;
+}
+
 int q4hip_kv8_append(q4hip_kv8* kv, int layer, const void* k, const void* v, int type, int64_t k_stride, int64_t v_stride,
                      void* stream) {
   if (!kv || !k || !v) return fail(Q4HIP_EINVAL, "null argument");

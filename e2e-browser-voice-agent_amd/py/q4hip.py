@@ -39,6 +39,7 @@ EXPORTS = [
     "q4hip_attn_ring_rows", "q4hip_check_ordered_sum", "q4hip_kv8_create", "q4hip_kv8_destroy", "q4hip_kv8_plan",
     "q4hip_batch_create_kv8", "q4hip_batch_release", "q4hip_batch_free_pages", "q4hip_batch_get_kv",
     "q4hip_kv8_status", "q4hip_kv8_append", "q4hip_kv8_read", "q4hip_kv8_attend", "q4hip_kv8_fork",
+    "q4hip_kv8_shared",
     "q4hip_rope_frequencies", "q4hip_rope_create", "q4hip_rope_run", "q4hip_rope_destroy",
     "q4hip_logits_create", "q4hip_logits_run", "q4hip_logits_destroy",
 ]
@@ -102,6 +103,7 @@ def lib() -> ctypes.CDLL:
         "q4hip_kv8_plan": (I, [P, P, P, I, P, P, P, P, P]),
         "q4hip_kv8_fork": (I, [P, P, P, P, P]),
         "q4hip_kv8_status": (I, [P, P, ctypes.POINTER(I), ctypes.POINTER(I)]),
+        "q4hip_kv8_shared": (I, [P, P, ctypes.POINTER(I), ctypes.POINTER(I)]),
         "q4hip_kv8_append": (I, [P, I, P, P, I, I64, I64, P]),
         "q4hip_kv8_read": (I, [P, I, P, P, I, P, P, P]),
         "q4hip_kv8_attend": (I, [P, I, P, P, I, I64, I64, F, P]),
@@ -458,6 +460,12 @@ class Kv8:
         rows, free = ctypes.c_int(0), ctypes.c_int(0)
         _check(lib().q4hip_kv8_status(self.h, stream or None, ctypes.byref(rows), ctypes.byref(free)))
         return rows.value, free.value
+
+    def shared(self, stream: int = 0) -> tuple:
+        """(whether any page belongs to several sequences, joints of the last plan's step)."""
+        shared, joints = ctypes.c_int(0), ctypes.c_int(0)
+        _check(lib().q4hip_kv8_shared(self.h, stream or None, ctypes.byref(shared), ctypes.byref(joints)))
+        return bool(shared.value), joints.value
 
     def append(self, layer: int, k: int, v: int, dtype: int, k_stride: int, v_stride: int, stream: int = 0) -> None:
         """K and V of the step's rows into the cache."""

@@ -310,6 +310,10 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
 int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables, void* stream);
 /* Waits for `stream` (NULL: the handle's) and returns the last plan's or fork's error, its rows and the pages left. */
 int q4hip_kv8_status(q4hip_kv8* kv, void* stream, int* rows, int* free_pages);
+/* Waits alike; *shared: whether any page belongs to several sequences; *joints: of the last plan's step, how many times 32 rows of
+ * attention of a kv head (or what is left of them) are attended to together over pages that their sequences have in common, 0 where every
+ * sequence is by itself. */
+int q4hip_kv8_shared(q4hip_kv8* kv, void* stream, int* shared, int* joints);
 /* K and V of the step's rows, `type` F32, F16 or BF16: row t, kv head g, column d at
  * k[t * k_stride + g * head_dim + d] (strides in elements; the buffers hold the `rows` of the plan).  Of the rows that fall
  * into one page, with the first at offset f of it, and one head: t = max|x| / 127 in fp32, or 0 where that is below
