@@ -173,6 +173,7 @@ struct q4hip_kv8 {
   q4::Kv8JointView j{};
   int* joint_scratch = nullptr;
   bool forked = false;         // whether pages may be shared: a plan makes lists with joints, too
+  bool fork_captured = false;  // a graph may fork at any time
   int device = 0, max_rows = 0;
   int rows = 0;                // rows the last plan was called for, outside of captures
   unsigned long long capture = 0;   // the last capture of a plan, and the rows of that

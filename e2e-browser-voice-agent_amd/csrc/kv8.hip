@@ -305,6 +305,7 @@ bool joined(const q4hip_kv8* kv, int rows) {
 int read_head(q4hip_kv8* kv, hipStream_t s) {
   HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
   HIPCHK(hipStreamSynchronize(s));
+  if (!kv->pin->shared && !kv->fork_captured) kv->forked = false;
   return Q4HIP_OK;
 }
 
@@ -579,6 +580,7 @@ int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables,
   HIPCHK(hipGetLastError());
   // the step is over: nothing is left to append or attend
   if (id) {
+    kv->fork_captured = true;
     kv->capture = id;
     kv->capture_rows = 0;
   } else {

@@ -332,7 +332,9 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
  * of F32, as sums of two fp16 numbers (22 bits); `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
  * the step's are left as they were.  q and out may be columns of the same rows, but not the same ones.
  * Sequences that begin with the same pages (q4hip_kv8_fork) are attended to together: one pass over these pages serves all that add a
- * few rows (16 / (heads / kv_heads) at most).  A captured plan and attend do so if they were captured after the handle's first fork. */
+ * few rows (16 / (heads / kv_heads) at most).  A captured plan and attend do so if they were captured after a fork,
+ * unless a call that waits (a plan or fork without stream, status, shared) has found since that no page is shared any more; after a captured
+ * fork all do. */
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
 
