@@ -23,11 +23,15 @@ constexpr int kKv8Block = 32;
 // sequences of up to 16,000 positions: parts of at most 128 pages 225 us, as long as the aim asks 245.
 constexpr int kKv8Whole = 16, kKv8MinPart = 8, kKv8MaxPart = 128, kKv8MoreItems = 4;
 constexpr int kKv8TileRows = 128;
-// Sequences are attended to together where that saves passes over so many pages of a kv head.  Together and one by one, us:
-// 64 sequences behind 300 positions (32 heads of 8 x 128, 4,000 pages saved) 19.6 and 15.0, behind 1,000 (13,900) 21.0 and 21.8, behind
-// 4,000 (56,000) 33.1 and 54.6; 32 of one to two rows behind 4,100 (12 of 2 x 128, 5,900) 19.1 and 23.0; 8 behind 131,072 (8 of 1 x 128,
-// 24,600) 26.2 and 55; 8 behind 4,000 (14 of 2 x 64, 1,500) 12.7 and 10.2.
-constexpr int kKv8JointSaves = 5500;
+// Sequences are attended to together where that saves passes over so many pages of a kv head, of 128 columns (one of 64 has half the
+// bytes), and kKv8JointRound more for each further round of workgroups that its items take.  Of 2,588 random steps (2 to 256 sequences of 7
+// layouts behind 260 to 16,000 positions, with up to 1,000 of their own) that is 1.0% slower than the better way in each; the pages alone,
+// 5,500 of them, 1.5%, never 36%, always 6%.  Together and one by one, us: 64 sequences (32 heads of 8 x 128), each with up to 40 positions of
+// its own and so in a round more, behind 900 (9,400 pages saved) 20.3 and 16.9, 1,600 (22,400) 23.5 and 25.3, 4,000 (56,000) 29.7
+// and 49.6; with up to 500 of their own, in no round more, behind 700 21.3 and 21.2, 900 21.3 and 23.0; 64 (16 heads of 8 x 64), a round
+// more, behind 1,200 (17,800 of half the bytes) 16.7 and 14.8, 2,400 (36,000) 17.9 and 21.2; 16 (20 of 20 x 64) behind 300 (2,700) 10.8
+// and 11.0, 700 (6,300) 10.9 and 12.7.
+constexpr int kKv8JointSaves = 3000, kKv8JointRound = 8000;
 // Joints of a step at most, which is 8,192 rows of attention of a kv head: two slots of 128 * head_dim bytes a kv head for each.
 constexpr int kKv8Joints = 256;
 constexpr int kKv8Chunk = 1024;     // pages whose free ones a workgroup of fork counts
@@ -151,7 +155,7 @@ struct Kv8JointView {
   Kv8Joint* joints;    // [most]
   Kv8JointRow* rows;   // [most][32]
   int workgroups;      // of attention
-  int saves;           // pages of a kv head that joints have to save
+  int saves;           // as kKv8JointSaves; 0: joints whatever they save
   int* queue;          // items of attention that have been drawn, 0 between launches
   int most;            // joints of a step.  The workspace's slots 0..most-1 are of joints in one part, rows of units in one part lie
                        // in the slots most..2 most-1 (32 each, as in the joints), other slots begin behind them

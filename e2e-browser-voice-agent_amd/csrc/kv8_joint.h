@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
     for (int k = 0; k < 2; k++) sum[k] += all[k];
   }
   __syncthreads();
-  if (!joints_all || (int64_t)saved * v.KVH < jv.saves) return;
+  if (!joints_all) return;
   // pages that a sequence's units do not look at themselves
   auto skipped = [&](int b) { return lead[b] >= 0 && in(count + lead[b]) ? in(common + lead[b]) : 0; };
   const bool in_tiles = head.tiles > 0;
@@ -162,6 +162,9 @@ __global__ __launch_bounds__(kJointThreads) void k_kv8_joints(Kv8View v, Kv8Join
   }
   __syncthreads();
   const int slots = 2 * jv.most, commons = (int)at[0], items = (int)(at[0] + at[2]);
+  // worth it? (kv8.h)
+  const int64_t rounds = ((int64_t)items * v.KVH - 1) / jv.workgroups - ((int64_t)head.items * v.KVH - 1) / jv.workgroups;
+  if (jv.saves && (int64_t)saved * v.KVH * v.HD < 128 * (jv.saves + kKv8JointRound * rounds)) return;
   for (int b = tid; b < B; b += kJointThreads) {
     const int a = lead[b];
     if (a < 0 || !in(count + a)) continue;

@@ -142,3 +142,20 @@ def test_no_joints():
     t.grow(rng, [400] * 8, [1] * 8)
     assert t.kv.shared() == (False, 0)
     t.attend(rng, "f32")
+
+
+@pytest.mark.parametrize("H,KVH,hd,positions,seqs,own,joins", [
+    (16, 8, 64, 1200, 64, 40, False),               # 17,760 pages of 64 columns, 8,880, and a round of workgroups more
+    (16, 8, 64, 1200, 16, 40, False), (16, 8, 64, 1200, 24, 40, True),      # 2,220 and 3,256, no round more
+    (4, 2, 64, 3000, 30, 40, False), (4, 2, 64, 3000, 34, 40, False), (4, 2, 64, 3000, 36, 40, True),     # 2,604, 2,883, 3,069
+    (4, 2, 64, 3000, 20, 40, False), (4, 2, 128, 3000, 20, 40, True),       # 1,674, 3,348
+    (16, 1, 64, 300, 2, 5, False)])
+def test_what_it_has_to_save(monkeypatch, H, KVH, hd, positions, seqs, own, joins):
+    """Pages of 128 columns: 3,000, and 8,000 for each further round of 512 items."""
+    monkeypatch.delenv("Q4HIP_KV8_JOINT_SAVES")
+    rng = np.random.default_rng(positions)
+    t, lens = grown(rng, H, KVH, hd, [(positions, seqs)], "bf16", own=own)
+    t.grow(rng, lens, [1] * seqs, "bf16")
+    want = joints_of(t)
+    assert want and t.kv.shared() == (True, want if joins else 0)
+    t.attend(rng, "bf16")
