@@ -125,7 +125,7 @@ struct Kv8View {
   float2* scales;      // [layers][pages][kv_heads] of K, V
   int* table;          // [seqs][blocks] pages, -1 past those a sequence holds
   int* held;           // [seqs] pages of a sequence
-  int* stack;          // [4][pages]: free pages, the next one to take last; refs(), count(), first()
+  int* stack;          // [4][pages]: free pages, the next one to take last; refs(), count(), first() (of a cache that forks)
   Kv8Head* head;
   int *base, *lens;    // [seqs] positions before and after the step
   int* starts;         // [seqs + 1] first row of a sequence in the step
@@ -187,6 +187,10 @@ struct q4hip_kv8 {
 };
 
 namespace q4 {
+
+// q4hip_kv8_create; a cache that is never forked (forks false) has no memory for that.
+int kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages, int max_rows,
+               int device, bool forks);
 
 // The operators' launches without the checks of their arguments (include/q4hip.h); q and out, k and v of `type`; rows: of the plan.
 void kv8_launch_plan(q4hip_kv8* kv, hipStream_t s, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,

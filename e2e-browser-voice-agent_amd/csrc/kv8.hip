@@ -237,8 +237,10 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v, Kv8ForkView f) {
   if (i < (size_t)v.B * v.W) v.table[i] = -1;
   if (i < (size_t)v.pages) {
     v.stack[i] = v.pages - 1 - (int)i;
-    v.count()[i] = 0;
-    v.first()[i] = INT32_MAX;
+    if (f.fork) {
+      v.count()[i] = 0;
+      v.first()[i] = INT32_MAX;
+    }
   }
   if (i <= (size_t)v.B) {
     v.starts[i] = 0;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(256) void k_kv8_reset(Kv8View v, Kv8ForkView f) {
   }
   if (i == 0) {
     *v.head = Kv8Head{KV8_OK, 0, v.pages, 0, 0, 0, 1, 0, 0, 0, 0};
-    *f.fork = Kv8Fork{};
+    if (f.fork) *f.fork = Kv8Fork{};
   }
 }
 
@@ -420,28 +422,8 @@ void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, co
   else k_kv8_read<128><<<grid, 256, 0, s>>>(w, layer, seq, pos, n, k, v);
 }
 
-}  // namespace q4
-
-using namespace q4;
-
-extern "C" {
-
-void q4hip_kv8_destroy(q4hip_kv8* kv) {
-  if (!kv) return;
-  (void)hipSetDevice(kv->device);
-  if (kv->stream) (void)hipStreamSynchronize(kv->stream);
-  Kv8View& v = kv->v;
-  void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
-                  kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived,
-                  kv->j.items, kv->j.joints, kv->j.rows, kv->j.queue, kv->joint_scratch};
-  for (void* p : bufs) if (p) (void)hipFree(p);
-  if (kv->pin) (void)hipHostFree(kv->pin);
-  if (kv->stream) (void)hipStreamDestroy(kv->stream);
-  delete kv;
-}
-
-int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages,
-                     int max_rows, int device) {
+int kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages, int max_rows,
+               int device, bool forks) {
   if (!out) return fail(Q4HIP_EINVAL, "null argument");
   *out = nullptr;
   if (layers <= 0 || heads <= 0 || kv_heads <= 0 || seqs <= 0 || max_len <= 0 || pages <= 0 || max_rows <= 0)
@@ -481,11 +463,13 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   al(&v.scales, blocks);
   al(&v.table, (size_t)seqs * v.W);
   al(&v.held, seqs);
-  al(&v.stack, (size_t)4 * pages);
-  al(&kv->f.next, (size_t)seqs * v.W);
-  al(&kv->f.copies, seqs);
-  al(&kv->f.chunk, (pages + kKv8Chunk - 1) / kKv8Chunk);
-  al(&kv->f.fork, 1);
+  al(&v.stack, (size_t)(forks ? 4 : 1) * pages);
+  if (forks) {
+    al(&kv->f.next, (size_t)seqs * v.W);
+    al(&kv->f.copies, seqs);
+    al(&kv->f.chunk, (pages + kKv8Chunk - 1) / kKv8Chunk);
+    al(&kv->f.fork, 1);
+  }
   al(&v.head, 1);
   al(&v.base, seqs);
   al(&v.lens, seqs);
@@ -494,7 +478,7 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   const size_t most_items = (size_t)kKv8MoreItems * v.items_aim;      // beyond one for each unit
   al(&v.items, max_rows + most_items);
   al(&v.tiles, tiles_bound(v, max_rows));
-  if (seqs > 1 && G <= 16) {
+  if (forks && seqs > 1 && G <= 16) {
     // the rows of groups of two and more, in whole joints
     kv->j.most = (int)std::min<int64_t>(((int64_t)seqs * v.unit_rows * G + 31) / 32 + seqs / 2, kKv8Joints);
     al(&kv->j.items, max_rows + most_items + kv->j.most);
@@ -529,6 +513,31 @@ int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int h
   }
   *out = kv;
   return Q4HIP_OK;
+}
+
+}  // namespace q4
+
+using namespace q4;
+
+extern "C" {
+
+void q4hip_kv8_destroy(q4hip_kv8* kv) {
+  if (!kv) return;
+  (void)hipSetDevice(kv->device);
+  if (kv->stream) (void)hipStreamSynchronize(kv->stream);
+  Kv8View& v = kv->v;
+  void* bufs[] = {v.codes, v.scales, v.table, v.held, v.stack, v.head, v.base, v.lens, v.starts, v.free_at, v.take_at,
+                  kv->f.next, kv->f.copies, kv->f.chunk, kv->f.fork, v.run_at, v.item_at, v.part_at, v.tile_at, v.runs, v.items, v.tiles, v.part_o, v.part_ml, v.arrived,
+                  kv->j.items, kv->j.joints, kv->j.rows, kv->j.queue, kv->joint_scratch};
+  for (void* p : bufs) if (p) (void)hipFree(p);
+  if (kv->pin) (void)hipHostFree(kv->pin);
+  if (kv->stream) (void)hipStreamDestroy(kv->stream);
+  delete kv;
+}
+
+int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages,
+                     int max_rows, int device) {
+  return kv8_create(out, layers, heads, kv_heads, head_dim, seqs, max_len, pages, max_rows, device, true);
 }
 
 int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int* starts, int* positions, int* slots,

@@ -3599,7 +3599,7 @@ static int create_batch(q4hip_batch** out, q4hip* h, int B, int pages) {
   if (pages) {
     bt->pages = pages;
     bt->len.assign(B, 0);
-    const int rc = q4hip_kv8_create(&bt->kv8, h->NL, h->H, h->KVH, h->HD, B, h->ctx, pages, std::max(h->MT, h->ctx), h->device);
+    const int rc = kv8_create(&bt->kv8, h->NL, h->H, h->KVH, h->HD, B, h->ctx, pages, std::max(h->MT, h->ctx), h->device, false);
     if (rc != Q4HIP_OK) {
       q4hip_batch_destroy(bt);
       return rc;

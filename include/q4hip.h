@@ -273,7 +273,9 @@ int q4hip_mv_run_noalloc(q4hip_mv* m, const float* x, float* y, void* stream);
 typedef struct q4hip_kv8 q4hip_kv8;
 #define Q4HIP_KV8_BLOCK 32
 /* A cache of `pages` pages for `seqs` sequences of up to max_len positions; plans hold up to max_rows
- * rows.  head_dim is 64 or 128, heads a multiple of kv_heads. */
+ * rows.  head_dim is 64 or 128, heads a multiple of kv_heads.  Beside the pages, and parts of sums that attention keeps, a cache of several
+ * sequences holds up to 256 * head_dim bytes for each kv head and sequence (of 256 sequences at most: 67 MB of 8 x 128) for attending to
+ * shared pages, and forks' scratch memory, 4 bytes for each entry of `tables` and 12 for each page. */
 int q4hip_kv8_create(q4hip_kv8** out, int layers, int heads, int kv_heads, int head_dim, int seqs, int max_len, int pages,
                      int max_rows, int device);
 void q4hip_kv8_destroy(q4hip_kv8* kv);
