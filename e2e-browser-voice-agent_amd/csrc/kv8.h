@@ -203,7 +203,6 @@ void kv8_launch_append_rope(q4hip_kv8* kv, hipStream_t s, int layer, float* qkv,
                             int rows);
 void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, void* out, int type, int64_t q_stride,
                        int64_t out_stride, float scale, int rows);
-void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables);
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v);
 
 }  // namespace q4

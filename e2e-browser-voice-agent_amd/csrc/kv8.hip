@@ -397,12 +397,14 @@ void kv8_launch_attend(q4hip_kv8* kv, hipStream_t s, int layer, const void* q, v
   });
 }
 
-void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables) {
+namespace {
+
+void launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables) {
   const Kv8View& v = kv->v;
   kv->forked = true;
   const unsigned chunks = (unsigned)((v.pages + kKv8Chunk - 1) / kKv8Chunk), all = (unsigned)kForkGrid;
   const size_t entries = (size_t)v.B * v.W;
-  if (v.B <= kPlanShared && v.pages <= kForkPages && entries <= (size_t)kForkEntries) {
+  if (v.B <= kPlanShared && v.pages <= kForkPages && entries + kForkEach * v.B <= (size_t)kForkEntries) {
     k_kv8_fork_small<<<1, kPlanThreads, 0, s>>>(v, kv->f, from, keep, tables);
   } else {
     k_kv8_fork_count<<<dim3((unsigned)std::min((v.W + kForkThreads - 1) / kForkThreads, 64), (unsigned)std::min(v.B, 65535)), kForkThreads,
@@ -413,6 +415,8 @@ void kv8_launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* k
   }
   k_kv8_fork_copy<<<(unsigned)std::min<int64_t>((int64_t)v.B * v.layers * v.KVH, all), kForkThreads, 0, s>>>(v, kv->f, keep, tables);
 }
+
+}  // namespace
 
 void kv8_launch_read(q4hip_kv8* kv, hipStream_t s, int layer, const int* seq, const int* pos, int n, float* k, float* v) {
   const Kv8View& w = kv->v;
@@ -585,7 +589,7 @@ int q4hip_kv8_fork(q4hip_kv8* kv, const int* from, const int* keep, int* tables,
   unsigned long long id;
   rc = capture_of(s, &id);
   if (rc) return rc;
-  kv8_launch_fork(kv, s, from, keep, tables);
+  launch_fork(kv, s, from, keep, tables);
   HIPCHK(hipGetLastError());
   // the step is over: nothing is left to append or attend
   if (id) {

@@ -148,9 +148,11 @@ __global__ __launch_bounds__(kKv8Chunk) void k_kv8_fork_commit(Kv8View v, Kv8For
   }
 }
 
-// Up to this many pages, and entries of all tables, one workgroup counts, weighs and commits: two launches less
-// (4 sequences of 301 positions, with two reads, 20.7 us for 28.4).
-constexpr int kForkPages = 4 * kPlanThreads, kForkEntries = 8192;
+// Up to this many pages, and entries of all tables with kForkEach more for each sequence, one workgroup counts, weighs and commits: two
+// launches less, but what many do at once one after the other.  By one and by many, a call with its copies, us: 4 sequences of 11 entries
+// 7.3 and 16.1, of 1,000 13.7 and 15.9, of 2,048 17.0 and 15.8; 64 of 64 11.9 and 16.4, of 128 17.7 and 16.9; 256 of 8 14.4 and 18.0,
+// of 16 20.0 and 17.5; 1,000 of 4 30.1 and 25.0.
+constexpr int kForkPages = 4 * kPlanThreads, kForkEntries = 6144, kForkEach = 16;
 
 // v.B <= kPlanShared.  A thread has a sequence, and four pages.
 __global__ __launch_bounds__(kPlanThreads) void k_kv8_fork_small(Kv8View v, Kv8ForkView f, const int* __restrict__ from,
