@@ -296,9 +296,10 @@ int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
   return rc;
 }
 
-// Whether a step's units may be joined, if the plan finds that it is worth it: then there is a launch more, which costs 2.5 us where it
-// is not (4 answers of 14 heads, 2 x 64, behind 300 positions 5.9 us without and 11.7 together, behind 32,000 13.3 and 14.1).  More than 16
-// rows of a kv head fill the matrix cores by themselves.
+// Whether a step's units may be joined, if the plan finds that it is worth it (no length is known here): then there is a launch more, which
+// costs 2.5 us where it is not.  Steps of few rows, which are mostly short, are not.  One by one and together, us: 4 answers of 14 heads
+// (2 x 64) behind 300 positions 6.2 and 12.0, behind 32,000 12.9 and 13.9; 12 of 20 heads (20 x 64) behind 300 6.4 and 10.5, behind 2,000
+// 11.5 and 11.4, but behind 16,000 50 and 16; 4 of 32 heads (8 x 128) behind 300 7.2 and 12.0, behind 16,000 20 and 15.
 bool joined(const q4hip_kv8* kv, int rows) {
   const int G = kv->v.H / kv->v.KVH;
   return kv->forked && kv->j.most && rows > 1 && ((int64_t)rows * G > 32 || (int64_t)rows * kv->v.H >= 256 || !kv->j.saves);

@@ -4,8 +4,9 @@
 // have the same pages before it.  So a group is the units (sequences that add up to a unit's rows) with the same first page, and
 // what they have in common with the first of them is found by search and not by comparing.  The group's rows of attention, unit
 // after unit, are joints of 32 (kv8.h).  Their pages, like a long unit's, may be shared among workgroups.
-// One workgroup does it in one launch behind the plan, once for all layers; the members' order is the sequences', whatever the
-// atomics' order was.  Where nothing is shared, or too little, there is no such list, and attention takes the plan's.
+// One workgroup does it in one launch behind the plan, once for all layers (32 sequences 14 us, 128 with joints in 256 parts 25); the
+// members' order is the sequences', whatever the atomics' order was.  Where nothing is shared, or too little, there is no such list, and
+// attention takes the plan's.
 #pragma once
 #include "kv8_plan.h"
 

@@ -155,6 +155,8 @@ __device__ __forceinline__ void kv8_fill(const Kv8View& v, const Kv8Sums& s, con
 // Which pages a step gives back while some belong to several sequences: those that all of their holders give up, at the place of
 // the first of them.  Entry i of the `gone` ones (sequences in order, their pages in order; at[b] counts those before) is in first()
 // and count() until kv8_shared_done().
+// One workgroup goes over them, three times and with a bisection each: 6 to 12 ns an entry.  Half of 128 sequences behind 14,500 positions
+// end in 0.27 ms, half of 1,024 behind 8,000 in 0.76, half of 64 behind 131,072 in 1.05; a plan by which none ends takes 9 to 14 us.
 // Both are calls, with what they need by value: within the kernel they cost every plan 0.25 us of 6.0, so 0.1.
 struct Kv8Gone {
   int *table, *refs, *count, *first;

@@ -7,7 +7,7 @@
 // bits go into sine and cosine, cut off there: the nearest quarter of a turn by the upper two, the rest, within an eighth, as an fp32
 // number by the power series.
 //
-// Bytes bound it: 8,192 rows of 40 heads of 128 (bf16), 168 MB read and written, take 36.1 us, 4.65 TB/s (a 1 GiB copy moves 5.15).
+// Bytes bound it: 8,192 rows of 40 heads of 128 (bf16), 168 MB read and written, take 36.0 us, 4.67 TB/s (a 1 GiB copy moves 5.18).
 // A workgroup takes `each` rows: its threads form the cosines and sines of these in shared memory, once for all heads, while
 // the first 16 bytes of each thread are on their way; then every thread takes 16 bytes (halves: and those rot / 2 columns later) at a time.
 #include <hip/hip_runtime.h>

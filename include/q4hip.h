@@ -333,10 +333,10 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
  * Scores, the softmax and the sums are fp32, whatever the type and the number of rows; the matrix products take the weights, and q
  * of F32, as sums of two fp16 numbers (22 bits); `out` is rounded once.  scale 0: head_dim^-1/2.  Rows of `out` behind
  * the step's are left as they were.  q and out may be columns of the same rows, but not the same ones.
- * Sequences that begin with the same pages (q4hip_kv8_fork) are attended to together: one pass over these pages serves all that add a
- * few rows (16 / (heads / kv_heads) at most).  A captured plan and attend do so if they were captured after a fork,
- * unless a call that waits (a plan or fork without stream, status, shared) has found since that no page is shared any more; after a captured
- * fork all do. */
+ * Sequences that begin with the same page (q4hip_kv8_fork) are attended to together where that saves enough: one pass over the pages that
+ * all of those that add a few rows (16 / (heads / kv_heads) at most, for up to 16 heads to a kv head) have in common, 8 at least, serves them.
+ * A captured plan and attend do so if they were captured after a fork, unless a call that waits (a plan or fork without stream, status,
+ * shared) has found since that no page is shared any more; after a captured fork all do. */
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
 
@@ -382,7 +382,8 @@ void q4hip_rope_destroy(q4hip_rope* r);
  *   c > 0 occurrences in the row's history:  x = x > 0 ? x / repetition : x * repetition;  x = x - (frequency * c + presence)
  *   biases of the row with this token:       x = x + value of the last one
  *   bit v % 32 of word v / 32 of the row's mask is 0:  x = -infinity
- * rounded once to the rows' type.  Entries of lists that name no token of the vocabulary count for nothing. */
+ * rounded once to the rows' type.  Entries of lists that name no token of the vocabulary count for nothing.  The three penalties count
+ * the same entries of the history. */
 typedef struct q4hip_logits q4hip_logits;
 typedef struct {
   float repetition, presence, frequency;   /* 1, 0 and 0 change nothing */
