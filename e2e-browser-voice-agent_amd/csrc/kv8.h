@@ -176,8 +176,10 @@ struct q4hip_kv8 {
   q4::Kv8ForkView f{};
   q4::Kv8JointView j{};
   int* joint_scratch = nullptr;
-  bool forked = false;         // whether pages may be shared: a plan makes lists with joints, too
-  bool fork_captured = false;  // a graph may fork at any time
+  // Whether pages may be shared, so that a plan makes lists with joints, too: there was a fork, and no call that waits has found since that
+  // none is.  A graph may be replayed after other forks, and fork at any time itself.
+  bool forked = false, unshared = false, fork_captured = false;
+  bool capturing = false;      // the call on its way
   int device = 0, max_rows = 0;
   int rows = 0;                // rows the last plan was called for, outside of captures
   unsigned long long capture = 0;   // the last capture of a plan, and the rows of that

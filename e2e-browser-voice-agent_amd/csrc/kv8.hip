@@ -289,9 +289,10 @@ int capture_of(hipStream_t s, unsigned long long* id) {
 }
 
 // Rows of the plan that a call on `s` follows: the one captured before it in the same capture, else the last one outside of any.
-int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
+int rows_on(q4hip_kv8* kv, hipStream_t s, int* rows) {
   unsigned long long id;
   const int rc = capture_of(s, &id);
+  kv->capturing = !rc && id;
   *rows = id && id == kv->capture ? kv->capture_rows : kv->rows;
   return rc;
 }
@@ -302,13 +303,14 @@ int rows_on(const q4hip_kv8* kv, hipStream_t s, int* rows) {
 // 11.5 and 11.4, but behind 16,000 50 and 16; 4 of 32 heads (8 x 128) behind 300 7.2 and 12.0, behind 16,000 20 and 15.
 bool joined(const q4hip_kv8* kv, int rows) {
   const int G = kv->v.H / kv->v.KVH;
-  return kv->forked && kv->j.most && rows > 1 && ((int64_t)rows * G > 32 || (int64_t)rows * kv->v.H >= 256 || !kv->j.saves);
+  const bool shared = kv->forked && (!kv->unshared || kv->capturing || kv->fork_captured);
+  return shared && kv->j.most && rows > 1 && ((int64_t)rows * G > 32 || (int64_t)rows * kv->v.H >= 256 || !kv->j.saves);
 }
 
 int read_head(q4hip_kv8* kv, hipStream_t s) {
   HIPCHK(hipMemcpyAsync(kv->pin, kv->v.head, sizeof(Kv8Head), hipMemcpyDeviceToHost, s));
   HIPCHK(hipStreamSynchronize(s));
-  if (!kv->pin->shared && !kv->fork_captured) kv->forked = false;
+  if (!kv->pin->shared) kv->unshared = true;
   return Q4HIP_OK;
 }
 
@@ -403,6 +405,7 @@ namespace {
 void launch_fork(q4hip_kv8* kv, hipStream_t s, const int* from, const int* keep, int* tables) {
   const Kv8View& v = kv->v;
   kv->forked = true;
+  kv->unshared = false;
   const unsigned chunks = (unsigned)((v.pages + kKv8Chunk - 1) / kKv8Chunk), all = (unsigned)kForkGrid;
   const size_t entries = (size_t)v.B * v.W;
   if (v.B <= kPlanShared && v.pages <= kForkPages && entries + kForkEach * v.B <= (size_t)kForkEntries) {
@@ -562,6 +565,7 @@ int q4hip_kv8_plan(q4hip_kv8* kv, const int* have, const int* add, int rows, int
   unsigned long long id;
   int rc = capture_of(s, &id);
   if (rc) return rc;
+  kv->capturing = id != 0;
   kv8_launch_plan(kv, s, have, add, rows, starts, positions, slots, tables);
   HIPCHK(hipGetLastError());
   if (id) {

@@ -335,8 +335,7 @@ int q4hip_kv8_read(q4hip_kv8* kv, int layer, const int* seq, const int* pos, int
  * the step's are left as they were.  q and out may be columns of the same rows, but not the same ones.
  * Sequences that begin with the same page (q4hip_kv8_fork) are attended to together where that saves enough: one pass over the pages that
  * all of those that add a few rows (16 / (heads / kv_heads) at most, for up to 16 heads to a kv head) have in common, 8 at least, serves them.
- * A captured plan and attend do so if they were captured after a fork, unless a call that waits (a plan or fork without stream, status,
- * shared) has found since that no page is shared any more; after a captured fork all do. */
+ * A captured plan and attend do so if they were captured after the handle's first fork. */
 int q4hip_kv8_attend(q4hip_kv8* kv, int layer, const void* q, void* out, int type, int64_t q_stride, int64_t out_stride,
                      float scale, void* stream);
 

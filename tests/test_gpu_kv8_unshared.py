@@ -4,6 +4,7 @@ import ctypes
 import numpy as np
 import pytest
 import torch
+from torch.profiler import ProfilerActivity, profile
 
 import q4hip
 from test_gpu_kv8 import ints
@@ -14,7 +15,16 @@ pytestmark = pytest.mark.gpu
 
 
 def launches(call):
-    """Nodes of a graph that holds the call."""
+    """Kernels of the cache that a call launches."""
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        call(0)
+        torch.cuda.synchronize()
+    return sum("k_kv8" in e.name for e in p.events())
+
+
+def captured(call):
+    """The same of a graph that holds the call."""
     hip, s = q4hip.lib(), torch.cuda.Stream()
     stream, graph, n = ctypes.c_void_p(s.cuda_stream), ctypes.c_void_p(), ctypes.c_size_t(0)
     assert hip.hipStreamBeginCapture(stream, 2) == 0
@@ -51,7 +61,12 @@ class Chats:
         self.lens = list(keep)
 
     def of(self):
+        """Launches of the last plan, again, and of its attention."""
+        self.h.copy_(ints(self.t.have))
         return launches(self.plan), launches(self.attend)
+
+    def captured(self):
+        return captured(self.plan), captured(self.attend)
 
 
 def test_until_nothing_is_shared():
@@ -59,9 +74,10 @@ def test_until_nothing_is_shared():
     c.grow()
     before = c.of()
     assert before[1] == 1
+    assert c.captured() == before
     c.fork(list(range(c.B)), [280] * c.B)            # cut back: nothing is shared
     c.grow()
-    assert c.of() == before
+    assert c.of() == before and c.captured() == (before[0] + 1, 2)      # a graph may be replayed after other forks
     c.fork([0] * 6, [281] * 6)
     c.grow()
     assert c.of() == (before[0] + 1, 2) and c.t.kv.shared() == (True, 1)
@@ -100,11 +116,10 @@ def test_without_a_call_that_waits():
     f, k = ints([0] * 6), ints([280] * 6)
     torch.cuda.synchronize()
     c.t.kv.fork(f.data_ptr(), k.data_ptr(), 0, s.cuda_stream)
-    assert c.of() == (before[0] + 1, 0)              # no step, nothing to attend to
+    assert launches(c.attend) == 0                   # no step, nothing to attend to
     c.h.copy_(k)
-    torch.cuda.synchronize()
-    c.plan(s.cuda_stream)
-    assert c.of() == (before[0] + 1, 2)
+    assert launches(lambda _: c.plan(s.cuda_stream)) == before[0] + 1
+    assert launches(lambda _: c.attend(s.cuda_stream)) == 2
     assert c.t.kv.shared(s.cuda_stream) == (True, 1)
 
 
